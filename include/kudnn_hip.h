@@ -59,7 +59,8 @@ enum {
     KUDNN_DT_BF16 = 3,
     KUDNN_DT_S32 = 4,
     KUDNN_DT_S8 = 5,
-    KUDNN_DT_U8 = 6
+    KUDNN_DT_U8 = 6,
+    KUDNN_DT_F8E4M3 = 7  /* OCP e4m3 (largest 448, no infinities); kudnn_linear_fp8_* only, no KuDNN counterpart */
 };
 
 /* Layouts: values == KuDNN::Layout (kudnn_layout.hpp:19-51); letters name logical dims listed from the
@@ -117,6 +118,10 @@ typedef struct kudnn_gemm_plan *kudnn_gemm_t;
 typedef struct kudnn_linear_act_plan *kudnn_linear_act_t;
 typedef struct kudnn_linear_res_plan *kudnn_linear_res_t;
 typedef struct kudnn_linear_postops_plan *kudnn_linear_postops_t;
+typedef struct kudnn_moe_route_plan *kudnn_moe_route_t;
+typedef struct kudnn_grouped_linear_plan *kudnn_grouped_linear_t;
+typedef struct kudnn_linear_fp8_plan *kudnn_linear_fp8_t;
+typedef struct kudnn_moe_combine_plan *kudnn_moe_combine_t;
 
 /* ---- library ------------------------------------------------------------------------------------ */
 
@@ -236,6 +241,102 @@ KUDNN_HIP_API int kudnn_linear_postops_destroy(kudnn_linear_postops_t plan);
 KUDNN_HIP_API int kudnn_linear_postops_run_noalloc(kudnn_linear_postops_t plan, const void *a, const void *b,
                                                    void *y, const void *bias, const void *src, float gamma,
                                                    void *stream);
+
+/* ---- mixture of experts ---------------------------------------------------------------------------- */
+/* Extensions with no reference counterpart: the router, the experts' Linear products over ragged groups of rows, the
+ * 8-bit products with a scale for each block of 128, and the weighted sum of a token's experts.
+ *
+ * Conventions of this section: every buffer is device memory (host pointers: KUDNN_STATUS_BAD_ARGUMENTS); the calls are
+ * asynchronous on `stream`, allocate nothing and hold no state, so a plan may run on any number of streams at once and
+ * under graph capture. A workspace, where one is asked for, is the caller's: at least *_workspace_bytes bytes, 16-byte
+ * aligned, used until the run's work on the stream is done. A dimension of zero is accepted where it leaves nothing to
+ * compute. "AB" rows may be strided (row pitch >= the row's length).
+ *
+ * The order by expert. A batch of T tokens with k experts each makes up to R = T * k rows. Sorted by expert, and within an
+ * expert by token, they are described by
+ *   offsets s32[E + 1]  expert e has the rows offsets[e] .. offsets[e + 1] - 1 (offsets[0] = 0);
+ *   rows    s32[R]      the token of each row, -1 past offsets[E];
+ *   slots   s32[T * k]  the row of each of a token's experts, -1 where it has none.
+ * Values outside their range are read as "none": no call reads or writes outside its buffers for any contents. */
+
+/* Router: softmax over each token's open experts, and the top_k of them by logit, ties to the lowest index.
+ * logits {T, E} AB, f32 / bf16 / f16, E <= 1024. mask (may be NULL) {T or 1, E or 1} u8: an expert is open where it is
+ * non-zero and the logit is not -infinity; a NaN or infinity in a closed place is not looked at. An open NaN counts as
+ * the largest value and makes the row's weights NaN, as the softmax does. normalize: weights are divided by the sum over
+ * the chosen ones. A token with fewer than top_k open experts has expert -1, weight 0 and slot -1 in the places left.
+ * Sums are in f32; the result does not depend on the order in which workgroups run. 1 <= top_k <= min(E, 32),
+ * T * top_k < 2^31. */
+KUDNN_HIP_API int kudnn_moe_route_create(const kudnn_tensor_desc *logits, const kudnn_tensor_desc *mask, int top_k,
+                                         int normalize, kudnn_moe_route_t *plan);
+KUDNN_HIP_API int64_t kudnn_moe_route_workspace_bytes(kudnn_moe_route_t plan);
+/* weights f32[T][k], experts s32[T][k] (by falling logit), offsets, rows, slots as above. */
+KUDNN_HIP_API int kudnn_moe_route_run(kudnn_moe_route_t plan, const void *logits, const void *mask, float *weights,
+                                      int32_t *experts, int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                                      void *stream);
+/* Gradient of the weights' inputs: dlogits {T, E} dense, of the logits' type, from dweights f32[T][k] and what the run
+ * gave. Without normalize, p (d - sum d p) over the whole softmax, which is formed again from the logits; with it, the same
+ * over the chosen experts alone. */
+KUDNN_HIP_API int kudnn_moe_route_backward(kudnn_moe_route_t plan, const void *logits, const void *mask,
+                                           const float *weights, const int32_t *experts, const float *dweights,
+                                           void *dlogits, void *stream);
+KUDNN_HIP_API int kudnn_moe_route_destroy(kudnn_moe_route_t plan);
+
+/* Grouped Linear: y[r] = x[r] x w[e] for the rows r of expert e. x {S, K} AB, w {E, K, N} ACB (each expert's weight
+ * physically [N][K], as nn.Linear holds it), y {R, N} AB; one type, bf16 or f16; f32 accumulation, one rounding. gather != 0:
+ * row r takes x[rows[r]], else S == R and it takes x[r]. Rows past offsets[E] are
+ * zero; a row whose token is out of range is taken as zeros. R < 2^31. */
+KUDNN_HIP_API int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc *w,
+                                              const kudnn_tensor_desc *y, int gather, kudnn_grouped_linear_t *plan);
+KUDNN_HIP_API int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const void *x, const void *w,
+                                           const int32_t *offsets, const int32_t *rows, void *y, void *stream);
+/* dx[r] = dy[r] x w[e]^T, {R, K} dense in the experts' order (with gather, a token's gradient is the sum over its slots:
+ * kudnn_moe_combine_run with NULL weights). */
+KUDNN_HIP_API int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void *dy, const void *w,
+                                                      const int32_t *offsets, void *dx, void *stream);
+/* dw[e] = sum over the rows r of expert e of dy[r] x[r]^T, dense [E][N][K]; zero for an expert without rows. */
+KUDNN_HIP_API int kudnn_grouped_linear_backward_weight(kudnn_grouped_linear_t plan, const void *dy, const void *x,
+                                                       const int32_t *offsets, const int32_t *rows, void *dw,
+                                                       void *stream);
+KUDNN_HIP_API int kudnn_grouped_linear_destroy(kudnn_grouped_linear_t plan);
+
+/* Block scales. A row's block of 128 columns is held as e4m3 values q = round(x / s), s = max(amax / 448, 2^-126) in f32
+ * (division and rounding to nearest even); a weight's block is 128 x 128. The last blocks of a row or column may be short.
+ * kudnn_quantize_rows: x {M, K} AB, f32 / bf16 / f16 -> q e4m3 [M][K] with row pitch ldq (bytes, >= K; columns K .. ldq - 1
+ * are not written), scale f32 [M][ceil(K / 128)].
+ * kudnn_quantize_blocks: w {E, K, N} ACB -> q e4m3 [E][N][K] dense, scale f32 [E][ceil(N / 128)][ceil(K / 128)]. */
+KUDNN_HIP_API int kudnn_quantize_rows(const kudnn_tensor_desc *x_desc, const void *x, void *q, int64_t ldq, float *scale,
+                                      void *stream);
+KUDNN_HIP_API int kudnn_quantize_blocks(const kudnn_tensor_desc *w_desc, const void *w, void *q, float *scale,
+                                        void *stream);
+
+/* Linear in 8-bit floating point: y[r] = sum over the blocks b of K of sx[r][b] sw[e][n / 128][b] (xq[r] x wq[e])_b + bias,
+ * accumulated in f32, rounded once. w {K, N} BA, or {E, K, N} ACB with groups: e4m3 and its block scales
+ * f32 [E][ceil(N / 128)][ceil(K / 128)]. x {S, K} AB: e4m3 with x_scale f32 [S][ceil(K / 128)], or bf16 / f16, which the run
+ * quantises as kudnn_quantize_rows does (x_scale NULL). y {R, N} AB, bf16 / f16 / f32. bias {1, N} of y's type or NULL
+ * (without groups only). grouped == 0: one weight for every row (S == R). grouped != 0: rows in the experts' order as for
+ * the grouped Linear, gather as there. */
+KUDNN_HIP_API int kudnn_linear_fp8_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc *w,
+                                          const kudnn_tensor_desc *y, const kudnn_tensor_desc *bias, int grouped,
+                                          int gather, kudnn_linear_fp8_t *plan);
+KUDNN_HIP_API int64_t kudnn_linear_fp8_workspace_bytes(kudnn_linear_fp8_t plan);
+KUDNN_HIP_API int kudnn_linear_fp8_run(kudnn_linear_fp8_t plan, const void *x, const float *x_scale, const void *w,
+                                       const float *w_scale, const void *bias, const int32_t *offsets,
+                                       const int32_t *rows, void *y, void *workspace, void *stream);
+KUDNN_HIP_API int kudnn_linear_fp8_destroy(kudnn_linear_fp8_t plan);
+
+/* Weighted sum: out[t] = sum over j of weights[t][j] y[slots[t][j]], in f32, rounded once; j without a slot adds nothing.
+ * y {R, N} AB, out {T, N} AB, one type of f32 / bf16 / f16; weights f32[T][k], or NULL for ones. top_k <= 64. */
+KUDNN_HIP_API int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kudnn_tensor_desc *out, int top_k,
+                                           kudnn_moe_combine_t *plan);
+KUDNN_HIP_API int kudnn_moe_combine_run(kudnn_moe_combine_t plan, const void *y, const float *weights,
+                                        const int32_t *slots, void *out, void *stream);
+/* dy[slots[t][j]] = weights[t][j] dout[t] (dense {R, N}) and dweights[t][j] = dout[t] . y[slots[t][j]] (f32, 0 without a
+ * slot). The slots are the router's: each row of 0 .. n - 1 once, n the number of slots that are not -1; the rows from n on
+ * are set to zero. Either output may be NULL. */
+KUDNN_HIP_API int kudnn_moe_combine_backward(kudnn_moe_combine_t plan, const void *y, const float *weights,
+                                             const int32_t *slots, const void *dout, void *dy, float *dweights,
+                                             void *stream);
+KUDNN_HIP_API int kudnn_moe_combine_destroy(kudnn_moe_combine_t plan);
 
 /* ---- introspection ---------------------------------------------------------------------------------- */
 /* Name of the kernel family the dispatcher chose for a plan ("mfma_bf16_256x256", "skinny_bf16_nt", ...).

@@ -22,8 +22,8 @@ MAX_DIMS = 5
 SUCCESS, UNSUPPORTED, BAD_ARGUMENTS, NULL_POINTER, ALLOC_FAILED, HIP_ERROR, INTERNAL = range(7)
 
 # element types == KuDNN::Element::TypeT
-DT_UNDEFINED, F32, F16, BF16, S32, S8, U8 = range(7)
-DT_SIZE = {F32: 4, F16: 2, BF16: 2, S32: 4, S8: 1, U8: 1}
+DT_UNDEFINED, F32, F16, BF16, S32, S8, U8, F8E4M3 = range(8)
+DT_SIZE = {F32: 4, F16: 2, BF16: 2, S32: 4, S8: 1, U8: 1, F8E4M3: 1}
 
 # layouts == KuDNN::Layout
 _LAYOUT_NAMES = [
@@ -131,6 +131,26 @@ _SIGS = {
     "kudnn_linear_postops_run": ([_P, _P, _P, _P, _P, _P, ctypes.c_float, _P], ctypes.c_int),
     "kudnn_linear_postops_destroy": ([_P], ctypes.c_int),
     "kudnn_linear_postops_run_noalloc": ([_P, _P, _P, _P, _P, _P, ctypes.c_float, _P], ctypes.c_int),
+    "kudnn_moe_route_create": ([_D, _D, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "kudnn_moe_route_workspace_bytes": ([_P], ctypes.c_int64),
+    "kudnn_moe_route_run": ([_P] * 10, ctypes.c_int),
+    "kudnn_moe_route_backward": ([_P] * 8, ctypes.c_int),
+    "kudnn_moe_route_destroy": ([_P], ctypes.c_int),
+    "kudnn_grouped_linear_create": ([_D, _D, _D, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "kudnn_grouped_linear_run": ([_P] * 7, ctypes.c_int),
+    "kudnn_grouped_linear_backward_input": ([_P] * 6, ctypes.c_int),
+    "kudnn_grouped_linear_backward_weight": ([_P] * 7, ctypes.c_int),
+    "kudnn_grouped_linear_destroy": ([_P], ctypes.c_int),
+    "kudnn_quantize_rows": ([_D, _P, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
+    "kudnn_quantize_blocks": ([_D, _P, _P, _P, _P], ctypes.c_int),
+    "kudnn_linear_fp8_create": ([_D, _D, _D, _D, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "kudnn_linear_fp8_workspace_bytes": ([_P], ctypes.c_int64),
+    "kudnn_linear_fp8_run": ([_P] * 11, ctypes.c_int),
+    "kudnn_linear_fp8_destroy": ([_P], ctypes.c_int),
+    "kudnn_moe_combine_create": ([_D, _D, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "kudnn_moe_combine_run": ([_P] * 6, ctypes.c_int),
+    "kudnn_moe_combine_backward": ([_P] * 8, ctypes.c_int),
+    "kudnn_moe_combine_destroy": ([_P], ctypes.c_int),
     "kudnn_plan_describe": ([_P, ctypes.c_char_p, ctypes.c_int], ctypes.c_int),
     "kudnn_pingpong_source_digest": ([], ctypes.c_char_p),
 }
@@ -294,6 +314,90 @@ class LinearPostOps(_Plan):
     def run(self, a, b, y, bias=None, src=None, gamma=1.0, stream=None):
         check(lib().kudnn_linear_postops_run(self.handle, _ptr(a), _ptr(b), _ptr(y), _ptr(bias), _ptr(src), gamma,
                                              _stream(stream)))
+
+
+class MoeRoute(_Plan):
+    """Router of a mixture of experts: softmax, the top_k experts of each token, and the rows in the experts' order."""
+
+    _destroy = "kudnn_moe_route_destroy"
+
+    def __init__(self, logits, top_k, normalize=True, mask=None):
+        super().__init__()
+        check(lib().kudnn_moe_route_create(_ref(logits), _ref(mask), top_k, int(normalize), ctypes.byref(self.handle)))
+        self.workspace_bytes = lib().kudnn_moe_route_workspace_bytes(self.handle)
+
+    def run(self, logits, mask, weights, experts, offsets, rows, slots, workspace=None, stream=None):
+        check(lib().kudnn_moe_route_run(self.handle, _ptr(logits), _ptr(mask), _ptr(weights), _ptr(experts), _ptr(offsets),
+                                        _ptr(rows), _ptr(slots), _ptr(workspace), _stream(stream)))
+
+    def backward(self, logits, mask, weights, experts, dweights, dlogits, stream=None):
+        check(lib().kudnn_moe_route_backward(self.handle, _ptr(logits), _ptr(mask), _ptr(weights), _ptr(experts),
+                                             _ptr(dweights), _ptr(dlogits), _stream(stream)))
+
+
+class GroupedLinear(_Plan):
+    """y[r] = x[r] x w[e] for the rows r of expert e, and its gradients."""
+
+    _destroy = "kudnn_grouped_linear_destroy"
+
+    def __init__(self, x, w, y, gather=False):
+        super().__init__()
+        check(lib().kudnn_grouped_linear_create(_ref(x), _ref(w), _ref(y), int(gather), ctypes.byref(self.handle)))
+
+    def run(self, x, w, offsets, rows, y, stream=None):
+        check(lib().kudnn_grouped_linear_run(self.handle, _ptr(x), _ptr(w), _ptr(offsets), _ptr(rows), _ptr(y),
+                                             _stream(stream)))
+
+    def backward_input(self, dy, w, offsets, dx, stream=None):
+        check(lib().kudnn_grouped_linear_backward_input(self.handle, _ptr(dy), _ptr(w), _ptr(offsets), _ptr(dx),
+                                                        _stream(stream)))
+
+    def backward_weight(self, dy, x, offsets, rows, dw, stream=None):
+        check(lib().kudnn_grouped_linear_backward_weight(self.handle, _ptr(dy), _ptr(x), _ptr(offsets), _ptr(rows), _ptr(dw),
+                                                         _stream(stream)))
+
+
+class LinearFp8(_Plan):
+    """Linear of e4m3 values with a scale for each block of 128, for one weight or for ragged groups of rows."""
+
+    _destroy = "kudnn_linear_fp8_destroy"
+
+    def __init__(self, x, w, y, bias=None, grouped=False, gather=False):
+        super().__init__()
+        check(lib().kudnn_linear_fp8_create(_ref(x), _ref(w), _ref(y), _ref(bias), int(grouped), int(gather),
+                                            ctypes.byref(self.handle)))
+        self.workspace_bytes = lib().kudnn_linear_fp8_workspace_bytes(self.handle)
+
+    def run(self, x, x_scale, w, w_scale, y, bias=None, offsets=None, rows=None, workspace=None, stream=None):
+        check(lib().kudnn_linear_fp8_run(self.handle, _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(bias),
+                                         _ptr(offsets), _ptr(rows), _ptr(y), _ptr(workspace), _stream(stream)))
+
+
+class MoeCombine(_Plan):
+    """out[t] = sum over j of weights[t][j] y[slots[t][j]], and its gradients."""
+
+    _destroy = "kudnn_moe_combine_destroy"
+
+    def __init__(self, y, out, top_k):
+        super().__init__()
+        check(lib().kudnn_moe_combine_create(_ref(y), _ref(out), top_k, ctypes.byref(self.handle)))
+
+    def run(self, y, weights, slots, out, stream=None):
+        check(lib().kudnn_moe_combine_run(self.handle, _ptr(y), _ptr(weights), _ptr(slots), _ptr(out), _stream(stream)))
+
+    def backward(self, y, weights, slots, dout, dy=None, dweights=None, stream=None):
+        check(lib().kudnn_moe_combine_backward(self.handle, _ptr(y), _ptr(weights), _ptr(slots), _ptr(dout), _ptr(dy),
+                                               _ptr(dweights), _stream(stream)))
+
+
+def quantize_rows(x_desc, x, q, ldq, scale, stream=None) -> None:
+    """e4m3 values and the f32 scale of each 1 x 128 block of the rows of x."""
+    check(lib().kudnn_quantize_rows(_ref(x_desc), _ptr(x), _ptr(q), ldq, _ptr(scale), _stream(stream)))
+
+
+def quantize_blocks(w_desc, w, q, scale, stream=None) -> None:
+    """e4m3 values and the f32 scale of each 128 x 128 block of the weights {E, K, N} ACB."""
+    check(lib().kudnn_quantize_blocks(_ref(w_desc), _ptr(w), _ptr(q), _ptr(scale), _stream(stream)))
 
 
 def synchronize(stream=None) -> None:

@@ -22,6 +22,7 @@
 #include "kernels.h"
 #include "kslice.h"
 #include "layout_table.h"
+#include "plan_base.h"
 #include "plan_types.h"
 
 namespace {
@@ -178,6 +179,11 @@ int ValidateGemm(const kudnn_tensor_desc &src, const kudnn_tensor_desc &wei, con
         return KUDNN_STATUS_UNSUPPORTED;
     }
     if (src.dtype == KUDNN_DT_S32 || wei.dtype == KUDNN_DT_S32) {
+        return KUDNN_STATUS_UNSUPPORTED;
+    }
+    // 8-bit floating point has operators of its own (kudnn_linear_fp8_*): its values mean nothing without their scales
+    if (src.dtype == KUDNN_DT_F8E4M3 || wei.dtype == KUDNN_DT_F8E4M3 || dst.dtype == KUDNN_DT_F8E4M3 ||
+        (!IsNone(bia) && bia->dtype == KUDNN_DT_F8E4M3)) {
         return KUDNN_STATUS_UNSUPPORTED;
     }
     if (numThreads < 0 || numThreads > MaxThreads()) {
@@ -1489,15 +1495,6 @@ int CopyDesc(const kudnn_tensor_desc *in, kudnn_tensor_desc &out)
 // ---------------------------------------------------------------------------------------------------
 // plan objects
 
-enum PlanKind { PLAN_GEMM = 1, PLAN_LINEAR_ACT, PLAN_LINEAR_RES, PLAN_LINEAR_POSTOPS };
-
-struct PlanBase {
-    int kind;
-    std::string desc;
-    explicit PlanBase(int k) : kind(k) {}
-    virtual ~PlanBase() = default;
-};
-
 int64_t DescExtentBytes(const kudnn_tensor_desc &d) { return Extent(d) * DtSize(d.dtype); }
 
 }  // namespace
@@ -1598,6 +1595,18 @@ void *ScratchOf(int &rc)
 // =====================================================================================================
 // exported C ABI
 
+int kudnn_host::SetError(int status, const char *msg) noexcept
+{
+    try {
+        g_lastError = msg;
+    } catch (...) {
+        g_lastError.clear();
+    }
+    return status;
+}
+
+bool kudnn_host::DeviceMemory(const void *p) noexcept { return IsDevicePtr(p); }
+
 extern "C" {
 
 const char *kudnn_last_error(void) { return g_lastError.c_str(); }
@@ -1616,7 +1625,7 @@ int kudnn_tensor_desc_init(kudnn_tensor_desc *desc, int32_t ndims, const int64_t
         return Fail(KUDNN_STATUS_NULL_POINTER, "Tensor Info: null descriptor or dims");
     }
     std::memset(desc, 0, sizeof(*desc));
-    if (dtype <= KUDNN_DT_UNDEFINED || dtype > KUDNN_DT_U8) {
+    if (dtype <= KUDNN_DT_UNDEFINED || dtype > KUDNN_DT_F8E4M3) {
         return Fail(KUDNN_STATUS_BAD_ARGUMENTS, "Tensor Info: Undefined data type of tensor");
     }
     if (ndims < 1 || ndims > KUDNN_HIP_MAX_DIMS) {

@@ -1,0 +1,88 @@
+// Kernel arguments and launchers of the mixture-of-experts operators. A launcher returns 0, or -1 if the launch failed.
+#ifndef KUDNN_MOE_H
+#define KUDNN_MOE_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/kudnn_hip.h"
+
+// ---- router (moe_route.hip)
+
+constexpr int KUDNN_ROUTE_MAX_EXPERTS = 1024, KUDNN_ROUTE_MAX_K = 32;
+constexpr int KUDNN_ROUTE_TOKENS = 64;  // tokens of a workgroup: one bit each in an expert's 64-bit mask
+
+struct RouteArgs {
+    const void *logits;
+    const uint8_t *mask;          // nullptr: every expert is open
+    int64_t T, ld, mask_st, mask_se;
+    int E, k, dt, normalize;
+    float *weights;
+    int32_t *experts, *offsets, *rows, *slots;
+    uint8_t *counts;              // [workgroups][counts_ld]: a workgroup's rows of each expert; unused with one workgroup
+    int counts_ld;
+};
+int kudnn_launch_moe_route(const RouteArgs &a, hipStream_t stream);
+
+struct RouteBackwardArgs {
+    const void *logits;
+    const uint8_t *mask;
+    int64_t T, ld, mask_st, mask_se;
+    int E, k, dt, normalize;
+    const float *weights, *dweights;
+    const int32_t *experts;
+    void *dlogits;                // dense [T][E]
+};
+int kudnn_launch_moe_route_backward(const RouteBackwardArgs &a, hipStream_t stream);
+
+// ---- weighted sum (moe_combine.hip)
+
+struct CombineArgs {
+    const void *y, *dout;
+    const float *weights;         // nullptr: ones
+    const int32_t *slots;
+    void *out, *dy;
+    float *dweights;
+    int64_t T, R, N, ldy, ldo;    // ldo: row pitch of out (dout and dy are dense)
+    int k, dt;
+};
+int kudnn_launch_moe_combine(const CombineArgs &a, hipStream_t stream);
+int kudnn_launch_moe_combine_backward(const CombineArgs &a, hipStream_t stream);
+
+// ---- block quantisation (fp8_quant.hip)
+
+// 8-bit rows made by the library for its own products: whole blocks of 128, zero past K.
+inline int64_t kudnn_fp8_pitch(int64_t K) { return (K + 127) / 128 * 128; }
+// zero_tail: columns K .. ldq - 1 (up to the end of the last block) are written as zeros.
+int kudnn_launch_quantize_rows(const void *x, int dt, int64_t M, int64_t K, int64_t ldx, void *q, int64_t ldq,
+                               float *scale, bool zero_tail, hipStream_t stream);
+int kudnn_launch_quantize_blocks(const void *w, int dt, int64_t E, int64_t N, int64_t K, int64_t we, int64_t ldw, void *q,
+                                 float *scale, hipStream_t stream);
+
+// ---- grouped products (grouped_*.hip)
+
+// C = A x B^T in one of three forms. Rows r of expert e are offsets[e] .. offsets[e + 1] - 1 of [0, R).
+//   GROUPED_FWD     C[r][j] = sum over c of A[row(r)][c] B[e][j][c]       I = rows, J = N, C = K
+//   GROUPED_BWD_IN  C[r][j] = sum over c of A[r][c] B[e][c][j]            I = rows, J = K, C = N
+//   GROUPED_BWD_W   C[e][i][j] = sum over r of A[r][i] B[row(r)][j]       I = N, J = K, C = rows
+// row(r) = rows[r] if rows is given, else r.
+enum { GROUPED_FWD = 0, GROUPED_BWD_IN = 1, GROUPED_BWD_W = 2 };
+
+struct GroupedArgs {
+    const void *a, *b;
+    void *c;
+    const float *a_scale, *b_scale;  // e4m3 operands: [S][KB] and [E][NB][KB]
+    const void *bias;                // of C's type, or nullptr
+    const int32_t *offsets;          // nullptr: one group of all rows
+    const int32_t *rows;             // nullptr: row(r) = r
+    int64_t R, S;                    // rows of the order by expert; rows of the gathered operand
+    int64_t E, I, J, C;              // I: R for the first two forms; C: unused for the last
+    int64_t lda, ldb, ldc;           // row pitches in elements
+    int64_t be, ce;                  // pitch of an expert in B (first two forms), in C (last)
+    int form, dt, c_dt;              // dt: BF16, F16 or F8E4M3 (GROUPED_FWD only)
+};
+
+// Any sizes, pitches and alignments (grouped_generic.hip).
+int kudnn_launch_grouped_generic(const GroupedArgs &g, hipStream_t stream);
+
+#endif  // KUDNN_MOE_H

@@ -1,0 +1,190 @@
+// Weighted sum of a token's experts, out[t] = sum over j of w[t][j] y[slots[t][j]], and its gradients. Both are bound by
+// HBM: the forward pass reads each row of y once and writes a row per token; the backward pass reads y and dout and writes
+// dy, taking the dot products of dweights on the way.
+//
+// A thread holds 16 bytes of a row (8 16-bit or 4 f32 values) and walks the token's k rows, so every access is a whole
+// line of consecutive lanes; rows that are not whole 16-byte pieces take the same kernel with one element a thread.
+// Sums over j run in j's order and dot products in a fixed tree, so results do not depend on timing.
+#include "device_common.h"
+#include "moe.h"
+
+using namespace kudnn_dev;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void *p, int64_t i, float (&v)[VEC])
+{
+    if constexpr (VEC == 1) {
+        v[0] = load_elem(p, DT, i);
+    } else if constexpr (DT == KUDNN_DT_F32) {
+        const float4 r = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+    } else {
+        const uint4 r = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            v[2 * q] = DT == KUDNN_DT_BF16 ? u2f(w[q] << 16) : f16_to_f32(static_cast<uint16_t>(w[q]));
+            v[2 * q + 1] = DT == KUDNN_DT_BF16 ? u2f(w[q] & 0xffff0000u) : f16_to_f32(static_cast<uint16_t>(w[q] >> 16));
+        }
+    }
+}
+
+template <int DT, int VEC>
+__device__ __forceinline__ void store_vec(void *p, int64_t i, const float (&v)[VEC])
+{
+    if constexpr (VEC == 1) {
+        store_elem(p, DT, i, v[0]);
+    } else if constexpr (DT == KUDNN_DT_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            w[q] = DT == KUDNN_DT_BF16 ? pack_bf16x2_rne(v[2 * q], v[2 * q + 1])
+                                       : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
+                                             (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
+        }
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int DT, bool WIDE>
+constexpr int vec_of() { return !WIDE ? 1 : (DT == KUDNN_DT_F32 ? 4 : 8); }
+
+__device__ __forceinline__ int64_t slot_of(const CombineArgs &a, int64_t t, int j)
+{
+    const int64_t s = a.slots[t * a.k + j];
+    return s >= 0 && s < a.R ? s : -1;
+}
+
+// grid: (column pieces, tokens)
+template <int DT, bool WIDE>
+__global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a)
+{
+    constexpr int VEC = vec_of<DT, WIDE>();
+    const int64_t col = (static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x) * VEC;
+    if (col >= a.N) return;
+    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
+        float sum[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) sum[q] = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t s = slot_of(a, t, j);
+            if (s < 0) continue;
+            const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
+            float v[VEC];
+            load_vec<DT, VEC>(a.y, s * a.ldy + col, v);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) sum[q] = fmaf(w, v[q], sum[q]);
+        }
+        store_vec<DT, VEC>(a.out, t * a.ldo + col, sum);
+    }
+}
+
+// A workgroup a token (the last one: the rows that no slot takes). Thread partials of the k dot products meet in LDS.
+template <int DT, bool WIDE>
+__global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs a)
+{
+    constexpr int VEC = vec_of<DT, WIDE>();
+    constexpr int kWaves = kThreads / 64;
+    __shared__ float part[64][kWaves];
+    __shared__ int count;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (blockIdx.x == gridDim.x - 1) {
+        // rows n .. R - 1 have no slot: zero
+        if (a.dy == nullptr) return;
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        int mine = 0;
+        for (int64_t i = threadIdx.x; i < a.T * a.k; i += kThreads) mine += a.slots[i] >= 0 ? 1 : 0;
+        atomicAdd(&count, mine);
+        __syncthreads();
+        const int64_t all = a.R * a.N;
+        float zero[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) zero[q] = 0.0f;
+        for (int64_t i = count * a.N + threadIdx.x * VEC; i < all; i += kThreads * VEC) store_vec<DT, VEC>(a.dy, i, zero);
+        return;
+    }
+    const int64_t t = blockIdx.x;
+    for (int j = 0; j < a.k; ++j) {
+        const int64_t s = slot_of(a, t, j);
+        const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
+        float dot = 0.0f;
+        if (s >= 0) {
+            for (int64_t col = threadIdx.x * VEC; col < a.N; col += kThreads * VEC) {
+                float g[VEC], v[VEC];
+                load_vec<DT, VEC>(a.dout, t * a.N + col, g);
+                if (a.dweights != nullptr) {
+                    load_vec<DT, VEC>(a.y, s * a.ldy + col, v);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) dot = fmaf(g[q], v[q], dot);
+                }
+                if (a.dy != nullptr) {
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) v[q] = w * g[q];
+                    store_vec<DT, VEC>(a.dy, s * a.N + col, v);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+        if (lane == 0) part[j][wave] = dot;
+    }
+    if (a.dweights == nullptr) return;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < a.k) {
+        float dot = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) dot += part[threadIdx.x][w];
+        a.dweights[t * a.k + threadIdx.x] = dot;
+    }
+}
+
+template <int DT>
+int launch(const CombineArgs &a, bool backward, bool wide, hipStream_t stream)
+{
+    constexpr int V = vec_of<DT, true>();
+    if (backward) {
+        const unsigned grid = static_cast<unsigned>(a.T + 1);
+        if (wide) {
+            combine_backward_kernel<DT, true><<<grid, kThreads, 0, stream>>>(a);
+        } else {
+            combine_backward_kernel<DT, false><<<grid, kThreads, 0, stream>>>(a);
+        }
+    } else {
+        const int64_t piece = kThreads * (wide ? V : 1), pieces = (a.N + piece - 1) / piece;
+        const dim3 grid(static_cast<unsigned>(a.T), static_cast<unsigned>(pieces));
+        if (wide) {
+            combine_kernel<DT, true><<<grid, kThreads, 0, stream>>>(a);
+        } else {
+            combine_kernel<DT, false><<<grid, kThreads, 0, stream>>>(a);
+        }
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int dispatch(const CombineArgs &a, bool backward, hipStream_t stream)
+{
+    const int64_t v = a.dt == KUDNN_DT_F32 ? 4 : 8;
+    const bool wide = a.N % v == 0 && a.ldy % v == 0 && a.ldo % v == 0 && aligned16(a.y) && aligned16(a.out) &&
+                      aligned16(a.dout) && aligned16(a.dy);
+    switch (a.dt) {
+        case KUDNN_DT_F32: return launch<KUDNN_DT_F32>(a, backward, wide, stream);
+        case KUDNN_DT_BF16: return launch<KUDNN_DT_BF16>(a, backward, wide, stream);
+        case KUDNN_DT_F16: return launch<KUDNN_DT_F16>(a, backward, wide, stream);
+        default: return -1;
+    }
+}
+
+}  // namespace
+
+int kudnn_launch_moe_combine(const CombineArgs &a, hipStream_t stream) { return dispatch(a, false, stream); }
+int kudnn_launch_moe_combine_backward(const CombineArgs &a, hipStream_t stream) { return dispatch(a, true, stream); }

@@ -1,0 +1,603 @@
+"""The mixture-of-experts operators on the GPU against plain implementations in 64 bits.
+
+Tolerances. A result is an f32 sum rounded once to its type, so it may be off by half a unit of that type (2^-8 of the value
+in bf16, 2^-11 in f16) and by the sum's own rounding, at most n 2^-23 of the sum of the terms' magnitudes for n terms (half
+of it by the order of summation alone; products of 16- and 8-bit values are exact in f32). Softmax weights are quotients of
+sums of exponentials whose arguments are rounded to f32: for logits within 40 of the largest, 40 x 2^-23 relative, and as
+much again for the exponential and the sums.
+"""
+import math
+
+import pytest
+import torch
+
+import kudnn_amd as K
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import kudnn_amd.torch_moe as km
+
+DEV = "cuda"
+HALF = {"bf16": torch.bfloat16, "f16": torch.float16}
+ALL = {"f32": torch.float32, **HALF}
+UNIT = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10, torch.float32: 2.0 ** -23}   # a unit of the last place over the value, at most
+WEIGHT_TOL = 2.0 ** -16
+F8 = torch.float8_e4m3fn
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def near(got, want, magnitude, terms, what=""):
+    """|got - want| within half a unit of got's type and n 2^-23 of the terms' magnitude; f16 below its normals."""
+    bound = UNIT[got.dtype] * want.abs() * 0.5 * 1.001 + terms * 2.0 ** -23 * magnitude + 2.0 ** -25 * (got.dtype == torch.float16)
+    off = (got.double() - want).abs() - bound
+    assert torch.isfinite(got).all() and float(off.max() if off.numel() else 0.0) <= 0.0, \
+        f"{what}: {float((got.double() - want).abs().max())} off, {int((off > 0).sum())} of {off.numel()} elements over their bound"
+
+
+# ---- router
+
+def route_plain(logits, k, normalize, mask=None):
+    """By definition, token by token on the host, in 64 bits."""
+    x = logits.detach().double().cpu()
+    t, e = x.shape
+    open_ = torch.ones(t, e, dtype=torch.bool) if mask is None else mask.cpu().bool().expand(t, e).clone()
+    open_ &= x != -math.inf
+    weights, experts = torch.zeros(t, k, dtype=torch.float64), torch.full((t, k), -1)
+    for i in range(t):
+        mine = [(float(x[i, j]), j) for j in range(e) if open_[i, j]]
+        mine.sort(key=lambda p: (-p[0] if p[0] == p[0] else -math.inf, p[1]))
+        picked = mine[:k]
+        if not mine:
+            continue
+        top = max(p[0] for p in mine)
+        of = [p[0] for p in (picked if normalize else mine)]
+        total = sum(math.exp(v - top) for v in of)
+        for j, (v, at) in enumerate(picked):
+            weights[i, j], experts[i, j] = math.exp(v - top) / total, at
+    order = sorted((int(experts[i, j]), i, j) for i in range(t) for j in range(k) if experts[i, j] >= 0)
+    offsets, rows, slots = [0] * (e + 1), [-1] * (t * k), torch.full((t, k), -1)
+    for s, (at, i, j) in enumerate(order):
+        offsets[at + 1] += 1
+        rows[s] = i
+        slots[i, j] = s
+    for j in range(e):
+        offsets[j + 1] += offsets[j]
+    return weights, experts, torch.tensor(offsets), torch.tensor(rows, dtype=torch.long), slots
+
+
+def check_route(r, plain):
+    weights, experts, offsets, rows, slots = plain
+    assert torch.equal(r.experts.cpu().long(), experts)
+    assert torch.equal(r.offsets.cpu().long(), offsets)
+    assert torch.equal(r.rows.cpu().long(), rows)
+    assert torch.equal(r.slots.cpu().long(), slots)
+    torch.testing.assert_close(r.weights.double().cpu(), weights, rtol=WEIGHT_TOL, atol=1e-30)
+
+
+@pytest.mark.parametrize("dtype", list(ALL))
+@pytest.mark.parametrize("tokens,experts,k", [(1, 1, 1), (1, 64, 8), (2, 4, 4), (63, 16, 2), (64, 17, 3), (65, 60, 8),
+                                              (129, 128, 6), (200, 130, 32), (130, 300, 8), (70, 1024, 5), (1000, 8, 2)])
+def test_route(tokens, experts, k, dtype):
+    logits = randn(gen(tokens + experts), tokens, experts).mul(2).to(ALL[dtype])   # 16-bit types tie often
+    for normalize in (True, False):
+        check_route(km.route(logits, k, normalize), route_plain(logits, k, normalize))
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_route_masks_and_values(tokens):
+    """Rows without an open expert, closed places that hold NaN, infinities and the lowest value, equal logits, -0 and 0."""
+    e, k = 24, 5
+    g = gen(tokens)
+    logits = randn(g, tokens, e)
+    mask = torch.rand(tokens, e, generator=g, device=DEV) > 0.3
+    mask[::7] = False
+    mask[3] = False
+    mask[3, 20] = True                       # one open expert of five asked for
+    odd = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(torch.float32).min], device=DEV)
+    logits = torch.where(mask, logits, odd[torch.randint(0, 4, (tokens, e), generator=g, device=DEV)])
+    logits[5] = torch.where(torch.arange(e, device=DEV) % 2 == 0, 0.0, -0.0)
+    mask[5] = True                           # all equal: the lowest indices
+    logits[8, 2:] = -math.inf
+    logits[8, :2] = 1.0
+    mask[8] = True                           # -infinity closes without a mask
+    logits[9] = torch.finfo(torch.float32).min
+    mask[9] = True                           # the lowest value is open
+    for normalize in (True, False):
+        r = km.route(logits, k, normalize, mask)
+        check_route(r, route_plain(logits, k, normalize, mask))
+    assert r.experts[5].tolist() == [0, 1, 2, 3, 4] and r.experts[3].tolist() == [20, -1, -1, -1, -1]
+    assert r.slots[7].tolist() == [-1] * k and float(r.weights[7].abs().sum()) == 0.0
+
+
+def test_route_mask_shapes_and_strides():
+    g = gen(5)
+    wide = randn(g, 90, 100)
+    logits = wide[:, 10:42]                  # a row pitch of its own
+    for mask in (torch.rand(32, generator=g, device=DEV) > 0.5, torch.rand(90, 1, generator=g, device=DEV) > 0.5,
+                 (torch.rand(32, 90, generator=g, device=DEV) > 0.5).t(), (torch.rand(1, 32, generator=g, device=DEV) > 0.5).to(torch.uint8)):
+        full = mask[None] if mask.dim() == 1 else mask
+        check_route(km.route(logits, 4, True, mask), route_plain(logits, 4, True, full))
+    check_route(km.route(logits.t().contiguous().t(), 4), route_plain(logits, 4, True))
+
+
+def test_route_nan_and_infinity_in_open_places():
+    """An open NaN is the largest and makes the row's weights NaN, as the softmax does; other rows are untouched."""
+    logits = randn(gen(1), 6, 8)
+    logits[1, 5] = math.nan
+    logits[2, 3] = math.inf
+    for normalize in (True, False):
+        r = km.route(logits, 2, normalize)
+        assert r.experts[1, 0] == 5 and torch.isnan(r.weights[1]).all()
+        assert r.experts[2, 0] == 3 and torch.isnan(r.weights[2, 0])
+        clean = [0, 3, 4, 5]
+        w, ex, *_ = route_plain(logits[clean], 2, normalize)
+        assert torch.equal(r.experts[clean].cpu().long(), ex)
+        torch.testing.assert_close(r.weights[clean].double().cpu(), w, rtol=WEIGHT_TOL, atol=0)
+
+
+def test_route_of_no_tokens():
+    r = km.route(torch.empty(0, 12, device=DEV), 3)
+    assert r.offsets.tolist() == [0] * 13 and r.rows.numel() == 0 and r.slots.shape == (0, 3)
+
+
+def soft_weights(x, experts, normalize, open_):
+    """The weights as a differentiable function of the logits in 64 bits, for chosen experts."""
+    p = torch.softmax(x.masked_fill(~open_, -math.inf), 1).nan_to_num(0.0)
+    w = torch.where(experts >= 0, p.gather(1, experts.clamp_min(0)), 0.0)
+    return w / w.sum(1, keepdim=True).clamp_min(1e-300) if normalize else w
+
+
+@pytest.mark.parametrize("dtype", list(ALL))
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("tokens,experts,k", [(1, 8, 2), (77, 60, 4), (130, 130, 8), (9, 700, 3)])
+def test_route_gradient(tokens, experts, k, normalize, dtype):
+    g = gen(11)
+    logits = randn(g, tokens, experts).to(ALL[dtype]).requires_grad_(True)
+    mask = torch.rand(tokens, experts, generator=g, device=DEV) > 0.2
+    mask[::5] = False
+    d = randn(g, tokens, k)
+    r = km.route(logits, k, normalize, mask)
+    grad, = torch.autograd.grad(r.weights, logits, d)
+    x = logits.detach().double().requires_grad_(True)
+    open_ = mask & (x.detach() != -math.inf)
+    rows = open_.any(1)                      # a row without open experts has no softmax: gradient zero
+    want = torch.zeros_like(x)
+    w = soft_weights(x[rows], r.experts[rows].long(), normalize, open_[rows])
+    want[rows] = torch.autograd.grad((w * d[rows].double()).sum(), x)[0][rows]
+    assert float(grad[~rows].abs().sum()) == 0.0
+    near(grad, want, WEIGHT_TOL * 2.0 ** 23 * d.double().abs().sum(1, keepdim=True) / k, 1, "dlogits")
+
+
+def test_route_gradient_against_differences():
+    g = gen(2)
+    logits = randn(g, 5, 12)
+    d = randn(g, 5, 3)
+    for normalize in (True, False):
+        x = logits.clone().requires_grad_(True)
+        r = km.route(x, 3, normalize)
+        grad, = torch.autograd.grad(r.weights, x, d)
+        base = r.experts
+        for i, j in [(0, int(base[0, 0])), (1, int(base[1, 2])), (2, 7), (4, int(base[4, 1]))]:
+            h = 2.0 ** -7
+            value = []
+            for sign in (1, -1):
+                moved = logits.clone()
+                moved[i, j] += sign * h
+                q = km.route(moved, 3, normalize)
+                if not torch.equal(q.experts, base):
+                    break
+                value.append(float((q.weights.double() * d.double()).sum()))
+            if len(value) == 2:
+                # central difference: h^2 / 6 of a third derivative of at most about 2 |d|, and the weights' rounding over h
+                bound = (h * h / 3 + WEIGHT_TOL / h) * float(d[i].abs().sum())
+                assert abs((value[0] - value[1]) / (2 * h) - float(grad[i, j])) <= bound
+
+
+# ---- grouped Linear
+
+def make_order(counts, extra, tokens, g):
+    """offsets and rows for groups of the given sizes, with `extra` rows of no expert behind them."""
+    offsets = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32, device=DEV)
+    total = sum(counts)
+    rows = torch.randint(0, max(1, tokens), (total + extra,), generator=g, device=DEV, dtype=torch.int32)
+    rows[total:] = -1
+    return offsets, rows
+
+
+def grouped_plain(x, w, offsets, rows, count, dy=None):
+    xs = x.double() if rows is None else torch.where(rows[:, None] >= 0, x.double()[rows.long().clamp_min(0)], 0.0)
+    o = offsets.tolist()
+    y = torch.zeros(count, w.shape[1], dtype=torch.float64, device=DEV)
+    my, mx, mw = torch.zeros_like(y), torch.zeros(count, w.shape[2], dtype=torch.float64, device=DEV), torch.zeros(w.shape, dtype=torch.float64, device=DEV)
+    dxs, dw = torch.zeros_like(mx), torch.zeros_like(mw)
+    for e, (lo, hi) in enumerate(zip(o, o[1:])):
+        if hi == lo:
+            continue
+        we = w[e].double()
+        y[lo:hi], my[lo:hi] = xs[lo:hi] @ we.t(), xs[lo:hi].abs() @ we.abs().t()
+        if dy is not None:
+            d = dy[lo:hi].double()
+            dxs[lo:hi], mx[lo:hi] = d @ we, d.abs() @ we.abs()
+            dw[e], mw[e] = d.t() @ xs[lo:hi], d.abs().t() @ xs[lo:hi].abs()
+    return y, my, dxs, mx, dw, mw
+
+
+SHAPES = [
+    # counts, rows of no expert, tokens, K, N
+    ([1], 0, 1, 64, 64),
+    ([3, 0, 1, 9], 0, 5, 64, 128),
+    ([0, 0, 0], 4, 4, 64, 64),                       # no rows at all
+    ([17, 64, 1, 0, 130], 6, 50, 128, 96),
+    ([40, 300, 7], 0, 90, 256, 264),
+    ([33, 5], 3, 20, 8, 8),
+    ([5, 70], 1, 20, 72, 40),                        # K past whole blocks of 64
+    ([5, 70], 1, 20, 33, 7),                         # nothing aligned
+    ([260, 1, 515], 9, 300, 320, 512),
+    ([700, 0, 30], 0, 400, 1000, 520),
+    ([1] * 70, 0, 9, 192, 320),                      # more experts than a wave has lanes
+    ([2, 1, 5] * 50, 2, 60, 64, 72),
+    ([12, 16, 15, 1], 0, 30, 2048, 136),
+]
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("counts,extra,tokens,width,out", SHAPES)
+def test_grouped_linear(counts, extra, tokens, width, out, gather, dtype):
+    dt = HALF[dtype]
+    g = gen(width + out)
+    offsets, rows = make_order(counts, extra, tokens, g)
+    count = sum(counts) + extra
+    x = randn(g, tokens if gather else count, width).to(dt).requires_grad_(True)
+    w = (randn(g, len(counts), out, width) * width ** -0.5).to(dt).requires_grad_(True)
+    dy = randn(g, count, out).to(dt)
+    r = rows if gather else None
+    y = km.grouped_linear(x.detach(), w.detach(), offsets, r)
+    want, my, dxs, mx, dw, mw = grouped_plain(x.detach(), w.detach(), offsets, r, count, dy)
+    near(y, want, my, width + 1, "y")
+    assert float(y[sum(counts):].abs().sum()) == 0.0
+    plan = K.GroupedLinear(K.desc(x.shape, K.BF16 if dtype == "bf16" else K.F16), K.desc([len(counts), width, out], K.BF16 if dtype == "bf16" else K.F16, "ACB"),
+                           K.desc([count, out], K.BF16 if dtype == "bf16" else K.F16), gather)
+    stream = torch.cuda.current_stream()
+    gx, gw = torch.full((count, width), math.nan, dtype=dt, device=DEV), torch.full(w.shape, math.nan, dtype=dt, device=DEV)
+    plan.backward_input(dy, w, offsets, gx, stream)
+    plan.backward_weight(dy, x, offsets, r, gw, stream)
+    near(gx, dxs, mx, out + 1, "dx")
+    near(gw, dw, mw, max(counts) + 1, "dw")
+
+
+def test_grouped_linear_autograd():
+    """Through the router's order: a token's gradient is the sum over its slots."""
+    for seed, (t, e, k, width, out) in enumerate([(40, 6, 2, 64, 72), (300, 12, 3, 256, 128), (7, 20, 4, 24, 16)]):
+        g = gen(seed)
+        mask = torch.rand(t, e, generator=g, device=DEV) > 0.3
+        mask[::6] = False
+        r = km.route(randn(g, t, e), k, True, mask)
+        x = randn(g, t, width).bfloat16().requires_grad_(True)
+        w = (randn(g, e, out, width) * width ** -0.5).bfloat16().requires_grad_(True)
+        y = km.grouped_linear(x, w, r.offsets, r.rows, r.slots)
+        dy = randn(g, *y.shape).bfloat16()
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        _, _, dxs, mx, want_w, mw = grouped_plain(x.detach(), w.detach(), r.offsets, r.rows, t * k, dy)
+        took = (r.slots >= 0)[:, :, None]
+        pick = lambda v: torch.where(took, v[r.slots.long().clamp_min(0)], 0.0)
+        # each slot's product is rounded to bf16 before the sum: half a unit of each
+        near(dx, pick(dxs).sum(1), pick(mx).sum(1) + (pick(dxs).abs().sum(1) * 2.0 ** -8 * 2.0 ** 23) / (out + 1 + k), out + 1 + k, "dx")
+        near(dw, want_w, mw, t + 1, "dw")
+
+
+def test_grouped_linear_strides():
+    """Rows and weights with a pitch of their own, aligned and not, bases off 16 bytes, a broadcast token, expanded gradients."""
+    g = gen(3)
+    counts = [20, 0, 300, 5]
+    count = sum(counts)
+    offsets, _ = make_order(counts, 0, 1, g)
+    for width, pad, shift in [(128, 64, 0), (128, 8, 8), (128, 5, 0), (96, 0, 1), (64, 16, 3)]:
+        base = randn(g, count * (width + pad) + 64).bfloat16()
+        x = base[shift:shift + count * (width + pad)].view(count, width + pad)[:, :width]
+        wb = (randn(g, 4 * 80 * (width + pad) + 64) * width ** -0.5).bfloat16()
+        w = wb[shift:shift + 4 * 80 * (width + pad)].view(4, 80, width + pad)[:, :72, :width]
+        xr, wr = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = km.grouped_linear(xr, wr, offsets)
+        want, my, dxs, mx, dw, mw = grouped_plain(x, w, offsets, None, count, torch.ones(count, 72, device=DEV))
+        near(y.detach(), want, my, width + 1, "y")
+        gx, gw = torch.autograd.grad(y.sum(), (xr, wr))     # the gradient of a sum is expanded, with strides of 0
+        near(gx, dxs, mx, 73, "dx")
+        near(gw, dw, mw, 301, "dw")
+    token = randn(g, 1, 128).bfloat16()
+    w = (randn(g, 4, 64, 128) * 0.1).bfloat16()
+    near(km.grouped_linear(token.expand(count, 128), w, offsets), *grouped_plain(token.expand(count, 128), w, offsets, None, count)[:2], 129)
+
+
+def test_grouped_linear_keeps_infinities_and_nan_in_their_rows():
+    """A NaN of one row or expert reaches no other; rows past the last expert are zero whatever the memory holds."""
+    g = gen(4)
+    for counts, width, out in [([6, 9, 4], 128, 64), ([200, 70, 300], 128, 512), ([30, 3], 40, 24)]:
+        offsets, _ = make_order(counts, 0, 1, g)
+        count = sum(counts) + 5
+        x = randn(g, count, width).bfloat16()
+        w = (randn(g, len(counts), out, width) * 0.1).bfloat16()
+        x[counts[0] - 1] = math.nan
+        x[sum(counts):] = math.inf
+        w[-1, 3] = math.inf
+        y = km.grouped_linear(x, w, offsets)
+        bad = torch.zeros(count, out, dtype=torch.bool, device=DEV)
+        bad[counts[0] - 1] = True
+        bad[sum(counts[:-1]):sum(counts), 3] = True
+        assert torch.equal(~torch.isfinite(y), bad)
+        clean = torch.nan_to_num(x.float(), 0.0, 0.0, 0.0).bfloat16(), torch.nan_to_num(w.float(), 0.0, 0.0, 0.0).bfloat16()
+        want, my, *_ = grouped_plain(*clean, offsets, None, count)
+        near(torch.where(bad, 0, y), torch.where(bad, 0.0, want), my, width + 1)
+        # the gradients: a NaN in dy stays in its row of dx and its expert's dw
+        dy = randn(g, count, out).bfloat16()
+        dy[counts[0]] = math.nan                        # the second expert's first row
+        plan = K.GroupedLinear(K.desc([count, width], K.BF16), K.desc([len(counts), width, out], K.BF16, "ACB"), K.desc([count, out], K.BF16))
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        plan.backward_input(dy, clean[1], offsets, dx, torch.cuda.current_stream())
+        plan.backward_weight(dy, clean[0], offsets, None, dw, torch.cuda.current_stream())
+        assert torch.isnan(dx[counts[0]]).all() and torch.isfinite(dx[:counts[0]]).all() and torch.isfinite(dx[counts[0] + 1:]).all()
+        assert torch.isnan(dw[1]).all() and torch.isfinite(dw[0]).all() and torch.isfinite(dw[2:]).all()
+
+
+def test_grouped_linear_survives_any_offsets_and_rows():
+    """Offsets and rows out of range or out of order are read as far as they make sense: no access outside the buffers."""
+    g = gen(6)
+    x, w = randn(g, 50, 64).bfloat16(), randn(g, 4, 96, 64).bfloat16()
+    rows = torch.tensor([0, 49, -5, 50, 1 << 30, 7] * 10, dtype=torch.int32, device=DEV)
+    for o in ([0, 10, 20, 30, 60], [0, 1000, 2000, 3000, 4000], [-7, -3, 5, 60, 60], [60, 40, 20, 10, 0]):
+        offsets = torch.tensor(o, dtype=torch.int32, device=DEV)
+        y = km.grouped_linear(x, w, offsets, rows)
+        dw = torch.empty_like(w)
+        plan = K.GroupedLinear(K.desc([50, 64], K.BF16), K.desc([4, 64, 96], K.BF16, "ACB"), K.desc([60, 96], K.BF16), True)
+        plan.backward_weight(y.nan_to_num(0.0), x, offsets, rows, dw, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+    offsets = torch.tensor([0, 10, 20, 30, 60], dtype=torch.int32, device=DEV)
+    y = km.grouped_linear(x, w, offsets, rows)
+    valid = (rows >= 0) & (rows < 50)
+    want, my, *_ = grouped_plain(x, w, offsets, torch.where(valid, rows, -1), 60)
+    near(y, want, my, 65)
+    assert float(y[~valid].abs().sum()) == 0.0
+
+
+# ---- 8-bit Linear
+
+def quant_plain(x):
+    """Values and scales of 1 x 128 blocks by definition (f32 divisions, rounding to nearest even), on the host."""
+    x = x.float().cpu()
+    m, k = x.shape
+    kb = (k + 127) // 128
+    full = torch.zeros(m, kb * 128)
+    full[:, :k] = x
+    blocks = full.reshape(m, kb, 128)
+    scale = torch.clamp(blocks.abs().amax(2) / 448.0, min=2.0 ** -126)
+    return (blocks / scale[:, :, None]).to(F8).reshape(m, kb * 128)[:, :k], scale
+
+
+def same_bits(a, b):
+    return torch.equal(a.cpu().contiguous().view(torch.uint8), b.cpu().contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", list(ALL))
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 128), (5, 200), (64, 1024), (7, 131), (200, 96)])
+def test_quantize_rows(m, k, dtype):
+    x = (randn(gen(m * k), m, k) * torch.exp(3 * randn(gen(1), m, k))).to(ALL[dtype])
+    x[0] = 0                                 # a block of zeros
+    if m > 2:
+        x[1] = 1e-30 if dtype != "f16" else 6e-8     # tiny values
+        x[2, 0] = torch.finfo(ALL[dtype]).max
+    q, s = km.quantize_rows(x)
+    qp, sp = quant_plain(x)
+    assert torch.equal(s.cpu(), sp) and same_bits(q, qp)
+    big = torch.zeros(m, k + 3, dtype=x.dtype, device=DEV)
+    big[:, :k] = x
+    q, s = km.quantize_rows(big[:, :k])      # rows with a pitch
+    assert torch.equal(s.cpu(), sp) and same_bits(q, qp)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (130, 260), (3, 64, 128), (2, 200, 72)])
+def test_quantize_blocks(shape):
+    w = (randn(gen(9), *shape) * torch.exp(randn(gen(10), *shape))).bfloat16()
+    q, s = km.quantize_blocks(w)
+    w3, q3, s3 = (t.reshape((1,) * (3 - t.dim()) + t.shape) for t in (w, q, s))
+    for e in range(w3.shape[0]):
+        for i in range(s3.shape[1]):
+            for j in range(s3.shape[2]):
+                part = w3[e, i * 128:i * 128 + 128, j * 128:j * 128 + 128].float().cpu()
+                scale = torch.clamp(part.abs().amax() / 448.0, min=2.0 ** -126)
+                assert float(scale) == float(s3[e, i, j])
+                assert same_bits(q3[e, i * 128:i * 128 + 128, j * 128:j * 128 + 128], (part / scale).to(F8))
+
+
+def dequant(q, s, rows=1):
+    full = s.double().repeat_interleave(rows, -2)[..., :q.shape[-2], :].repeat_interleave(128, -1)[..., :q.shape[-1]]
+    return q.double() * full
+
+
+def make_fp8(g, e, n, k):
+    q = torch.empty(e, n, k, dtype=F8, device=DEV)
+    s = torch.empty(e, (n + 127) // 128, (k + 127) // 128, device=DEV)
+    for i in range(e):
+        q[i], s[i] = km.quantize_blocks(randn(g, n, k) * torch.exp(randn(g, 1, k)) * k ** -0.5)
+    return q, s
+
+
+@pytest.mark.parametrize("out_dtype", list(ALL))
+@pytest.mark.parametrize("m,k,n", [(1, 128, 128), (1, 4096, 256), (2, 64, 40), (5, 1000, 300), (16, 512, 640), (17, 384, 130),
+                                   (64, 256, 512), (100, 96, 72), (300, 640, 700), (33, 50, 9), (513, 1024, 256)])
+def test_linear_fp8(m, k, n, out_dtype):
+    g = gen(m + k + n)
+    x = (randn(g, m, k) * torch.exp(randn(g, 1, k))).bfloat16()
+    w, ws = make_fp8(g, 1, n, k)
+    bias = randn(g, n).to(ALL[out_dtype])
+    xq, xs = quant_plain(x)
+    xd, wd = dequant(xq.to(DEV), xs.to(DEV)), dequant(w[0], ws[0], 128)
+    want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    # the two scales' product and its product with the block's sum are rounded as well: two more terms a block
+    terms = k + 3 * (k // 128 + 1)
+    near(km.linear_fp8(x, w[0], ws[0], out_dtype=ALL[out_dtype]), want, mag, terms, "from bf16")
+    near(km.linear_fp8(x, w[0], ws[0], bias, out_dtype=ALL[out_dtype]), want + bias.double(), mag + bias.double().abs(), terms + 1, "bias")
+    near(km.linear_fp8(xq.to(DEV), w[0], ws[0], x_scale=xs.to(DEV), out_dtype=ALL[out_dtype]), want, mag, terms, "from e4m3")
+
+
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("counts,extra,tokens,width,out", SHAPES)
+def test_grouped_linear_fp8(counts, extra, tokens, width, out, gather):
+    g = gen(width + out + 1)
+    offsets, rows = make_order(counts, extra, tokens, g)
+    count = sum(counts) + extra
+    x = (randn(g, tokens if gather else count, width) * torch.exp(randn(g, 1, width))).half()
+    w, ws = make_fp8(g, len(counts), out, width)
+    r = rows if gather else None
+    xq, xs = quant_plain(x)
+    want, mag, *_ = grouped_plain(dequant(xq.to(DEV), xs.to(DEV)), dequant(w, ws, 128), offsets, r, count)
+    y = km.grouped_linear_fp8(x, w, ws, offsets, r)
+    near(y, want, mag, width + 3 * (width // 128 + 1), "y")
+    assert y.dtype == torch.float16 and float(y[sum(counts):].abs().sum()) == 0.0
+
+
+def test_fp8_nan_and_infinity_stay_in_their_row():
+    g = gen(8)
+    for m, k, n in [(4, 256, 64), (40, 256, 64), (300, 512, 512)]:
+        x = randn(g, m, k).bfloat16()
+        w, ws = make_fp8(g, 1, n, k)
+        clean = km.linear_fp8(x, w[0], ws[0])
+        x[1, 3], x[2, k - 1] = math.nan, math.inf
+        y = km.linear_fp8(x, w[0], ws[0])
+        keep = [i for i in range(m) if i not in (1, 2)]
+        assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all() and torch.equal(y[keep], clean[keep])
+
+
+# ---- weighted sum
+
+@pytest.mark.parametrize("dtype", list(ALL))
+@pytest.mark.parametrize("tokens,experts,k,width", [(1, 4, 2, 64), (3, 8, 8, 4096), (65, 6, 3, 1000), (40, 5, 1, 7), (300, 9, 4, 129)])
+def test_combine(tokens, experts, k, width, dtype):
+    dt = ALL[dtype]
+    g = gen(width)
+    mask = torch.rand(tokens, experts, generator=g, device=DEV) > 0.3
+    mask[::4] = tokens == 1
+    r = km.route(randn(g, tokens, experts), k, True, mask)
+    y = randn(g, tokens * k, width).to(dt).requires_grad_(True)
+    w = r.weights.clone().requires_grad_(True)
+    dout = randn(g, tokens, width).to(dt)
+    out = km.combine(y, w, r.slots)
+    dy, dw = torch.autograd.grad(out, (y, w), dout)
+    took = r.slots >= 0
+    picked = torch.where(took[:, :, None], y.detach().double()[r.slots.long().clamp_min(0)], 0.0)
+    wd = w.detach().double()[:, :, None]
+    near(out.detach(), (wd * picked).sum(1), (wd * picked).abs().sum(1), k, "out")
+    products = dout.double()[:, None, :] * picked
+    near(dw, products.sum(2), products.abs().sum(2), width, "dweights")
+    want = torch.zeros(tokens * k, width, dtype=torch.float64, device=DEV)
+    want[r.slots[took].long()] = (wd * dout.double()[:, None, :])[took]
+    near(dy, want, want.abs(), 1, "dy")
+    near(km.combine(y.detach(), None, r.slots), picked.sum(1), picked.abs().sum(1), k, "ones")
+
+
+def test_combine_strides_and_rows_without_a_slot():
+    g = gen(12)
+    wide = randn(g, 30, 80).bfloat16()
+    slots = torch.tensor([[0, -1], [2, 1], [-1, -1]], dtype=torch.int32, device=DEV)
+    w = torch.tensor([[2.0, math.nan], [0.5, -1.0], [math.inf, 3.0]], device=DEV)   # weights without a slot are not looked at
+    for y in (wide[:, 8:72], wide[:, 3:67], wide[::2, :64], wide.t()[:64, :30].t()):
+        out = km.combine(y, w, slots)
+        want = torch.stack([2.0 * y[0].double(), 0.5 * y[2].double() - y[1].double(), torch.zeros(64, device=DEV, dtype=torch.float64)])
+        near(out, want, want.abs() + 3 * y[1].double().abs(), 2)
+        yr = y.detach().clone().requires_grad_(True)
+        dy, = torch.autograd.grad(km.combine(yr, w, slots).sum(), yr)
+        assert float(dy[3:].abs().sum()) == 0.0 and torch.equal(dy[:3, 0].float(), torch.tensor([2.0, -1.0, 0.5], device=DEV))
+    out = torch.full((2, 64), math.nan, device=DEV, dtype=torch.bfloat16)
+    bad = torch.tensor([[99, 1], [-9, 2]], dtype=torch.int32, device=DEV)            # out of range: none
+    K.MoeCombine(K.desc([30, 64], K.BF16), K.desc([2, 64], K.BF16), 2).run(wide[:, :64].contiguous(), None, bad, out, torch.cuda.current_stream())
+    assert torch.equal(out, wide[1:3, :64])
+
+
+# ---- together
+
+def test_mlp_trains_and_serves():
+    """The operators together: the layer's output and gradients against the formula in 64 bits, and its 8-bit form."""
+    torch.manual_seed(0)
+    layer = km.MoEMlp(256, 320, 12, 3, device=DEV)
+    x = torch.randn(4, 33, 256, device=DEV).bfloat16().requires_grad_(True)
+    mask = torch.rand(4, 33, device=DEV) > 0.2
+    out = layer(x, mask)
+    dout = torch.randn_like(out)
+    grads = torch.autograd.grad(out, (x, layer.up, layer.down, layer.router), dout)
+    # the same in 64 bits on the choice that the layer made; its own roundings to bf16 (logits, products, activation,
+    # gradients) are some ten steps of 2^-9 each, in norm
+    xd = x.detach().double().reshape(-1, 256).requires_grad_(True)
+    up, down, router = (p.detach().double().requires_grad_(True) for p in (layer.up, layer.down, layer.router))
+    r = km.route(torch.nn.functional.linear(x.detach().reshape(-1, 256), layer.router.detach()), 3, True, mask.reshape(-1, 1))
+    p = torch.softmax(xd @ router.t(), 1)
+    total = torch.zeros(132, 256, dtype=torch.float64, device=DEV)
+    picked = torch.where(r.experts >= 0, p.gather(1, r.experts.long().clamp_min(0)), 0.0)
+    picked = picked / picked.sum(1, keepdim=True).clamp_min(1e-300)
+    for e in range(12):
+        h = xd @ up[e].t()
+        y = (torch.nn.functional.silu(h[:, :320]) * h[:, 320:]) @ down[e].t()
+        total = total + (picked * (r.experts == e)).sum(1, keepdim=True) * y
+    want = torch.autograd.grad(total, (xd, up, down, router), dout.double().reshape(-1, 256))
+    rel = lambda a, b: float((a.double().reshape(b.shape) - b).norm() / b.norm())
+    assert rel(out.detach(), total.detach()) < 10 * 2.0 ** -9
+    for a, b in zip(grads, want):
+        assert rel(a, b) < 10 * 2.0 ** -9
+    assert float(out.detach()[~mask].abs().sum()) == 0.0
+    # e4m3 has 3 bits of fraction: 2^-4 relative at most for each value, about 0.03 in norm, three operands deep
+    served = layer.quantized()(x.detach(), mask)
+    assert rel(served, total.detach()) < 0.1
+
+
+def test_one_token():
+    layer = km.MoEMlp(128, 192, 8, 2, device=DEV)
+    with torch.no_grad():
+        many = torch.randn(70, 128, device=DEV).bfloat16()
+        all_ = layer(many)
+        for i in (0, 69):
+            one = layer(many[i:i + 1])
+            # other kernels may serve one token: the sums' order differs, then a rounding to bf16
+            assert float((one - all_[i:i + 1]).float().norm() / all_[i].float().norm()) < 2.0 ** -6
+
+
+def test_streams_and_graphs():
+    """On a stream that is not the default one, and replayed from a graph between eager calls on other values."""
+    g = gen(21)
+    layer = km.MoEMlp(256, 256, 16, 4, device=DEV)
+    served = layer.quantized()
+    x = randn(g, 130, 256).bfloat16()
+    with torch.no_grad():
+        logits = torch.nn.functional.linear(x, layer.router)
+
+        def step(lg, xx):
+            r = km.route(lg, 4)
+            h = km.grouped_linear(xx, layer.up, r.offsets, r.rows)
+            h8 = km.grouped_linear_fp8(xx, served.up, served.up_scale, r.offsets, r.rows)
+            return km.combine(h, r.weights, r.slots), km.combine(h8, r.weights, r.slots)
+
+        want = step(logits, x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = step(logits, x)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        static = logits.clone(), x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step(*static)
+        for i in range(3):
+            other = randn(g, 130, 16).bfloat16(), randn(g, 130, 256).bfloat16()
+            eager = step(*other)
+            torch.cuda.synchronize()
+            for s, o in zip(static, other):
+                s.copy_(o)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(eager, captured))
