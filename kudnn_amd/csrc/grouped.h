@@ -17,7 +17,21 @@ inline bool kudnn_grouped_fits(int64_t R, int64_t E, int64_t N, int64_t K, bool 
 
 inline int kudnn_launch_grouped(const GroupedArgs &g, hipStream_t stream)
 {
-    return kudnn_launch_grouped_generic(g, stream);
+    if (!kudnn_grouped_pingpong_eligible(g)) {
+        return kudnn_launch_grouped_generic(g, stream);
+    }
+    if (g.form == GROUPED_FWD) {
+        const int64_t groups = g.offsets == nullptr ? 1 : (g.E < g.R ? g.E : g.R);
+        const int64_t rows = (g.R + groups - 1) / groups;   // of an expert, on average
+        const int64_t tiles = groups * ((rows + 255) / 256) * ((g.J + 255) / 256);
+        const bool f8 = g.dt == KUDNN_DT_F8E4M3;
+        if (rows <= 64 || (f8 && (g.c_dt == KUDNN_DT_F32 || tiles < 128))) {
+            const int bm = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+            const int64_t narrow = groups * ((rows + bm - 1) / bm) * ((g.J + 63) / 64);
+            return kudnn_launch_grouped_stream(g, bm, bm == 16 && narrow < 512 ? 32 : 64, stream);
+        }
+    }
+    return kudnn_launch_grouped_pingpong(g, stream);
 }
 
 #endif  // KUDNN_GROUPED_H

@@ -11,55 +11,77 @@ namespace kudnn_dev {
 struct RowTile {
     int e, begin, end;   // the expert's rows
     int r0;              // first row of the tile
-    int index;           // the tile's place among the experts' tiles (for the order of workgroups)
 };
 
 __device__ __forceinline__ int clamp_row(int v, int R) { return v < 0 ? 0 : (v > R ? R : v); }
 
-// Row tiles of all experts and of the rest, by one wave: 64 experts at a time, a scan over the lanes. Returns whether tile
-// number `want` exists and fills it in; `total` gets the number of tiles. Offsets are clamped to [0, R], so any contents
-// stay inside the buffers.
-__device__ __forceinline__ bool find_row_tile(const int32_t *offsets, int E, int R, int bm, int want, RowTile &t, int &total)
-{
-    const int lane = threadIdx.x & 63;
-    bool found = false;
-    int carry = 0;
-    if (offsets == nullptr) {   // one group of all rows
-        total = (R + bm - 1) / bm;
-        t = RowTile{0, 0, R, want * bm, want};
-        return want < total;
-    }
-    for (int base = 0; base <= E; base += 64) {
-        const int e = base + lane;
-        int lo = 0, hi = 0;
-        if (e <= E) {
-            lo = clamp_row(offsets[e], R);
-            hi = e < E ? clamp_row(offsets[e + 1], R) : R;
+// Row tiles of all experts and of the rest, as one wave sees them: 64 experts at a time, a scan over the lanes. Offsets are
+// clamped to [0, R], so any contents stay inside the buffers. With up to 63 experts the offsets are read once.
+class RowTiles {
+public:
+    __device__ __forceinline__ RowTiles(const int32_t *offsets, int E, int R, int bm) : offsets_(offsets), E_(E), R_(R), bm_(bm)
+    {
+        if (offsets == nullptr) {   // one group of all rows
+            total_ = (R + bm - 1) / bm;
+            return;
         }
-        const int tiles = hi > lo ? (hi - lo + bm - 1) / bm : 0;
-        int incl = tiles;
+        int carry = 0;
+        for (int base = 0; base <= E; base += 64) {
+            scan(base, carry);
+            carry += __shfl(first_ + tiles_ - carry, 63);
+        }
+        total_ = __builtin_amdgcn_readfirstlane(carry);
+    }
+    __device__ __forceinline__ int total() const { return total_; }
+    // Tile number `want` < total(). Its members are the same in every lane.
+    __device__ __forceinline__ RowTile find(int want)
+    {
+        RowTile t{0, 0, 0, 0};
+        if (offsets_ == nullptr) {
+            t.end = R_;
+            t.r0 = want * bm_;
+            return t;
+        }
+        int carry = 0;
+        for (int base = 0; base <= E_; base += 64) {
+            if (E_ >= 64) scan(base, carry);
+            const unsigned long long who = __ballot(tiles_ > 0 && want >= first_ && want < first_ + tiles_);
+            if (who != 0ull) {
+                const int src = __ffsll(who) - 1;
+                t.e = base + src;
+                t.begin = __builtin_amdgcn_readlane(lo_, src);
+                t.end = __builtin_amdgcn_readlane(hi_, src);
+                t.r0 = t.begin + (want - __builtin_amdgcn_readlane(first_, src)) * bm_;
+                break;
+            }
+            carry += __shfl(first_ + tiles_ - carry, 63);
+        }
+        return t;
+    }
+
+private:
+    // Expert base + lane: its rows, its tiles, and how many tiles there are before.
+    __device__ __forceinline__ void scan(int base, int carry)
+    {
+        const int lane = threadIdx.x & 63, e = base + lane;
+        lo_ = hi_ = 0;
+        if (e <= E_) {
+            lo_ = clamp_row(offsets_[e], R_);
+            hi_ = e < E_ ? clamp_row(offsets_[e + 1], R_) : R_;
+        }
+        tiles_ = hi_ > lo_ ? (hi_ - lo_ + bm_ - 1) / bm_ : 0;
+        int incl = tiles_;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(incl, d);
             incl += lane >= d ? o : 0;
         }
-        const bool mine = tiles > 0 && want >= carry + incl - tiles && want < carry + incl;
-        const unsigned long long who = __ballot(mine);
-        if (who != 0ull) {
-            const int src = __ffsll(static_cast<unsigned long long>(who)) - 1;
-            const int first = carry + __shfl(incl - tiles, src);
-            t.e = base + src;
-            t.begin = __shfl(lo, src);
-            t.end = __shfl(hi, src);
-            t.r0 = t.begin + (want - first) * bm;
-            t.index = want;
-            found = true;
-        }
-        carry += __shfl(incl, 63);
+        first_ = carry + incl - tiles_;
     }
-    total = carry;
-    return found;
-}
+    const int32_t *offsets_;
+    int E_, R_, bm_, total_ = 0;
+    int lo_ = 0, hi_ = 0, tiles_ = 0, first_ = 0;
+};
 
 // Most row tiles that offsets of any contents in order can make: each group of rows leaves at most one part tile.
 inline int64_t max_row_tiles(int64_t R, int64_t E, int64_t bm, bool grouped)

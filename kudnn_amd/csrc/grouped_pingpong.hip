@@ -1,0 +1,621 @@
+// Grouped products on 256 x 256 tiles: the experts' Linear layers, their gradients, and the e4m3 product with block scales.
+//
+// The tile's sum runs over k-tiles of 128 bytes of each operand row (64 16-bit or 128 8-bit values; in the forms that sum
+// over an operand's rows, 64 rows of 512 bytes). Eight waves in two groups of four: while a wave of one group issues MFMAs
+// on a SIMD, its partner of the other group reads its fragments from LDS and sends the copies of later k-tiles, and a
+// barrier swaps the roles (group 1 runs one phase behind). Group 0 streams operand A (double-buffered), group 1 operand B
+// (triple-buffered: its partner group reads a B tile one phase longer); 5 x 32 KB fill the CU's LDS. Wave (p, g) has A's
+// 64 indices from 64 p and B's 128 from 128 g of the tile.
+//
+//   GROUPED_FWD     A = rows of x (gathered), B = rows of W[e]; both contiguous along the sum.
+//   GROUPED_BWD_IN  A = rows of dy, B = W[e] with the summed index as rows: read from LDS by transposing reads.
+//   GROUPED_BWD_W   A = x (gathered), B = dy, both with the summed index, the expert's rows, as rows. Any count of rows: those
+//                   past the expert's last read as zero.
+//
+// Every copy is a buffer load into LDS of 64 x 16 bytes. A lane's row and chunk are its vector offset, the k-tile is the
+// scalar one. What lies outside - rows past the group's end or without a token, chunks past the last column or past the end
+// of the sum - has a vector offset beyond the resource's range and is written as zeros, so ragged groups cost no extra
+// code in the loop, and a neighbour's NaN cannot come in.
+//
+// e4m3: one v_mfma_*_16x16x128 covers a block of 128 for 16 x 16 outputs; its result is added to the running f32 sum times
+// sx[row] sw[block]. A lane's four results share the row of x, so a k-tile costs a wave 32 MFMAs (1024 cycles), 128 fused
+// multiply-adds (512) and 4 products of scales. The row scales are loaded three k-tiles ahead, a lane a row, and pass to the
+// lanes that need them through ds_bpermute.
+//
+// The MFMAs bound the tiles that fill the chip several times; with 256 rows of one expert or fewer a tile it is the
+// weight's stream, and rows that do not fill a tile are multiplied all the same (grouped.h says where the smaller tiles
+// of grouped_stream.hip take over).
+#include <type_traits>
+#include <utility>
+
+#include "grouped_common.h"
+
+using namespace kudnn_dev;
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(4))) float const_float;
+
+constexpr int kBM = 256, kBN = 256, kKC = 8, kTile = 256 * kKC;  // kTile: 16-byte chunks of a buffer (32 KB)
+constexpr uint32_t kOut = 0xffffffffu;                            // a vector offset outside every resource
+constexpr int kPitch = 68;                                        // epilogue staging: 64 columns + 4 (floats)
+
+template <int... I, typename F>
+__device__ __forceinline__ void sfor_impl(std::integer_sequence<int, I...>, F &&f)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void sfor(F &&f)
+{
+    sfor_impl(std::make_integer_sequence<int, N>{}, f);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt()
+{
+    // s_waitcnt: vmcnt[3:0] bits 3:0, vmcnt[5:4] bits 15:14; expcnt (7) and lgkmcnt (15) left unconstrained
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
+}
+__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+__device__ __forceinline__ uint32_t lds_addr(const uint4 *p)
+{
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)p));
+}
+
+// Raw buffer resource: base address, no stride, `bytes` in range, 32-bit data format.
+__device__ __forceinline__ i32x4_t make_rsrc(const void *base, uint64_t bytes)
+{
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    i32x4_t rs;
+    rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(p)));
+    rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((p >> 32) & 0xffffu));
+    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0xfffffff0ull ? static_cast<uint32_t>(bytes) : 0xfffffff0u));
+    rs.w = 0x00020000;
+    return rs;
+}
+
+// One copy to LDS: lane l's 16 bytes at voff + soff of the resource land at lds + 16 l, zeros where voff is out of range.
+// Inline asm, so that the compiler does not wait for every copy before the next LDS read: the kernel's own waits order
+// them. The s_nop is the wait state between the write of M0 and the copy that reads it; the resource and soff were written
+// by scalar instructions, or at least five instructions earlier (the s_nop 4 before the first copy of a k-tile).
+__device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
+{
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                 ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
+}
+
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Eight outputs of a row from column j: one or two 16-byte stores where the row allows it, else element by element.
+__device__ __forceinline__ void store8(const GroupedArgs &g, int64_t at, int64_t j, const float (&v)[8], bool wide)
+{
+    if (wide && j + 8 <= g.J) {
+        if (g.c_dt == KUDNN_DT_F32) {
+            float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(g.c) + at);
+            p[0] = make_float4(v[0], v[1], v[2], v[3]);
+            p[1] = make_float4(v[4], v[5], v[6], v[7]);
+            return;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            w[q] = g.c_dt == KUDNN_DT_BF16 ? pack_bf16x2_rne(v[2 * q], v[2 * q + 1])
+                                           : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
+                                                 (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
+        }
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(g.c) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        if (j + q < g.J) store_elem(g.c, g.c_dt, at + q, v[q]);
+    }
+}
+
+template <int CT, int FORM>
+__global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga, int tilesJ, int order)
+{
+    constexpr bool F8 = CT == KUDNN_DT_F8E4M3;
+    constexpr uint32_t ES = F8 ? 1u : 2u;
+    constexpr bool AK = FORM == GROUPED_BWD_W;      // A is read with the summed index as rows
+    constexpr bool BK = FORM != GROUPED_FWD;        // so is B
+    __shared__ uint4 a0[kTile], a1[kTile], b0[kTile], b1[kTile], b2[kTile];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = wave >> 2, p = wave & 3;
+    const int R = static_cast<int>(ga.R), E = static_cast<int>(ga.E);
+
+    // ---- which tile: A's and B's first index, the group's rows, the k-tiles
+    int e, aFirst, bFirst, begin, end, sumLen;
+    if constexpr (FORM == GROUPED_BWD_W) {
+        const int tilesI = static_cast<int>((ga.I + kBN - 1) / kBN), perExpert = tilesI * tilesJ;
+        const int lid = xcd_remap(blockIdx.x, gridDim.x);
+        e = lid / perExpert;
+        int ti, tj;
+        grouped_tile(lid - e * perExpert, tilesI, tilesJ, order, ti, tj);
+        begin = clamp_row(ga.offsets[e], R);
+        end = clamp_row(ga.offsets[e + 1], R);
+        aFirst = tj * kBM;                          // columns of x, C's columns
+        bFirst = ti * kBN;                          // columns of dy, C's rows
+        sumLen = end > begin ? end - begin : 0;
+    } else {
+        RowTiles tiles(ga.offsets, E, R, kBM);
+        const int actual = tiles.total() * tilesJ;
+        if (static_cast<int>(blockIdx.x) >= actual) return;
+        int ti, tj;
+        grouped_tile(xcd_remap(blockIdx.x, actual), tiles.total(), tilesJ, order, ti, tj);
+        const RowTile t = tiles.find(ti);
+        e = t.e;
+        begin = t.r0;
+        end = t.end;
+        aFirst = begin;                             // rows
+        bFirst = tj * kBN;                          // columns of C
+        sumLen = ga.offsets != nullptr && e == E ? 0 : static_cast<int>(ga.C);   // rows of no expert: zero
+    }
+    constexpr int kPerTile = BK && AK ? 64 : static_cast<int>(128u / ES);       // summed indices of a k-tile
+    const int nk = (sumLen + kPerTile - 1) / kPerTile;
+    const int tailLen = sumLen - (nk - 1) * kPerTile;                            // summed indices of the last k-tile
+
+    // ---- this wave's stream: group 0 copies A, group 1 copies B; wave p copies pieces 8 p .. 8 p + 7 of a tile.
+    // Contiguous along the sum: piece q holds rows 8 q .. 8 q + 7, 128 bytes each; lane -> row l / 8, LDS slot l % 8, source
+    // chunk slot ^ ((row / 2) % 8), so that the 16 lanes of a quarter-wave read 16 different slots.
+    // Summed index as rows: piece q holds rows 2 q and 2 q + 1 of 512 bytes; lane -> row l / 32, source chunk
+    // (l % 32) ^ (4 (row % 4)).
+    const uint32_t lda = static_cast<uint32_t>(ga.lda) * ES, ldb = static_cast<uint32_t>(ga.ldb) * ES;
+    uint32_t vo[8];
+    int tailAt[2];      // the first summed index (or row) that this lane's chunk holds, in even and odd pieces
+    uint32_t kStep;     // scalar offset of a k-tile
+    i32x4_t rs;
+    const uint8_t *ax = static_cast<const uint8_t *>(ga.a), *bx = static_cast<const uint8_t *>(ga.b);
+    if (g == 0) {
+        const uint8_t *base;
+        uint64_t bytes;
+        if constexpr (AK) {
+            // x [rows][K]: the expert's rows, or rows of all tokens when gathered
+            base = bx + (ga.rows == nullptr ? static_cast<uint64_t>(begin) * ldb : 0u);
+            bytes = ga.rows == nullptr ? static_cast<uint64_t>(sumLen) * ldb : static_cast<uint64_t>(ga.S) * ldb;
+            kStep = ga.rows == nullptr ? 64u * ldb : 0u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t q = static_cast<uint32_t>(p * 8 + j), row = 2u * q + (static_cast<uint32_t>(lane) >> 5);
+                const uint32_t col = static_cast<uint32_t>(aFirst) + (((static_cast<uint32_t>(lane) & 31u) ^ (4u * (row & 3u))) * 8u);
+                vo[j] = col < static_cast<uint32_t>(ga.J) ? (ga.rows == nullptr ? row * ldb : 0u) + col * ES : kOut;
+            }
+            tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
+        } else {
+            const bool gather = ga.rows != nullptr;
+            base = ax + (gather ? 0u : static_cast<uint64_t>(aFirst) * lda);
+            bytes = gather ? static_cast<uint64_t>(ga.S) * lda : static_cast<uint64_t>(end - aFirst) * lda;
+            kStep = 128u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int q = p * 8 + j, row = q * 8 + (lane >> 3), r = aFirst + row;
+                const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ ((row >> 1) & 7));
+                uint32_t at = kOut;
+                if (r < end) {
+                    if (FORM == GROUPED_FWD && gather) {
+                        const int64_t s = source_row(ga, r);
+                        at = s >= 0 ? static_cast<uint32_t>(s) * lda + chunk * 16u : kOut;
+                    } else {
+                        at = static_cast<uint32_t>(row) * lda + chunk * 16u;
+                    }
+                }
+                vo[j] = at;
+            }
+            tailAt[0] = ((lane & 7) ^ (lane >> 4)) * static_cast<int>(16u / ES);
+            tailAt[1] = ((lane & 7) ^ (4 + (lane >> 4))) * static_cast<int>(16u / ES);
+        }
+        rs = make_rsrc(base, bytes);
+    } else {
+        if constexpr (AK) {
+            // dy [rows][N], the expert's rows
+            rs = make_rsrc(ax + static_cast<uint64_t>(begin) * lda, static_cast<uint64_t>(sumLen) * lda);
+            kStep = 64u * lda;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t q = static_cast<uint32_t>(p * 8 + j), row = 2u * q + (static_cast<uint32_t>(lane) >> 5);
+                const uint32_t col = static_cast<uint32_t>(bFirst) + (((static_cast<uint32_t>(lane) & 31u) ^ (4u * (row & 3u))) * 8u);
+                vo[j] = col < static_cast<uint32_t>(ga.I) ? row * lda + col * ES : kOut;
+            }
+            tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
+        } else if constexpr (BK) {
+            // W[e] [C][J]
+            rs = make_rsrc(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES, static_cast<uint64_t>(ga.C) * ldb);
+            kStep = 64u * ldb;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t q = static_cast<uint32_t>(p * 8 + j), row = 2u * q + (static_cast<uint32_t>(lane) >> 5);
+                const uint32_t col = static_cast<uint32_t>(bFirst) + (((static_cast<uint32_t>(lane) & 31u) ^ (4u * (row & 3u))) * 8u);
+                vo[j] = col < static_cast<uint32_t>(ga.J) ? row * ldb + col * ES : kOut;
+            }
+            tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
+        } else {
+            // W[e] [J][C]
+            rs = make_rsrc(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES + static_cast<uint64_t>(bFirst) * ldb,
+                           static_cast<uint64_t>(kBN) * ldb);
+            kStep = 128u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int q = p * 8 + j, row = q * 8 + (lane >> 3);
+                const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ ((row >> 1) & 7));
+                vo[j] = bFirst + row < ga.J ? static_cast<uint32_t>(row) * ldb + chunk * 16u : kOut;
+            }
+            tailAt[0] = ((lane & 7) ^ (lane >> 4)) * static_cast<int>(16u / ES);
+            tailAt[1] = ((lane & 7) ^ (4 + (lane >> 4))) * static_cast<int>(16u / ES);
+        }
+    }
+    // Gathered rows of x in the weight's gradient change with the k-tile: lane l < 16 holds the byte offset of row l of the
+    // wave's 16 in the k-tile to come. Only group 0 loads them, which waits for all its copies in every phase anyway.
+    const bool gatherK = AK && ga.rows != nullptr;
+    uint32_t rowOff = kOut;
+    auto load_rows = [&](int t) __attribute__((always_inline)) {
+        if (gatherK && g == 0) {
+            const int r = begin + t * 64 + p * 16 + (lane & 15);
+            const int64_t s = r < end ? source_row(ga, r) : -1;
+            rowOff = s >= 0 ? static_cast<uint32_t>(s) * ldb : kOut;
+        }
+    };
+    auto stream = [&](int t, uint32_t lds) __attribute__((always_inline)) {
+        const uint32_t soff = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(t) * kStep);
+        lds = __builtin_amdgcn_readfirstlane(lds + static_cast<uint32_t>(p * 8) * 1024u);
+        if (AK && gatherK && g == 0) {
+            sfor<8>([&](auto jc) __attribute__((always_inline)) {
+                constexpr int j = decltype(jc)::value;
+                const uint32_t r0 = __builtin_amdgcn_readlane(rowOff, 2 * j), r1 = __builtin_amdgcn_readlane(rowOff, 2 * j + 1);
+                const uint32_t r = lane < 32 ? r0 : r1;
+                copy_lds(rs, r == kOut || vo[j] == kOut ? kOut : r + vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
+            });
+        } else if (t == nk - 1 && tailLen < kPerTile) {
+            // past the end of the sum: rows (2 apart from piece to piece), or chunks (whole ones: the sum is a multiple of one)
+            sfor<8>([&](auto jc) __attribute__((always_inline)) {
+                constexpr int j = decltype(jc)::value;
+                const bool rowsAreSummed = g == 0 ? AK : BK;
+                const int at = rowsAreSummed ? tailAt[0] + 2 * j : tailAt[j & 1];
+                copy_lds(rs, at < tailLen ? vo[j] : kOut, soff, lds + static_cast<uint32_t>(j) * 1024u);
+            });
+        } else {
+            sfor<8>([&](auto jc) __attribute__((always_inline)) {
+                constexpr int j = decltype(jc)::value;
+                copy_lds(rs, vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
+            });
+        }
+    };
+
+    // ---- scales (e4m3): lane l holds sx of row 64 p + l for the three k-tiles to come
+    const int KB = static_cast<int>((ga.C + 127) / 128);
+    float sx[3];
+    uint32_t sxAt = kOut;
+    const_float *sw = nullptr;
+    if constexpr (F8) {
+        const int r = aFirst + p * 64 + lane;
+        const int64_t s = r < end ? source_row(ga, r) : -1;
+        sxAt = s >= 0 ? static_cast<uint32_t>(s) * static_cast<uint32_t>(KB) : kOut;
+        const int64_t NB = (ga.J + 127) / 128;
+        int64_t nb = bFirst / 128 + g;
+        nb = nb < NB ? nb : NB - 1;                 // a half tile past the last column: its results are not stored
+        sw = (const_float *)(ga.b_scale + ((e < E ? e : 0) * NB + nb) * KB);
+    }
+    auto load_sx = [&](int t) __attribute__((always_inline)) { return sxAt != kOut && t < nk ? ga.a_scale[sxAt + static_cast<uint32_t>(t)] : 0.0f; };
+
+    // ---- fragments
+    const int lrow = lane & 31, lh = lane >> 5;
+    const int fsw = (lrow >> 1) & 7;
+    const uint32_t kmJJ = static_cast<uint32_t>((lane & 15) >> 2);
+    // transposing reads: row 8 (l / 32) + jj of the 16-row step, column bytes within 64: 16 (2 ((l / 16) & 1) + (l & 3) / 2) +
+    // 8 (l & 1), the 64-byte strip XOR jj
+    const uint32_t trRow = (8u * static_cast<uint32_t>(lane >> 5) + kmJJ) * 512u;
+    const uint32_t trCol = 16u * (2u * static_cast<uint32_t>((lane >> 4) & 1) + static_cast<uint32_t>((lane & 3) >> 1)) + 8u * static_cast<uint32_t>(lane & 1);
+    auto read_tr = [&](const uint4 *buf, uint32_t strip, int s) __attribute__((always_inline)) -> uint4 {
+        typedef short v4i16_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) v4i16_t lds_v4i16;
+        typedef __attribute__((address_space(3))) char lds_char;
+        lds_char *at = (lds_char *)(const_cast<uint4 *>(buf)) + (trRow + ((strip * 64u) ^ (64u * kmJJ)) + trCol);
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *)(at + (16 * s) * 512));
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *)(at + (16 * s + 4) * 512));
+        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+        return make_uint4(l2.x, l2.y, h2.x, h2.y);
+    };
+    const int offA = (p * 64 + lrow) * kKC, offB = (g * 128 + lrow) * kKC;
+    // e4m3: 16 rows, lane group l / 16 has chunks 2 (l / 16) and + 1
+    const int row16 = lane & 15, c16 = (lane >> 4) * 2, sw16 = (row16 >> 1) & 7;
+    auto read16 = [&](const uint4 *buf, int row0) __attribute__((always_inline)) -> i32x8_t {
+        const uint4 lo = buf[(row0 + row16) * kKC + (c16 ^ sw16)], hi = buf[(row0 + row16) * kKC + ((c16 + 1) ^ sw16)];
+        return i32x8_t{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(lo.z), static_cast<int>(lo.w),
+                       static_cast<int>(hi.x), static_cast<int>(hi.y), static_cast<int>(hi.z), static_cast<int>(hi.w)};
+    };
+
+    f32x16_t acc[4][2];      // [strip of 32 of B][strip of 32 of A]
+    f32x4_t acc8[8][4];      // e4m3: [16 of B][16 of A]
+    if constexpr (F8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc8[j][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.0f;
+            }
+        }
+    }
+
+    auto step = [&](auto ic, int t) __attribute__((always_inline)) {
+        constexpr int I = decltype(ic)::value;
+        const uint4 *at = I % 2 == 0 ? a0 : a1;
+        const uint4 *bt = I % 3 == 0 ? b0 : (I % 3 == 1 ? b1 : b2);
+        const uint32_t la = lds_addr(I % 2 == 0 ? a1 : a0), lb = lds_addr(I % 3 == 0 ? b2 : (I % 3 == 1 ? b0 : b1));
+        // ---- memory phase
+        uint4 fa[4][2], fb[2][4];
+        i32x8_t fa8[4], fb8[2];
+        float s8[4];
+        if constexpr (F8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa8[i] = read16(at, p * 64 + i * 16);
+            const float swt = sw[t];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s8[i] = u2f(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute((i * 16 + row16) * 4, static_cast<int>(f2u(sx[I % 3]))))) * swt;
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (AK) {
+                        fa[s][i] = read_tr(at, static_cast<uint32_t>(p * 2 + i), s);
+                    } else {
+                        fa[s][i] = at[offA + i * 32 * kKC + ((2 * s + lh) ^ fsw)];
+                    }
+                }
+            }
+        }
+        const int tt = t + 1 + g;  // group 0 copies A(t + 1), group 1 copies B(t + 2)
+        if (tt < nk) {
+            stream(tt, g == 0 ? la : lb);
+        }
+        // group 1 lets this phase's copies (B(t + 2)) fly and waits for the previous phase's (B(t + 1)), which group 0 reads
+        // in the next phase
+        if (g == 1) {
+            if (t + 2 < nk) {
+                wait_vmcnt<8>();
+            } else {
+                wait_vmcnt<0>();
+            }
+        }
+        if constexpr (F8) {
+            sx[I % 3] = load_sx(t + 3);
+        }
+        load_rows(t + 2);
+        auto read_b = [&](auto slotc, auto stepc) __attribute__((always_inline)) {
+            constexpr int slot = decltype(slotc)::value, s = decltype(stepc)::value;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (BK) {
+                    fb[slot][j] = read_tr(bt, static_cast<uint32_t>(g * 4 + j), s);
+                } else {
+                    fb[slot][j] = bt[offB + j * 32 * kKC + ((2 * s + lh) ^ fsw)];
+                }
+            }
+        };
+        if constexpr (F8) {
+            fb8[0] = read16(bt, g * 128);
+        } else {
+            read_b(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+        }
+        wait_lgkmcnt0();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- compute phase, at raised wave priority
+        __builtin_amdgcn_s_setprio(1);
+        if constexpr (F8) {
+            // product m = 4 j + i of strips j of B and i of A; the sums of product m - 2 run under it
+            f32x4_t part[4];
+            sfor<8>([&](auto jc) __attribute__((always_inline)) {
+                constexpr int j = decltype(jc)::value;
+                if constexpr (j + 1 < 8) {
+                    fb8[(j + 1) & 1] = read16(bt, g * 128 + (j + 1) * 16);
+                }
+                asm volatile("" ::: "memory");   // keeps the later strips' reads, and their registers, behind this one's
+                __builtin_amdgcn_sched_barrier(0);
+                sfor<4>([&](auto ic2) __attribute__((always_inline)) {
+                    constexpr int i = decltype(ic2)::value, m = 4 * j + i - 2;
+                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb8[j & 1], fa8[i], f32x4_t{0.0f, 0.0f, 0.0f, 0.0f},
+                                                                              0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    if constexpr (m >= 0) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc8[m / 4][m % 4][r] = fmaf(s8[m % 4], part[m % 4][r], acc8[m / 4][m % 4][r]);
+                        // the sums belong here: nothing else keeps the compiler from moving all of them to the next k-tile
+                        asm volatile("" : "+v"(acc8[m / 4][m % 4]));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+#pragma unroll
+            for (int i = 2; i < 4; ++i) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc8[7][i][r] = fmaf(s8[i], part[i][r], acc8[7][i][r]);
+                asm volatile("" : "+v"(acc8[7][i]));
+            }
+        } else {
+            sfor<4>([&](auto sc) __attribute__((always_inline)) {
+                constexpr int s = decltype(sc)::value;
+                if constexpr (s + 1 < 4) {
+                    read_b(std::integral_constant<int, (s + 1) & 1>{}, std::integral_constant<int, s + 1>{});
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // the first operand's index runs over a lane's registers: the one that is contiguous in C
+                        const uint4 first = AK ? fa[s][i] : fb[s & 1][j], second = AK ? fb[s & 1][j] : fa[s][i];
+                        if constexpr (CT == KUDNN_DT_BF16) {
+                            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, first),
+                                                                                __builtin_bit_cast(bf16x8_t, second), acc[j][i], 0, 0, 0);
+                        } else {
+                            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, first),
+                                                                               __builtin_bit_cast(f16x8_t, second), acc[j][i], 0, 0, 0);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (g == 0) {
+            wait_vmcnt<0>();   // A(t + 1), which this group reads in the next phase
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    if (nk > 0) {
+        if constexpr (F8) {
+            sfor<3>([&](auto ic) __attribute__((always_inline)) { sx[decltype(ic)::value] = load_sx(decltype(ic)::value); });
+        }
+        load_rows(0);
+        stream(0, g == 0 ? lds_addr(a0) : lds_addr(b0));
+        load_rows(1);
+        if (g == 1 && nk > 1) {
+            stream(1, lds_addr(b1));
+            wait_vmcnt<8>();
+        } else {
+            wait_vmcnt<0>();
+        }
+        __builtin_amdgcn_s_barrier();
+        if (g == 1) {
+            __builtin_amdgcn_s_barrier();  // group 1 runs one phase behind
+        }
+        for (int t = 0; t < nk; t += 6) {
+            sfor<6>([&](auto ic) __attribute__((always_inline)) {
+                if (t + decltype(ic)::value < nk) step(ic, t + decltype(ic)::value);
+            });
+        }
+        if (g == 0) {
+            __builtin_amdgcn_s_barrier();  // matches group 1's extra barrier at the start
+        }
+    }
+
+    // ---- epilogue: units of 32 rows x 64 columns of C pass through LDS (32 x 68 floats a wave, in the tile buffers) and come
+    // back 8 columns a lane: stores of whole 128-byte lines
+    __syncthreads();   // every wave is done with the tile buffers
+    float *stage = reinterpret_cast<float *>(wave < 3 ? a0 : (wave < 6 ? a1 : b0)) + (wave % 3) * (32 * kPitch);
+    const int64_t rowW = FORM == GROUPED_BWD_W ? bFirst + g * 128 : aFirst + p * 64;
+    const int64_t colW = FORM == GROUPED_BWD_W ? aFirst + p * 64 : bFirst + g * 128;
+    const int64_t rowEnd = FORM == GROUPED_BWD_W ? ga.I : end;
+    const int64_t cBase = FORM == GROUPED_BWD_W ? e * ga.ce : 0;
+    const bool wide = ga.ldc % 8 == 0 && ga.ce % 8 == 0 && reinterpret_cast<uintptr_t>(ga.c) % 16 == 0;
+    const int col8 = (lane & 7) * 8, rl = lane >> 3;
+    sfor<4>([&](auto uc) __attribute__((always_inline)) {
+        constexpr int u = decltype(uc)::value;
+        constexpr int rowU = FORM == GROUPED_BWD_W ? u * 32 : (u % 2) * 32, colU = FORM == GROUPED_BWD_W ? 0 : (u / 2) * 64;
+        if constexpr (F8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f32x4_t v = acc8[(u / 2) * 4 + j][(u % 2) * 2 + i];
+                    *reinterpret_cast<float4 *>(stage + (i * 16 + row16) * kPitch + j * 16 + (lane >> 4) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int sh = 0; sh < 2; ++sh) {
+                const f32x16_t &v = FORM == GROUPED_BWD_W ? acc[u][sh] : acc[2 * (u / 2) + sh][u % 2];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    *reinterpret_cast<float4 *>(stage + lrow * kPitch + sh * 32 + q * 8 + lh * 4) =
+                        make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                }
+            }
+        }
+        wave_sync();
+#pragma unroll
+        for (int ps = 0; ps < 4; ++ps) {
+            const int64_t row = rowW + rowU + rl + ps * 8, col = colW + colU + col8;
+            const float *sp = stage + (rl + ps * 8) * kPitch + col8;
+            const float4 lo = *reinterpret_cast<const float4 *>(sp), hi = *reinterpret_cast<const float4 *>(sp + 4);
+            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            if (row < rowEnd && col < ga.J) {
+                if (F8 && ga.bias != nullptr) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] += col + q < ga.J ? load_elem(ga.bias, ga.c_dt, col + q) : 0.0f;
+                }
+                store8(ga, cBase + row * ga.ldc + col, col, v, wide);
+            }
+        }
+        wave_sync();
+    });
+}
+
+template <int CT, int FORM>
+void launch(const GroupedArgs &g, hipStream_t stream)
+{
+    const int64_t tilesJ = (g.J + 255) / 256;
+    const int64_t tiles = FORM == GROUPED_BWD_W ? g.E * ((g.I + 255) / 256) : max_row_tiles(g.R, g.E, 256, g.offsets != nullptr);
+    grouped_pingpong_kernel<CT, FORM><<<static_cast<unsigned>(tiles * tilesJ), 512, 0, stream>>>(g, static_cast<int>(tilesJ), 4);
+}
+
+template <int CT>
+void launch_form(const GroupedArgs &g, hipStream_t stream)
+{
+    switch (g.form) {
+        case GROUPED_FWD: launch<CT, GROUPED_FWD>(g, stream); break;
+        case GROUPED_BWD_IN: launch<CT, GROUPED_BWD_IN>(g, stream); break;
+        default: launch<CT, GROUPED_BWD_W>(g, stream); break;
+    }
+}
+
+}  // namespace
+
+bool kudnn_grouped_pingpong_eligible(const GroupedArgs &g)
+{
+    const int64_t es = g.dt == KUDNN_DT_F8E4M3 ? 1 : 2, whole = 16 / es;
+    const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    // rows are whole 16-byte chunks apart, from aligned bases, and hold whole chunks
+    bool ok = aligned(g.a) && aligned(g.b) && g.lda % whole == 0 && g.ldb % whole == 0;
+    if (g.form == GROUPED_BWD_W) {
+        // the summed index counts rows: the chunks lie along both outputs' indices. 32-bit offsets of the rows of x (all that
+        // a row may come from) and of the expert's rows
+        const int64_t span = (int64_t(1) << 32) - (int64_t(1) << 20);
+        return ok && g.offsets != nullptr && g.I % whole == 0 && g.J % whole == 0 && g.R < span / (g.lda * es) &&
+               (g.S > g.R ? g.S : g.R) < span / (g.ldb * es);
+    }
+    ok = ok && g.be % whole == 0 && g.C % whole == 0 && (g.form == GROUPED_FWD || g.J % whole == 0);
+    const int64_t span = (int64_t(1) << 32) - (int64_t(1) << 20);
+    const int64_t rowsA = g.rows != nullptr ? g.S : 256, rowsB = g.form == GROUPED_FWD ? 256 : g.C;
+    return ok && rowsA < span / (g.lda * es) && rowsB < span / (g.ldb * es);
+}
+
+int kudnn_launch_grouped_pingpong(const GroupedArgs &g, hipStream_t stream)
+{
+    switch (g.dt) {
+        case KUDNN_DT_BF16: launch_form<KUDNN_DT_BF16>(g, stream); break;
+        case KUDNN_DT_F16: launch_form<KUDNN_DT_F16>(g, stream); break;
+        case KUDNN_DT_F8E4M3: launch<KUDNN_DT_F8E4M3, GROUPED_FWD>(g, stream); break;
+        default: return -1;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}

@@ -1,0 +1,351 @@
+// Grouped products of few rows: the experts' Linear layers of one token or a decode batch, e4m3 products of any size that does
+// not fill the chip with 256 x 256 tiles, and every e4m3 product into f32.
+//
+// A workgroup has a tile of BM rows of one expert and BN columns; its waves split the sum: wave w of W takes the blocks
+// w, w + W, ... of 128 bytes of each row and accumulates the whole tile over them. A wave copies a block's rows into LDS of
+// its own, reads them into registers once they are there, sends the copies of its next block and multiplies while they fly.
+// Nothing is shared and no barrier orders the waves until their sums meet in LDS at the end, in wave order (the same bits
+// every run).
+//
+// What bounds it is the weight's way from HBM. A copy covers 8 rows of whole 128-byte lines: reading 16 rows of 64 bytes, the
+// layout the MFMAs want, straight into registers streamed 90 MB at 4.4 TB/s where this pattern gave 5.2, and 5.7 with
+// the non-temporal hint (1 GB: 6.2, 6.1 and 7.0; a plain read of whole rows 7.1). The hint is for weights that one row tile
+// reads.
+//
+// v_mfma_f32_16x16x32: lane l has row l % 16 of an operand and 8 of its 32 summed indices. A block's row is 8 chunks of 16
+// bytes; lane group l / 16 takes chunks g and g + 4. Which index of the sum a lane has does not matter as long as both operands
+// agree. Rows are held with chunk c in slot c ^ ((row / 2) % 8), so that 16 lanes read 16 different slots.
+//
+// e4m3: the matrix instruction for e4m3 aligns the products of 8 consecutive indices to the largest of them and drops what
+// lies more than 13 bits below (measured; groups of 8 are then added in f32). Here, where the weight's way from HBM or the
+// launch takes the time, the values are widened to bf16, which holds them exactly, and multiplied by the bf16 instruction, whose
+// sums are f32's. A block of 128 is four chained MFMAs; its sum times sx[row] sw[block] is added to the running sum.
+//
+// Copies go through buffer resources: rows past the group's end or without a token, columns past the last and chunks past
+// the end of the sum have an offset outside and read as zeros.
+#include <type_traits>
+
+#include "grouped_common.h"
+
+using namespace kudnn_dev;
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(4))) float const_float;
+
+constexpr uint32_t kOut = 0xffffffffu;
+
+// Raw buffer resource: base address, no stride, `bytes` in range, 32-bit data format.
+__device__ __forceinline__ i32x4_t resource(const void *base, uint64_t bytes)
+{
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    i32x4_t rs;
+    rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(p)));
+    rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((p >> 32) & 0xffffu));
+    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0xfffffff0ull ? static_cast<uint32_t>(bytes) : 0xfffffff0u));
+    rs.w = 0x00020000;
+    return rs;
+}
+
+// One copy to LDS: lane l's 16 bytes at voff + soff of the resource land at lds + 16 l, zeros where voff is out of range.
+// Inline asm, so that the compiler does not wait for it before other LDS reads; the waits below order it. The s_nops are the
+// wait states a copy needs after VALU writes of the SGPRs it reads (v_readfirstlane) and after the write of M0.
+template <bool NT>
+__device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
+{
+    if constexpr (NT) {
+        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen nt lds"
+                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
+    } else {
+        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
+    }
+}
+
+// Four e4m3 bytes as four bf16, exactly.
+__device__ __forceinline__ uint2 widen4(uint32_t w)
+{
+    const bf16x2v_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// Operand registers of one MFMA from a chunk: 16-bit types the chunk itself, e4m3 its half h.
+template <int CT>
+__device__ __forceinline__ u32x4_t operand(const u32x4_t &chunk, int h)
+{
+    if constexpr (CT == KUDNN_DT_F8E4M3) {
+        const uint2 a = widen4(chunk[2 * h]), b = widen4(chunk[2 * h + 1]);
+        return u32x4_t{a.x, a.y, b.x, b.y};
+    } else {
+        return chunk;
+    }
+}
+
+template <int CT>
+__device__ __forceinline__ f32x4_t mfma(const u32x4_t &a, const u32x4_t &b, const f32x4_t &c)
+{
+    if constexpr (CT == KUDNN_DT_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+
+// BM x BN tile, W waves. HINT: the weights are read by one row tile (non-temporal).
+template <int CT, int BM, int BN, int W, bool HINT>
+__global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, int tilesJ)
+{
+    constexpr bool F8 = CT == KUDNN_DT_F8E4M3;
+    constexpr int ES = F8 ? 1 : 2, MT = BM / 16, NT = BN / 16, kPitch = BN + 4;
+    constexpr int kStage = (BM + BN) * 8;                        // 16-byte chunks of a wave's block: A's rows, then B's
+    constexpr int kSums = W * BM * kPitch / 4;                   // the sums reuse the stages
+    __shared__ uint4 lds[W * kStage > kSums ? W * kStage : kSums];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row16 = lane & 15, grp = lane >> 4;
+
+    const int E = static_cast<int>(g.E);
+    RowTiles tiles(g.offsets, E, static_cast<int>(g.R), BM);
+    const int actual = tiles.total() * tilesJ;
+    if (static_cast<int>(blockIdx.x) >= actual) return;
+    // the row tiles of one block of columns are neighbours: those of one expert read the same weights
+    const int lid = xcd_remap(blockIdx.x, actual);
+    const int tj = lid / tiles.total();
+    const RowTile t = tiles.find(lid - tj * tiles.total());
+    const int j0 = tj * BN;
+    const bool none = g.offsets != nullptr && t.e == E;   // rows of no expert: zero
+    const int e = none ? 0 : t.e;
+
+    const uint32_t lda = static_cast<uint32_t>(g.lda) * ES, ldb = static_cast<uint32_t>(g.ldb) * ES;
+    const uint32_t rowBytes = static_cast<uint32_t>(g.C) * ES;
+    const int blocks = none ? 0 : static_cast<int>((rowBytes + 127) / 128);
+    const bool gather = g.rows != nullptr;
+    const i32x4_t ra = gather ? resource(g.a, static_cast<uint64_t>(g.S) * lda)
+                              : resource(static_cast<const uint8_t *>(g.a) + static_cast<uint64_t>(t.r0) * lda, static_cast<uint64_t>(t.end - t.r0) * lda);
+    const i32x4_t rb = resource(static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES +
+                                    static_cast<uint64_t>(j0) * ldb, static_cast<uint64_t>(BN) * ldb);
+    // copy i has rows 8 i .. 8 i + 7: lane -> row l / 8, slot l % 8, chunk slot ^ ((row / 2) % 8)
+    uint32_t va[BM / 8], vb[BN / 8];
+    const uint32_t chunk0 = static_cast<uint32_t>((lane & 7) ^ (lane >> 4));
+#pragma unroll
+    for (int i = 0; i < BM / 8; ++i) {
+        const int row = i * 8 + (lane >> 3), r = t.r0 + row;
+        const int64_t s = r < t.end ? source_row(g, r) : -1;
+        va[i] = s < 0 ? kOut : (gather ? static_cast<uint32_t>(s) : static_cast<uint32_t>(row)) * lda + (chunk0 ^ (4u * (i & 1))) * 16u;
+    }
+#pragma unroll
+    for (int i = 0; i < BN / 8; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        vb[i] = j0 + row < g.J ? static_cast<uint32_t>(row) * ldb + (chunk0 ^ (4u * (i & 1))) * 16u : kOut;
+    }
+    const uint32_t stage = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)(lds + wave * kStage)));
+    auto copy = [&](int kb) __attribute__((always_inline)) {
+        const uint32_t at = static_cast<uint32_t>(kb) * 128u;
+        const bool tail = at + 128u > rowBytes;     // chunks past the end of the sum
+        const uint32_t left = rowBytes - at;
+#pragma unroll
+        for (int i = 0; i < BN / 8; ++i) {
+            const bool in = !tail || (chunk0 ^ (4u * (i & 1))) * 16u < left;
+            copy_lds<HINT>(rb, in ? vb[i] : kOut, at, stage + static_cast<uint32_t>(BM / 8 + i) * 1024u);
+        }
+#pragma unroll
+        for (int i = 0; i < BM / 8; ++i) {
+            const bool in = !tail || (chunk0 ^ (4u * (i & 1))) * 16u < left;
+            copy_lds<false>(ra, in ? va[i] : kOut, at, stage + static_cast<uint32_t>(i) * 1024u);
+        }
+    };
+    // scales: lane l has the row of x that its results have, 16 i + l % 16
+    const_float *sw = nullptr;
+    uint32_t sxAt[MT];
+    const uint32_t KB = static_cast<uint32_t>((g.C + 127) / 128);
+    if constexpr (F8) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int r = t.r0 + i * 16 + row16;
+            const int64_t s = r < t.end ? source_row(g, r) : -1;
+            sxAt[i] = s < 0 ? kOut : static_cast<uint32_t>(s) * KB;
+        }
+        sw = (const_float *)(g.b_scale + (static_cast<int64_t>(e) * ((g.J + 127) / 128) + j0 / 128) * KB);
+    }
+    struct Block {
+        u32x4_t a[MT][2], b[NT][2];
+        float sx[MT], sw;
+    };
+    const uint4 *mine = lds + wave * kStage;
+    const int sw16 = (row16 >> 1) & 7;
+    auto fetch = [&](Block &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int slot = (grp + 4 * h) ^ sw16;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) x.b[j][h] = __builtin_bit_cast(u32x4_t, mine[(BM + j * 16 + row16) * 8 + slot]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x.a[i][h] = __builtin_bit_cast(u32x4_t, mine[(i * 16 + row16) * 8 + slot]);
+        }
+    };
+    auto scales = [&](Block &x, int kb) __attribute__((always_inline)) {
+        if constexpr (F8) {
+            x.sw = sw[kb];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x.sx[i] = sxAt[i] != kOut ? g.a_scale[sxAt[i] + static_cast<uint32_t>(kb)] : 0.0f;
+        }
+    };
+
+    f32x4_t acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto multiply = [&](const Block &x) __attribute__((always_inline)) {
+        // the first operand's index runs over a lane's registers: four consecutive columns of one row
+        if constexpr (F8) {
+            u32x4_t a[MT][4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) a[i][s] = operand<CT>(x.a[i][s / 2], s & 1);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                u32x4_t b[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) b[s] = operand<CT>(x.b[j][s / 2], s & 1);
+                f32x4_t part[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) part[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) part[i] = mfma<CT>(b[s], a[i][s], part[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const float s = x.sx[i] * x.sw;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(s, part[i][r], acc[j][i][r]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[j][i] = mfma<CT>(x.b[j][h], x.a[i][h], acc[j][i]);
+                }
+            }
+        }
+    };
+    if (wave < blocks) {
+        copy(wave);
+        for (int kb = wave; kb < blocks; kb += W) {
+            Block x;
+            scales(x, kb);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's copies of block kb have landed
+            fetch(x);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and left LDS before the next ones arrive there
+            if (kb + W < blocks) copy(kb + W);
+            multiply(x);
+        }
+    }
+
+    __syncthreads();   // the sums lie over all waves' stages
+    float *sums = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            *reinterpret_cast<float4 *>(sums + (wave * BM + i * 16 + row16) * kPitch + j * 16 + grp * 4) =
+                make_float4(acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]);
+        }
+    }
+    __syncthreads();
+    const bool wide = g.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(g.c) % 16 == 0;
+    for (int x = threadIdx.x; x < BM * BN / 4; x += W * 64) {
+        const int r = x / (BN / 4), c = x % (BN / 4) * 4;
+        const int64_t row = t.r0 + r, col = j0 + c;
+        if (row >= t.end || col >= g.J) continue;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float4 p = *reinterpret_cast<const float4 *>(sums + (w * BM + r) * kPitch + c);
+            v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+        }
+        const int64_t at = row * g.ldc + col;
+        if (g.bias != nullptr) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] += col + q < g.J ? load_elem(g.bias, g.c_dt, col + q) : 0.0f;
+        }
+        if (wide && col + 4 <= g.J) {
+            if (g.c_dt == KUDNN_DT_F32) {
+                *reinterpret_cast<float4 *>(static_cast<float *>(g.c) + at) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                uint32_t w[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    w[q] = g.c_dt == KUDNN_DT_BF16 ? pack_bf16x2_rne(v[2 * q], v[2 * q + 1])
+                                                   : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
+                                                         (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
+                }
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(g.c) + at) = make_uint2(w[0], w[1]);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (col + q < g.J) store_elem(g.c, g.c_dt, at + q, v[q]);
+            }
+        }
+    }
+}
+
+template <int CT, int BM, int BN, int W>
+void launch(const GroupedArgs &g, bool hint, hipStream_t stream)
+{
+    const int64_t tilesJ = (g.J + BN - 1) / BN;
+    const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    if (hint) {
+        grouped_stream_kernel<CT, BM, BN, W, true><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+    } else {
+        grouped_stream_kernel<CT, BM, BN, W, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+    }
+}
+
+template <int CT>
+void launch_tile(const GroupedArgs &g, int bm, int bn, hipStream_t stream)
+{
+    const int64_t groups = g.offsets == nullptr ? 1 : (g.E < g.R ? g.E : g.R);
+    const bool hint = g.R <= groups * bm;   // one row tile an expert, on average
+    if (bm == 16) {
+        if (bn == 32) {
+            launch<CT, 16, 32, 8>(g, hint, stream);
+        } else {
+            launch<CT, 16, 64, 8>(g, hint, stream);
+        }
+    } else if (bm == 32) {
+        launch<CT, 32, 64, 8>(g, hint, stream);
+    } else if (bn == 64) {
+        launch<CT, 64, 64, 8>(g, hint, stream);
+    } else {
+        launch<CT, 64, 128, 4>(g, hint, stream);
+    }
+}
+
+}  // namespace
+
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, hipStream_t stream)
+{
+    switch (g.dt) {
+        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, stream); break;
+        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, stream); break;
+        case KUDNN_DT_F8E4M3: launch_tile<KUDNN_DT_F8E4M3>(g, bm, bn, stream); break;
+        default: return -1;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}

@@ -84,5 +84,11 @@ struct GroupedArgs {
 
 // Any sizes, pitches and alignments (grouped_generic.hip).
 int kudnn_launch_grouped_generic(const GroupedArgs &g, hipStream_t stream);
+// 256 x 256 tiles (grouped_pingpong.hip): operands of whole 16-byte chunks and 32-bit offsets.
+bool kudnn_grouped_pingpong_eligible(const GroupedArgs &g);
+int kudnn_launch_grouped_pingpong(const GroupedArgs &g, hipStream_t stream);
+// Few rows, the sum dealt to the waves (grouped_stream.hip): GROUPED_FWD under the same conditions, products exact in f32;
+// tiles (bm, bn) of (16, 32), (16, 64), (32, 64) and (64, 64).
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, hipStream_t stream);
 
 #endif  // KUDNN_MOE_H
