@@ -27,7 +27,7 @@ INCLUDE = ROOT / "include"
 
 ARCH = os.environ.get("KUDNN_OFFLOAD_ARCH", "gfx950")
 HIP_SOURCES = ["gemm_mfma.hip", "gemm_pingpong.hip", "gemm_kslice.hip", "gemm_wavek.hip", "gemm_wavek8.hip", "skinny_bf16.hip", "pack.hip",
-               "moe_route.hip", "moe_combine.hip", "fp8_quant.hip", "grouped_generic.hip", "grouped_pingpong.hip", "grouped_stream.hip", "moe_capi.cpp", "capi.cpp"]
+               "moe_route.hip", "moe_combine.hip", "fp8_quant.hip", "grouped_generic.hip", "grouped_pingpong.hip", "grouped_stream.hip", "grouped_ring.hip", "moe_capi.cpp", "capi.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

@@ -1,7 +1,9 @@
 // e4m3 values with a f32 scale for each block: 1 x 128 of a row, 128 x 128 of a weight.
-//   s = max(amax / 448, 2^-126),  q = round to nearest even of x / s
-// Both divisions are IEEE f32 divisions, so the values are the same on every machine that follows the definition. amax / 448
-// is at most 1 + 2^-24 off, so |x / s| stays below 464, where e4m3 would leave its range: no clamp is needed. A NaN in a block
+//   s = max(amax * r, 2^-126) with r = 1 / 448 rounded to f32,  q = round to nearest even of x / s
+// The product is rounded to f32 and the division is an IEEE f32 division, so the values are the same on every machine that
+// follows the definition. (A bf16 x lies on a tie between two e4m3 values in one of 16 cases where s is a power of two, so the last
+// bit of s decides many roundings: the product, and not a quotient, is what torch's division by a number gives on a GPU.)
+// s is at most 2^-23 of itself off amax / 448, so |x / s| stays below 464, where e4m3 would leave its range: no clamp is needed. A NaN in a block
 // stays NaN and an infinity becomes one (inf / inf), which the product hands on.
 // Bound by HBM: x is read once, a byte an element is written.
 #include "device_common.h"
@@ -12,9 +14,9 @@ using namespace kudnn_dev;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kMax = 448.0f, kTiny = 1.17549435e-38f;
+constexpr float kInvMax = 1.0f / 448.0f, kTiny = 1.17549435e-38f;
 
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax / kMax, kTiny); }
+__device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax * kInvMax, kTiny); }
 
 // Four values as e4m3 bytes, lowest first.
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d)

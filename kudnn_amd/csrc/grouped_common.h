@@ -1,4 +1,4 @@
-// Device helpers shared by the grouped product kernels: which rows a workgroup has.
+// Device helpers shared by the grouped product kernels: copies to LDS, operands, and which rows a workgroup has.
 #ifndef KUDNN_GROUPED_COMMON_H
 #define KUDNN_GROUPED_COMMON_H
 
@@ -6,6 +6,87 @@
 #include "moe.h"
 
 namespace kudnn_dev {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(4))) float const_float;
+
+constexpr uint32_t kOut = 0xffffffffu;   // a vector offset outside every resource
+
+// Raw buffer resource: base address, no stride, `bytes` in range, 32-bit data format.
+__device__ __forceinline__ i32x4_t resource(const void *base, uint64_t bytes)
+{
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    i32x4_t rs;
+    rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(p)));
+    rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((p >> 32) & 0xffffu));
+    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0xfffffff0ull ? static_cast<uint32_t>(bytes) : 0xfffffff0u));
+    rs.w = 0x00020000;
+    return rs;
+}
+
+// One copy to LDS: lane l's 16 bytes at voff + soff of the resource land at lds + 16 l, zeros where voff is out of range.
+// Inline asm, so that the compiler does not wait for it before other LDS reads; the waits below order it. The s_nops are the
+// wait states a copy needs after VALU writes of the SGPRs it reads (v_readfirstlane) and after the write of M0.
+template <bool NT>
+__device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
+{
+    if constexpr (NT) {
+        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen nt lds"
+                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
+    } else {
+        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
+    }
+}
+
+// Four e4m3 bytes as four bf16, exactly.
+__device__ __forceinline__ uint2 widen4(uint32_t w)
+{
+    const bf16x2v_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// Operand registers of one MFMA from a chunk: 16-bit types the chunk itself, e4m3 its half h.
+template <int CT>
+__device__ __forceinline__ u32x4_t operand(const u32x4_t &chunk, int h)
+{
+    if constexpr (CT == KUDNN_DT_F8E4M3) {
+        const uint2 a = widen4(chunk[2 * h]), b = widen4(chunk[2 * h + 1]);
+        return u32x4_t{a.x, a.y, b.x, b.y};
+    } else {
+        return chunk;
+    }
+}
+
+__device__ __forceinline__ i32x8_t join(const u32x4_t &lo, const u32x4_t &hi)
+{
+    return i32x8_t{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(lo.z), static_cast<int>(lo.w),
+                   static_cast<int>(hi.x), static_cast<int>(hi.y), static_cast<int>(hi.z), static_cast<int>(hi.w)};
+}
+
+// 16 x 16 sums over 128 e4m3 products (block exponents of 1).
+__device__ __forceinline__ f32x4_t mfma_e4m3(const i32x8_t &a, const i32x8_t &b)
+{
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+}
+
+template <int CT>
+__device__ __forceinline__ f32x4_t mfma(const u32x4_t &a, const u32x4_t &b, const f32x4_t &c)
+{
+    if constexpr (CT == KUDNN_DT_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+
 
 // A tile of rows of one expert. e == E: the rows that belong to no expert (past offsets[E]).
 struct RowTile {
@@ -16,35 +97,31 @@ struct RowTile {
 __device__ __forceinline__ int clamp_row(int v, int R) { return v < 0 ? 0 : (v > R ? R : v); }
 
 // Row tiles of all experts and of the rest, as one wave sees them: 64 experts at a time, a scan over the lanes. Offsets are
-// clamped to [0, R], so any contents stay inside the buffers. With up to 63 experts the offsets are read once.
+// clamped to [0, R], so any contents stay inside the buffers. With up to 64 experts the offsets are read once.
 class RowTiles {
 public:
     __device__ __forceinline__ RowTiles(const int32_t *offsets, int E, int R, int bm) : offsets_(offsets), E_(E), R_(R), bm_(bm)
     {
         if (offsets == nullptr) {   // one group of all rows
-            total_ = (R + bm - 1) / bm;
+            total_ = experts_ = (R + bm - 1) / bm;
             return;
         }
-        int carry = 0;
-        for (int base = 0; base <= E; base += 64) {
-            scan(base, carry);
-            carry += __shfl(first_ + tiles_ - carry, 63);
-        }
-        total_ = __builtin_amdgcn_readfirstlane(carry);
+        for (int base = 0; base < E; base += 64) experts_ = scan(base, experts_);
+        experts_ = __builtin_amdgcn_readfirstlane(experts_);
+        rest_ = __builtin_amdgcn_readlane(hi_, (E - 1) & 63);    // the last expert's end
+        total_ = experts_ + (R - rest_ + bm - 1) / bm;
     }
     __device__ __forceinline__ int total() const { return total_; }
     // Tile number `want` < total(). Its members are the same in every lane.
     __device__ __forceinline__ RowTile find(int want)
     {
-        RowTile t{0, 0, 0, 0};
+        RowTile t{E_, rest_, R_, rest_ + (want - experts_) * bm_};
         if (offsets_ == nullptr) {
-            t.end = R_;
-            t.r0 = want * bm_;
-            return t;
+            return RowTile{0, 0, R_, want * bm_};
         }
-        int carry = 0;
-        for (int base = 0; base <= E_; base += 64) {
-            if (E_ >= 64) scan(base, carry);
+        int before = 0;
+        for (int base = 0; base < E_ && want < experts_; base += 64) {
+            if (E_ > 64) before = scan(base, before);
             const unsigned long long who = __ballot(tiles_ > 0 && want >= first_ && want < first_ + tiles_);
             if (who != 0ull) {
                 const int src = __ffsll(who) - 1;
@@ -54,20 +131,19 @@ public:
                 t.r0 = t.begin + (want - __builtin_amdgcn_readlane(first_, src)) * bm_;
                 break;
             }
-            carry += __shfl(first_ + tiles_ - carry, 63);
         }
         return t;
     }
 
 private:
-    // Expert base + lane: its rows, its tiles, and how many tiles there are before.
-    __device__ __forceinline__ void scan(int base, int carry)
+    // Expert base + lane: its rows, its tiles, and the number of tiles before; returns the number up to the 64th.
+    __device__ __forceinline__ int scan(int base, int before)
     {
         const int lane = threadIdx.x & 63, e = base + lane;
         lo_ = hi_ = 0;
-        if (e <= E_) {
+        if (e < E_) {
             lo_ = clamp_row(offsets_[e], R_);
-            hi_ = e < E_ ? clamp_row(offsets_[e + 1], R_) : R_;
+            hi_ = clamp_row(offsets_[e + 1], R_);
         }
         tiles_ = hi_ > lo_ ? (hi_ - lo_ + bm_ - 1) / bm_ : 0;
         int incl = tiles_;
@@ -76,10 +152,11 @@ private:
             const int o = __shfl_up(incl, d);
             incl += lane >= d ? o : 0;
         }
-        first_ = carry + incl - tiles_;
+        first_ = before + incl - tiles_;
+        return before + __shfl(incl, 63);
     }
     const int32_t *offsets_;
-    int E_, R_, bm_, total_ = 0;
+    int E_, R_, bm_, total_ = 0, experts_ = 0, rest_ = 0;
     int lo_ = 0, hi_ = 0, tiles_ = 0, first_ = 0;
 };
 
@@ -90,6 +167,34 @@ inline int64_t max_row_tiles(int64_t R, int64_t E, int64_t bm, bool grouped)
     const int64_t groups = E + 1 < R ? E + 1 : R;
     // n groups of which every one has a part tile: (R - n) / bm whole ones besides, at most
     return groups + (R - groups) / bm;
+}
+
+// Four outputs of a row from column j at element `at` of C, with the bias; `wide`: a 16- or 8-byte store is aligned.
+__device__ __forceinline__ void store4(const GroupedArgs &g, int64_t at, int64_t j, float (&v)[4], bool wide)
+{
+    if (g.bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += j + q < g.J ? load_elem(g.bias, g.c_dt, j + q) : 0.0f;
+    }
+    if (wide && j + 4 <= g.J) {
+        if (g.c_dt == KUDNN_DT_F32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(g.c) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint32_t w[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                w[q] = g.c_dt == KUDNN_DT_BF16 ? pack_bf16x2_rne(v[2 * q], v[2 * q + 1])
+                                               : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
+                                                     (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
+            }
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(g.c) + at) = make_uint2(w[0], w[1]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (j + q < g.J) store_elem(g.c, g.c_dt, at + q, v[q]);
+    }
 }
 
 // Row of the gathered operand that row r takes, or -1.

@@ -34,17 +34,9 @@ using namespace kudnn_dev;
 
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(4))) float const_float;
 
 constexpr int kBM = 256, kBN = 256, kKC = 8, kTile = 256 * kKC;  // kTile: 16-byte chunks of a buffer (32 KB)
-constexpr uint32_t kOut = 0xffffffffu;                            // a vector offset outside every resource
 constexpr int kPitch = 68;                                        // epilogue staging: 64 columns + 4 (floats)
 
 template <int... I, typename F>
@@ -69,28 +61,6 @@ __device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xC
 __device__ __forceinline__ uint32_t lds_addr(const uint4 *p)
 {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)p));
-}
-
-// Raw buffer resource: base address, no stride, `bytes` in range, 32-bit data format.
-__device__ __forceinline__ i32x4_t make_rsrc(const void *base, uint64_t bytes)
-{
-    const uint64_t p = reinterpret_cast<uint64_t>(base);
-    i32x4_t rs;
-    rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(p)));
-    rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((p >> 32) & 0xffffu));
-    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0xfffffff0ull ? static_cast<uint32_t>(bytes) : 0xfffffff0u));
-    rs.w = 0x00020000;
-    return rs;
-}
-
-// One copy to LDS: lane l's 16 bytes at voff + soff of the resource land at lds + 16 l, zeros where voff is out of range.
-// Inline asm, so that the compiler does not wait for every copy before the next LDS read: the kernel's own waits order
-// them. The s_nop is the wait state between the write of M0 and the copy that reads it; the resource and soff were written
-// by scalar instructions, or at least five instructions earlier (the s_nop 4 before the first copy of a k-tile).
-__device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
-{
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
-                 ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
 }
 
 __device__ __forceinline__ void wave_sync()
@@ -220,11 +190,11 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             tailAt[0] = ((lane & 7) ^ (lane >> 4)) * static_cast<int>(16u / ES);
             tailAt[1] = ((lane & 7) ^ (4 + (lane >> 4))) * static_cast<int>(16u / ES);
         }
-        rs = make_rsrc(base, bytes);
+        rs = resource(base, bytes);
     } else {
         if constexpr (AK) {
             // dy [rows][N], the expert's rows
-            rs = make_rsrc(ax + static_cast<uint64_t>(begin) * lda, static_cast<uint64_t>(sumLen) * lda);
+            rs = resource(ax + static_cast<uint64_t>(begin) * lda, static_cast<uint64_t>(sumLen) * lda);
             kStep = 64u * lda;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -235,7 +205,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
         } else if constexpr (BK) {
             // W[e] [C][J]
-            rs = make_rsrc(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES, static_cast<uint64_t>(ga.C) * ldb);
+            rs = resource(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES, static_cast<uint64_t>(ga.C) * ldb);
             kStep = 64u * ldb;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -246,7 +216,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
         } else {
             // W[e] [J][C]
-            rs = make_rsrc(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES + static_cast<uint64_t>(bFirst) * ldb,
+            rs = resource(bx + static_cast<uint64_t>(e < E ? e : 0) * static_cast<uint64_t>(ga.be) * ES + static_cast<uint64_t>(bFirst) * ldb,
                            static_cast<uint64_t>(kBN) * ldb);
             kStep = 128u;
 #pragma unroll
@@ -278,7 +248,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 constexpr int j = decltype(jc)::value;
                 const uint32_t r0 = __builtin_amdgcn_readlane(rowOff, 2 * j), r1 = __builtin_amdgcn_readlane(rowOff, 2 * j + 1);
                 const uint32_t r = lane < 32 ? r0 : r1;
-                copy_lds(rs, r == kOut || vo[j] == kOut ? kOut : r + vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
+                copy_lds<false>(rs, r == kOut || vo[j] == kOut ? kOut : r + vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
             });
         } else if (t == nk - 1 && tailLen < kPerTile) {
             // past the end of the sum: rows (2 apart from piece to piece), or chunks (whole ones: the sum is a multiple of one)
@@ -286,12 +256,12 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 constexpr int j = decltype(jc)::value;
                 const bool rowsAreSummed = g == 0 ? AK : BK;
                 const int at = rowsAreSummed ? tailAt[0] + 2 * j : tailAt[j & 1];
-                copy_lds(rs, at < tailLen ? vo[j] : kOut, soff, lds + static_cast<uint32_t>(j) * 1024u);
+                copy_lds<false>(rs, at < tailLen ? vo[j] : kOut, soff, lds + static_cast<uint32_t>(j) * 1024u);
             });
         } else {
             sfor<8>([&](auto jc) __attribute__((always_inline)) {
                 constexpr int j = decltype(jc)::value;
-                copy_lds(rs, vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
+                copy_lds<false>(rs, vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
             });
         }
     };
@@ -335,8 +305,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     const int row16 = lane & 15, c16 = (lane >> 4) * 2, sw16 = (row16 >> 1) & 7;
     auto read16 = [&](const uint4 *buf, int row0) __attribute__((always_inline)) -> i32x8_t {
         const uint4 lo = buf[(row0 + row16) * kKC + (c16 ^ sw16)], hi = buf[(row0 + row16) * kKC + ((c16 + 1) ^ sw16)];
-        return i32x8_t{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(lo.z), static_cast<int>(lo.w),
-                       static_cast<int>(hi.x), static_cast<int>(hi.y), static_cast<int>(hi.z), static_cast<int>(hi.w)};
+        return join(__builtin_bit_cast(u32x4_t, lo), __builtin_bit_cast(u32x4_t, hi));
     };
 
     f32x16_t acc[4][2];      // [strip of 32 of B][strip of 32 of A]
@@ -439,8 +408,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 __builtin_amdgcn_sched_barrier(0);
                 sfor<4>([&](auto ic2) __attribute__((always_inline)) {
                     constexpr int i = decltype(ic2)::value, m = 4 * j + i - 2;
-                    part[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb8[j & 1], fa8[i], f32x4_t{0.0f, 0.0f, 0.0f, 0.0f},
-                                                                              0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                    part[i] = mfma_e4m3(fb8[j & 1], fa8[i]);
                     if constexpr (m >= 0) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc8[m / 4][m % 4][r] = fmaf(s8[m % 4], part[m % 4][r], acc8[m / 4][m % 4][r]);
@@ -590,7 +558,7 @@ void launch_form(const GroupedArgs &g, hipStream_t stream)
 
 }  // namespace
 
-bool kudnn_grouped_pingpong_eligible(const GroupedArgs &g)
+bool kudnn_grouped_tiled(const GroupedArgs &g)
 {
     const int64_t es = g.dt == KUDNN_DT_F8E4M3 ? 1 : 2, whole = 16 / es;
     const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };

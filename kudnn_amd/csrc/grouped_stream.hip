@@ -31,73 +31,6 @@ using namespace kudnn_dev;
 
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(4))) float const_float;
-
-constexpr uint32_t kOut = 0xffffffffu;
-
-// Raw buffer resource: base address, no stride, `bytes` in range, 32-bit data format.
-__device__ __forceinline__ i32x4_t resource(const void *base, uint64_t bytes)
-{
-    const uint64_t p = reinterpret_cast<uint64_t>(base);
-    i32x4_t rs;
-    rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(p)));
-    rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((p >> 32) & 0xffffu));
-    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes < 0xfffffff0ull ? static_cast<uint32_t>(bytes) : 0xfffffff0u));
-    rs.w = 0x00020000;
-    return rs;
-}
-
-// One copy to LDS: lane l's 16 bytes at voff + soff of the resource land at lds + 16 l, zeros where voff is out of range.
-// Inline asm, so that the compiler does not wait for it before other LDS reads; the waits below order it. The s_nops are the
-// wait states a copy needs after VALU writes of the SGPRs it reads (v_readfirstlane) and after the write of M0.
-template <bool NT>
-__device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
-{
-    if constexpr (NT) {
-        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen nt lds"
-                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
-    } else {
-        asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
-                     ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
-    }
-}
-
-// Four e4m3 bytes as four bf16, exactly.
-__device__ __forceinline__ uint2 widen4(uint32_t w)
-{
-    const bf16x2v_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
-    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
-}
-
-// Operand registers of one MFMA from a chunk: 16-bit types the chunk itself, e4m3 its half h.
-template <int CT>
-__device__ __forceinline__ u32x4_t operand(const u32x4_t &chunk, int h)
-{
-    if constexpr (CT == KUDNN_DT_F8E4M3) {
-        const uint2 a = widen4(chunk[2 * h]), b = widen4(chunk[2 * h + 1]);
-        return u32x4_t{a.x, a.y, b.x, b.y};
-    } else {
-        return chunk;
-    }
-}
-
-template <int CT>
-__device__ __forceinline__ f32x4_t mfma(const u32x4_t &a, const u32x4_t &b, const f32x4_t &c)
-{
-    if constexpr (CT == KUDNN_DT_F16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    }
-}
-
 // BM x BN tile, W waves. HINT: the weights are read by one row tile (non-temporal).
 template <int CT, int BM, int BN, int W, bool HINT>
 __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, int tilesJ)
@@ -278,30 +211,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
             const float4 p = *reinterpret_cast<const float4 *>(sums + (w * BM + r) * kPitch + c);
             v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
         }
-        const int64_t at = row * g.ldc + col;
-        if (g.bias != nullptr) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += col + q < g.J ? load_elem(g.bias, g.c_dt, col + q) : 0.0f;
-        }
-        if (wide && col + 4 <= g.J) {
-            if (g.c_dt == KUDNN_DT_F32) {
-                *reinterpret_cast<float4 *>(static_cast<float *>(g.c) + at) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                uint32_t w[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    w[q] = g.c_dt == KUDNN_DT_BF16 ? pack_bf16x2_rne(v[2 * q], v[2 * q + 1])
-                                                   : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
-                                                         (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
-                }
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(g.c) + at) = make_uint2(w[0], w[1]);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (col + q < g.J) store_elem(g.c, g.c_dt, at + q, v[q]);
-            }
-        }
+        store4(g, row * g.ldc + col, col, v, wide);
     }
 }
 
@@ -318,33 +228,27 @@ void launch(const GroupedArgs &g, bool hint, hipStream_t stream)
 }
 
 template <int CT>
-void launch_tile(const GroupedArgs &g, int bm, int bn, hipStream_t stream)
+void launch_tile(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream)
 {
-    const int64_t groups = g.offsets == nullptr ? 1 : (g.E < g.R ? g.E : g.R);
-    const bool hint = g.R <= groups * bm;   // one row tile an expert, on average
-    if (bm == 16) {
-        if (bn == 32) {
-            launch<CT, 16, 32, 8>(g, hint, stream);
-        } else {
-            launch<CT, 16, 64, 8>(g, hint, stream);
-        }
-    } else if (bm == 32) {
-        launch<CT, 32, 64, 8>(g, hint, stream);
-    } else if (bn == 64) {
-        launch<CT, 64, 64, 8>(g, hint, stream);
+    if (bm == 16 && bn == 32) {
+        launch<CT, 16, 32, 8>(g, hint, stream);
+    } else if (bm == 16) {
+        launch<CT, 16, 64, 8>(g, hint, stream);
+    } else if (waves == 4) {
+        launch<CT, 64, 64, 4>(g, hint, stream);
     } else {
-        launch<CT, 64, 128, 4>(g, hint, stream);
+        launch<CT, 64, 64, 8>(g, hint, stream);
     }
 }
 
 }  // namespace
 
-int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, hipStream_t stream)
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream)
 {
     switch (g.dt) {
-        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, stream); break;
-        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, stream); break;
-        case KUDNN_DT_F8E4M3: launch_tile<KUDNN_DT_F8E4M3>(g, bm, bn, stream); break;
+        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, waves, hint, stream); break;
+        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, waves, hint, stream); break;
+        case KUDNN_DT_F8E4M3: launch_tile<KUDNN_DT_F8E4M3>(g, bm, bn, waves, hint, stream); break;
         default: return -1;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;

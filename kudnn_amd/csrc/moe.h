@@ -84,11 +84,15 @@ struct GroupedArgs {
 
 // Any sizes, pitches and alignments (grouped_generic.hip).
 int kudnn_launch_grouped_generic(const GroupedArgs &g, hipStream_t stream);
-// 256 x 256 tiles (grouped_pingpong.hip): operands of whole 16-byte chunks and 32-bit offsets.
-bool kudnn_grouped_pingpong_eligible(const GroupedArgs &g);
+// Whether the operands are whole 16-byte chunks within 32-bit offsets, as the tiled kernels need them (grouped_pingpong.hip).
+bool kudnn_grouped_tiled(const GroupedArgs &g);
+// 256 x 256 tiles (grouped_pingpong.hip); e4m3 products by the e4m3 matrix instruction.
 int kudnn_launch_grouped_pingpong(const GroupedArgs &g, hipStream_t stream);
-// Few rows, the sum dealt to the waves (grouped_stream.hip): GROUPED_FWD under the same conditions, products exact in f32;
-// tiles (bm, bn) of (16, 32), (16, 64), (32, 64) and (64, 64).
-int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, hipStream_t stream);
+// GROUPED_FWD of few rows, the sum dealt to the waves (grouped_stream.hip); products exact in f32. Tiles (bm, bn) and waves:
+// (16, 32) and (16, 64) with 8, (64, 64) with 4 or 8. hint: the weights are read by one row tile.
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream);
+// GROUPED_FWD on tiles of bm (64 or 128) rows and 128 columns, a ring of 2 or (128 rows) 4 stages (grouped_ring.hip). native:
+// e4m3 products by the e4m3 matrix instruction, else exact in f32.
+int kudnn_launch_grouped_ring(const GroupedArgs &g, int bm, int stages, bool native, bool hint, hipStream_t stream);
 
 #endif  // KUDNN_MOE_H

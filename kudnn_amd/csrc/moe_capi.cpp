@@ -107,6 +107,22 @@ int CheckBuffers(const Buffer (&b)[N])
     return KUDNN_STATUS_SUCCESS;
 }
 
+// The forward kernel of a product whose operands are whole 16-byte chunks, for describe().
+std::string TileName(int64_t R, int64_t groups, int64_t N, int64_t K, int dt, int c_dt)
+{
+    const int64_t whole = dt == KUDNN_DT_F8E4M3 ? 16 : 8;
+    if (R == 0) {
+        return "";
+    }
+    if (K % whole != 0) {
+        return " tile=generic";
+    }
+    const GroupedTile t = kudnn_grouped_rule(R, groups < R ? groups : R, N, K, dt, c_dt);
+    return std::string(" tile=") + (t.kind == GroupedTile::STREAM ? "stream" : (t.kind == GroupedTile::RING ? "ring" : "pingpong")) +
+           std::to_string(t.bm) + "x" + std::to_string(t.bn) + (t.form > 0 ? "/" + std::to_string(t.form) : "") +
+           (t.native || (dt == KUDNN_DT_F8E4M3 && t.kind == GroupedTile::PINGPONG) ? " e4m3" : "");
+}
+
 int Launched(int rc, const char *what)
 {
     return rc == 0 ? KUDNN_STATUS_SUCCESS : SetError(KUDNN_STATUS_HIP_ERROR, what);
@@ -319,7 +335,7 @@ int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const kudnn_tensor_d
         p->dt = x->dtype;
         p->gather = gather != 0;
         p->desc = "grouped_linear E=" + std::to_string(E) + " R=" + std::to_string(R) + " N=" + std::to_string(N) + " K=" +
-                  std::to_string(K) + (p->gather ? " gather" : "");
+                  std::to_string(K) + (p->gather ? " gather" : "") + TileName(R, E, N, K, p->dt, p->dt);
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });
@@ -580,7 +596,7 @@ int kudnn_linear_fp8_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc 
             p->workspace = p->scaleOffset + S * ((K + 127) / 128) * static_cast<int64_t>(sizeof(float));
         }
         p->desc = "linear_fp8 E=" + std::to_string(E) + " R=" + std::to_string(R) + " N=" + std::to_string(N) + " K=" +
-                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "");
+                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "") + TileName(R, E, N, K, KUDNN_DT_F8E4M3, p->ydt);
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });

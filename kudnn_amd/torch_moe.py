@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import (BF16, F16, F32, F8E4M3, U8, GroupedLinear, LinearFp8, MoeCombine, MoeRoute, desc)
+from . import BF16, F16, F32, F8E4M3, U8, GroupedLinear, LinearFp8, MoeCombine, MoeRoute, check, desc, lib
 from . import quantize_blocks as _quantize_blocks
 from . import quantize_rows as _quantize_rows
 
@@ -62,37 +62,26 @@ class Routing(NamedTuple):
     slots: torch.Tensor
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# The calls of one token are bound by the time these functions take (a launch is some 3 us of a call's 8 to 10), so the common
+# path makes no views, context managers or messages that it does not need, and hands pointers to the C ABI as numbers.
+_current = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _on:
-    """Makes the tensors' device the current one where it is not (launches go to the current device)."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.device.index:
-            torch._C._cuda_setDevice(self.device.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch._C._cuda_setDevice(self.before)
-
-
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
-def _gpu(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+def _gpu(name: str, *tensors: Optional[torch.Tensor]) -> None:
     device = tensors[0].device
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != device):
+        if t is not None and not (t.is_cuda and t.device == device):
             raise ValueError(f"kudnn {name} takes GPU tensors of one device")
-    return device
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(plan, device: torch.device) -> Optional[torch.Tensor]:
+    n = plan.workspace_bytes
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
@@ -122,10 +111,10 @@ def _weight_desc(w: torch.Tensor, dt: int):
 
 
 def _order(name: str, offsets: torch.Tensor, experts: int, rows: Optional[torch.Tensor]) -> None:
-    _need(offsets.dtype == torch.int32 and offsets.shape == (experts + 1,) and offsets.is_contiguous(),
-          f"kudnn {name}: offsets must be int32 [{experts + 1}]")
-    if rows is not None:
-        _need(rows.dtype == torch.int32 and rows.dim() == 1 and rows.is_contiguous(), f"kudnn {name}: rows must be int32 [R]")
+    if not (offsets.dtype == torch.int32 and offsets.shape == (experts + 1,) and offsets.is_contiguous()):
+        raise ValueError(f"kudnn {name}: offsets must be int32 [{experts + 1}]")
+    if rows is not None and not (rows.dtype == torch.int32 and rows.dim() == 1 and rows.is_contiguous()):
+        raise ValueError(f"kudnn {name}: rows must be int32 [R]")
 
 
 # ---- router
@@ -138,39 +127,45 @@ def _route_plan(logits, mask, top_k, normalize) -> MoeRoute:
 
 
 def _route(logits, mask, top_k, normalize):
+    device = logits.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _route(logits, mask, top_k, normalize)
     tokens, experts = logits.shape
     plan = _route_plan(logits, mask, top_k, normalize)
-    device = logits.device
-    with _on(device):
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
-        chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
-        offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-        rows = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
-        slots = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
-        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device) if plan.workspace_bytes else None
-        plan.run(logits, mask, weights, chosen, offsets, rows, slots, ws, _stream(device))
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
+    chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+    rows = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+    slots = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    rc = lib().kudnn_moe_route_run(plan.handle, logits.data_ptr(), _at(mask), weights.data_ptr(), chosen.data_ptr(), offsets.data_ptr(),
+                                   rows.data_ptr(), slots.data_ptr(), _at(_workspace(plan, device)), _stream(device.index))
+    if rc:
+        check(rc)
     return weights, chosen, offsets, rows, slots
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, mask, top_k, normalize):
-        outs = _route(logits, mask, top_k, normalize)
-        # the logits are needed again only for the whole softmax
-        ctx.save_for_backward(logits, mask, outs[0], outs[1])
+    def forward(ctx, logits, mask, top_k, normalize, rest):
+        weights, *order = _route(logits, mask, top_k, normalize)
+        rest += order           # whole numbers: nothing for autograd to follow
+        ctx.save_for_backward(logits, mask, weights, order[0])
         ctx.top_k, ctx.normalize = top_k, normalize
-        ctx.mark_non_differentiable(*outs[1:])
-        return outs
+        return weights
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dweights, *_):
+    def backward(ctx, dweights):
         logits, mask, weights, experts = ctx.saved_tensors
         plan = _route_plan(logits, mask, ctx.top_k, ctx.normalize)
-        with _on(logits.device):
-            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            plan.backward(logits, mask, weights, experts, dweights.contiguous(), dlogits, _stream(logits.device))
-        return dlogits, None, None, None
+        dweights = dweights.contiguous()
+        device = logits.device
+        with torch.cuda.device(device):
+            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+            check(lib().kudnn_moe_route_backward(plan.handle, logits.data_ptr(), _at(mask), weights.data_ptr(), experts.data_ptr(),
+                                                 dweights.data_ptr(), dlogits.data_ptr(), _stream(device.index)))
+        return dlogits, None, None, None, None
 
 
 def route(logits: torch.Tensor, top_k: int, normalize: bool = True, mask: Optional[torch.Tensor] = None) -> Routing:
@@ -181,20 +176,21 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True, mask: Option
     index. weights are the softmax's values, over the sum of the chosen ones if normalize. A token without open experts
     has none and adds no rows. Differentiable in the weights.
     """
-    _need(logits.dim() == 2, "kudnn route: logits must be [tokens, experts]")
+    if logits.dim() != 2 or logits.dtype not in _FLOAT:
+        raise ValueError(f"kudnn route: logits must be [tokens, experts], float32, bfloat16 or float16, got {logits.dtype} {tuple(logits.shape)}")
     _gpu("route", logits, mask)
-    _need(logits.dtype in _FLOAT, f"kudnn route: logits of {logits.dtype}")
     if mask is not None:
-        _need(mask.dtype in (torch.bool, torch.uint8), "kudnn route: mask must be bool or uint8")
         if mask.dim() == 1:
             mask = mask[None, :]
-        _need(mask.dim() == 2 and mask.shape[0] in (1, logits.shape[0]) and mask.shape[1] in (1, logits.shape[1]),
-              "kudnn route: mask must be [tokens or 1, experts or 1]")
+        if (mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 or mask.shape[0] not in (1, logits.shape[0])
+                or mask.shape[1] not in (1, logits.shape[1])):
+            raise ValueError("kudnn route: mask must be bool or uint8 of [tokens or 1, experts or 1]")
         mask = mask.contiguous()
     logits = _matrix(logits)
     normalize = bool(normalize)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(*_Route.apply(logits, mask, top_k, normalize))
+    if logits.requires_grad and torch.is_grad_enabled():
+        rest = []
+        return Routing(_Route.apply(logits, mask, top_k, normalize, rest), *rest)
     return Routing(*_route(logits, mask, top_k, normalize))
 
 
@@ -207,11 +203,16 @@ def _grouped_plan(x, w, rows_out, gather) -> GroupedLinear:
 
 
 def _grouped(x, w, offsets, rows):
-    count = x.shape[0] if rows is None else rows.shape[0]
     device = x.device
-    with _on(device):
-        y = torch.empty((count, w.shape[1]), dtype=x.dtype, device=device)
-        _grouped_plan(x, w, count, rows is not None).run(x, w, offsets, rows, y, _stream(device))
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _grouped(x, w, offsets, rows)
+    count = x.shape[0] if rows is None else rows.shape[0]
+    y = torch.empty((count, w.shape[1]), dtype=x.dtype, device=device)
+    rc = lib().kudnn_grouped_linear_run(_grouped_plan(x, w, count, rows is not None).handle, x.data_ptr(), w.data_ptr(),
+                                        offsets.data_ptr(), _at(rows), y.data_ptr(), _stream(device.index))
+    if rc:
+        check(rc)
     return y
 
 
@@ -229,8 +230,8 @@ class _GroupedLinear(torch.autograd.Function):
         device = x.device
         plan = _grouped_plan(x, w, dy.shape[0], rows is not None)
         dx = dw = None
-        with _on(device):
-            stream = _stream(device)
+        with torch.cuda.device(device):
+            stream = _stream(device.index)
             if ctx.needs_input_grad[0]:
                 dx = torch.empty((dy.shape[0], x.shape[1]), dtype=x.dtype, device=device)
                 plan.backward_input(dy, w, offsets, dx, stream)
@@ -250,17 +251,16 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     offsets, rows, slots as ``route`` gives them. Differentiable in x and weight; with rows, the gradient of x is a sum over
     each token's slots and needs them.
     """
-    _need(x.dim() == 2 and weight.dim() == 3 and x.shape[1] == weight.shape[2],
-          f"kudnn grouped_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or x.dtype not in _HALF or weight.dtype != x.dtype:
+        raise ValueError(f"kudnn grouped_linear: x {x.dtype} {tuple(x.shape)}, weight {weight.dtype} {tuple(weight.shape)}")
     _gpu("grouped_linear", x, weight, offsets, rows, slots)
-    _need(x.dtype in _HALF and weight.dtype == x.dtype, f"kudnn grouped_linear: {x.dtype} x {weight.dtype}")
     _order("grouped_linear", offsets, weight.shape[0], rows)
     xm, w = _matrix(x), _weight(weight)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        if rows is not None and x.requires_grad:
-            _need(slots is not None and slots.dtype == torch.int32 and slots.dim() == 2 and slots.shape[0] == x.shape[0]
-                  and slots.numel() == rows.numel() and slots.is_contiguous(),
-                  "kudnn grouped_linear: the gradient of gathered rows needs slots, int32 [T, k]")
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        if rows is not None and x.requires_grad and not (
+                slots is not None and slots.dtype == torch.int32 and slots.dim() == 2 and slots.shape[0] == x.shape[0]
+                and slots.numel() == rows.numel() and slots.is_contiguous()):
+            raise ValueError("kudnn grouped_linear: the gradient of gathered rows needs slots, int32 [T, k]")
         return _GroupedLinear.apply(xm, w, offsets, rows, slots)
     return _grouped(xm, w, offsets, rows)
 
@@ -269,56 +269,74 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[M, K] -> e4m3 values [M, K] and the f32 scale [M, ceil(K / 128)] of each row's block of 128: amax / 448."""
-    _need(x.dim() == 2 and x.dtype in _FLOAT, "kudnn quantize_rows: a matrix of float32, bfloat16 or float16")
-    device = _gpu("quantize_rows", x)
+    if x.dim() != 2 or x.dtype not in _FLOAT:
+        raise ValueError("kudnn quantize_rows: a matrix of float32, bfloat16 or float16")
+    _gpu("quantize_rows", x)
     x = _matrix(x)
     m, k = x.shape
-    with _on(device):
-        q = torch.empty((m, k), dtype=_F8, device=device)
-        scale = torch.empty((m, (k + 127) // 128), dtype=torch.float32, device=device)
-        _quantize_rows(_matrix_desc(x, _FLOAT[x.dtype]), x, q, k, scale, _stream(device))
+    with torch.cuda.device(x.device):
+        q = torch.empty((m, k), dtype=_F8, device=x.device)
+        scale = torch.empty((m, (k + 127) // 128), dtype=torch.float32, device=x.device)
+        _quantize_rows(_matrix_desc(x, _FLOAT[x.dtype]), x, q, k, scale, _stream(x.device.index))
     return q, scale
 
 
 def quantize_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[N, K] or [E, N, K] -> e4m3 values and the f32 scale [.., ceil(N / 128), ceil(K / 128)] of each 128 x 128 block."""
-    _need(weight.dim() in (2, 3) and weight.dtype in _FLOAT, "kudnn quantize_blocks: float32, bfloat16 or float16 weights")
-    device = _gpu("quantize_blocks", weight)
+    if weight.dim() not in (2, 3) or weight.dtype not in _FLOAT:
+        raise ValueError("kudnn quantize_blocks: float32, bfloat16 or float16 weights of [N, K] or [E, N, K]")
+    _gpu("quantize_blocks", weight)
     w = _weight(weight if weight.dim() == 3 else weight[None])
     e, n, k = w.shape
-    with _on(device):
-        q = torch.empty((e, n, k), dtype=_F8, device=device)
-        scale = torch.empty((e, (n + 127) // 128, (k + 127) // 128), dtype=torch.float32, device=device)
-        _quantize_blocks(_weight_desc(w, _FLOAT[w.dtype]), w, q, scale, _stream(device))
+    with torch.cuda.device(w.device):
+        q = torch.empty((e, n, k), dtype=_F8, device=w.device)
+        scale = torch.empty((e, (n + 127) // 128, (k + 127) // 128), dtype=torch.float32, device=w.device)
+        _quantize_blocks(_weight_desc(w, _FLOAT[w.dtype]), w, q, scale, _stream(w.device.index))
     return (q, scale) if weight.dim() == 3 else (q[0], scale[0])
 
 
+def _fp8_plan(x, w, dtype, bias, grouped, count, gather) -> LinearFp8:
+    """A weight of [N, K] or [E, N, K]."""
+    def make():
+        n, k = w.shape[-2:]
+        wd = _weight_desc(w if w.dim() == 3 else w[None], F8E4M3)
+        return LinearFp8(_matrix_desc(x, F8E4M3 if x.dtype == _F8 else _HALF[x.dtype]), wd, desc([count, n], _FLOAT[dtype]),
+                         desc([1, n], _FLOAT[dtype]) if bias else None, grouped, gather)
+
+    return _plan(("fp8", x.shape, x.stride(), x.dtype, w.shape, w.stride(), dtype, bias, grouped, count, gather), make)
+
+
 def _fp8(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype):
-    device = _gpu(name, x, w, w_scale, bias, offsets, rows, x_scale)
-    e, n, k = w.shape
-    _need(w.dtype == _F8, f"kudnn {name}: weight must be float8_e4m3fn")
-    _need(w_scale.dtype == torch.float32 and w_scale.shape == (e, (n + 127) // 128, (k + 127) // 128),
-          f"kudnn {name}: weight_scale must be float32, one for each block of 128 x 128")
-    quantized = x.dtype == _F8
-    if quantized:
-        _need(x_scale is not None and x_scale.dtype == torch.float32 and x_scale.shape == (x.shape[0], (k + 127) // 128),
-              f"kudnn {name}: x_scale must be float32, one for each row's block of 128")
+    _gpu(name, x, w, w_scale, bias, offsets, rows, x_scale)
+    device = x.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _fp8(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype)
+    n, k = w.shape[-2:]
+    blocks = ((n + 127) // 128, (k + 127) // 128)
+    if w.dtype != _F8 or w_scale.dtype != torch.float32 or w_scale.shape != (*w.shape[:-2], *blocks):
+        raise ValueError(f"kudnn {name}: weight must be float8_e4m3fn and weight_scale float32, one for each block of 128 x 128")
+    if x.dtype == _F8:
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != (x.shape[0], blocks[1]):
+            raise ValueError(f"kudnn {name}: x_scale must be float32, one for each row's block of 128")
         x_scale = x_scale.contiguous()
+        dtype = out_dtype or torch.bfloat16
     else:
-        _need(x.dtype in _HALF and x_scale is None, f"kudnn {name}: x must be bfloat16 or float16, or e4m3 with its x_scale")
-    dtype = out_dtype or (torch.bfloat16 if quantized else x.dtype)
-    _need(dtype in _FLOAT, f"kudnn {name}: output of {dtype}")
-    x, w, w_scale = _matrix(x), _weight(w), w_scale.contiguous()
-    grouped = offsets is not None
+        if x.dtype not in _HALF or x_scale is not None:
+            raise ValueError(f"kudnn {name}: x must be bfloat16 or float16, or e4m3 with its x_scale")
+        dtype = out_dtype or x.dtype
+    if dtype not in _FLOAT:
+        raise ValueError(f"kudnn {name}: output of {dtype}")
+    x, w_scale = _matrix(x), w_scale.contiguous()
+    w = w if w.is_contiguous() else (_weight(w) if w.dim() == 3 else _matrix(w))
     count = x.shape[0] if rows is None else rows.shape[0]
-    key = ("fp8", x.shape, x.stride(), x.dtype, w.shape, w.stride(), dtype, bias is None, grouped, count, rows is None)
-    plan = _plan(key, lambda: LinearFp8(_matrix_desc(x, F8E4M3 if quantized else _HALF[x.dtype]), _weight_desc(w, F8E4M3),
-                                        desc([count, n], _FLOAT[dtype]),
-                                        None if bias is None else desc([1, n], _FLOAT[dtype]), grouped, rows is not None))
-    with _on(device):
-        y = torch.empty((count, n), dtype=dtype, device=device)
-        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=device) if plan.workspace_bytes else None
-        plan.run(x, x_scale, w, w_scale, y, bias, offsets, rows, ws, _stream(device))
+    plan = _fp8_plan(x, w, dtype, bias is not None, offsets is not None, count, rows is not None)
+    y = torch.empty((count, n), dtype=dtype, device=device)
+    ws = _workspace(plan, device)
+    rc = lib().kudnn_linear_fp8_run(plan.handle, x.data_ptr(), _at(x_scale), w.data_ptr(), w_scale.data_ptr(), _at(bias), _at(offsets),
+                                    _at(rows), y.data_ptr(), _at(ws), _stream(device.index))
+    if rc:
+        check(rc)
     return y
 
 
@@ -329,25 +347,27 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
     x: [..., K], bfloat16 or float16 (quantised here as ``quantize_rows`` does), or e4m3 with x_scale; weight: [N, K] and
     weight_scale as ``quantize_blocks`` gives them; bias: [N] of the output's type. out_dtype: x's type, bfloat16 for e4m3 x.
     """
-    _need(weight.dim() == 2 and weight_scale.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
-          f"kudnn linear_fp8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"kudnn linear_fp8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
     if bias is not None:
         dtype = out_dtype or (torch.bfloat16 if x.dtype == _F8 else x.dtype)
-        _need(bias.shape == (weight.shape[0],) and bias.dtype == dtype, "kudnn linear_fp8: bias must be [N] of the output's type")
+        if bias.shape != (weight.shape[0],) or bias.dtype != dtype:
+            raise ValueError("kudnn linear_fp8: bias must be [N] of the output's type")
         bias = bias.contiguous()
-    if x_scale is not None and x_scale.dim() != 2:
+    if x.dim() == 2:
+        return _fp8("linear_fp8", x, weight, weight_scale, bias, None, None, x_scale, out_dtype)
+    if x_scale is not None:
         x_scale = x_scale.reshape(-1, x_scale.shape[-1])
-    y = _fp8("linear_fp8", x2, weight[None], weight_scale[None], bias, None, None, x_scale, out_dtype)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
+    y = _fp8("linear_fp8", x.reshape(-1, x.shape[-1]), weight, weight_scale, bias, None, None, x_scale, out_dtype)
+    return y.reshape(*x.shape[:-1], weight.shape[0])
 
 
 def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, offsets: torch.Tensor,
                        rows: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
                        out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``grouped_linear`` with e4m3 operands and a scale for each block of 128. x as for ``linear_fp8``; weight: [E, N, K]."""
-    _need(x.dim() == 2 and weight.dim() == 3 and x.shape[1] == weight.shape[2],
-          f"kudnn grouped_linear_fp8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise ValueError(f"kudnn grouped_linear_fp8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
     _order("grouped_linear_fp8", offsets, weight.shape[0], rows)
     return _fp8("grouped_linear_fp8", x, weight, weight_scale, None, offsets, rows, x_scale, out_dtype)
 
@@ -362,10 +382,15 @@ def _combine_plan(y, tokens, k) -> MoeCombine:
 
 def _combine(y, weights, slots):
     device = y.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _combine(y, weights, slots)
     tokens, k = slots.shape
-    with _on(device):
-        out = torch.empty((tokens, y.shape[1]), dtype=y.dtype, device=device)
-        _combine_plan(y, tokens, k).run(y, weights, slots, out, _stream(device))
+    out = torch.empty((tokens, y.shape[1]), dtype=y.dtype, device=device)
+    rc = lib().kudnn_moe_combine_run(_combine_plan(y, tokens, k).handle, y.data_ptr(), _at(weights), slots.data_ptr(), out.data_ptr(),
+                                     _stream(device.index))
+    if rc:
+        check(rc)
     return out
 
 
@@ -381,10 +406,11 @@ class _Combine(torch.autograd.Function):
         y, weights, slots = ctx.saved_tensors
         device = y.device
         dout = dout.contiguous()
-        with _on(device):
+        with torch.cuda.device(device):
             dy = torch.empty(y.shape, dtype=y.dtype, device=device) if ctx.needs_input_grad[0] else None
             dw = torch.empty(slots.shape, dtype=torch.float32, device=device) if ctx.needs_input_grad[1] else None
-            _combine_plan(y, *slots.shape).backward(y, weights, slots, dout, dy, dw, _stream(device))
+            check(lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
+                                                   dout.data_ptr(), _at(dy), _at(dw), _stream(device.index)))
         return dy, dw, None
 
 
@@ -395,15 +421,16 @@ def combine(y: torch.Tensor, weights: Optional[torch.Tensor], slots: torch.Tenso
     them, -1 adds nothing. Differentiable in y and weights; the rows of y that no slot takes are the last ones, and get a
     gradient of zero.
     """
-    _need(y.dim() == 2 and y.dtype in _FLOAT, "kudnn combine: y must be a matrix of float32, bfloat16 or float16")
+    if y.dim() != 2 or y.dtype not in _FLOAT:
+        raise ValueError("kudnn combine: y must be a matrix of float32, bfloat16 or float16")
     _gpu("combine", y, weights, slots)
-    _need(slots.dtype == torch.int32 and slots.dim() == 2 and slots.is_contiguous() and slots.shape[1] > 0,
-          "kudnn combine: slots must be int32 [T, k]")
-    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == slots.shape),
-          "kudnn combine: weights must be float32 of slots' shape")
+    if slots.dtype != torch.int32 or slots.dim() != 2 or not slots.is_contiguous() or slots.shape[1] == 0:
+        raise ValueError("kudnn combine: slots must be int32 [T, k]")
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != slots.shape):
+        raise ValueError("kudnn combine: weights must be float32 of slots' shape")
     ym = _matrix(y)
     w = None if weights is None else weights.contiguous()
-    if torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad)):
+    if (y.requires_grad or (w is not None and w.requires_grad)) and torch.is_grad_enabled():
         return _Combine.apply(ym, w, slots)
     return _combine(ym, w, slots)
 

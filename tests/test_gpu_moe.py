@@ -369,15 +369,18 @@ def test_grouped_linear_survives_any_offsets_and_rows():
 
 # ---- 8-bit Linear
 
+INV_448 = torch.tensor(1.0) / torch.tensor(448.0)      # rounded to f32
+
+
 def quant_plain(x):
-    """Values and scales of 1 x 128 blocks by definition (f32 divisions, rounding to nearest even), on the host."""
+    """Values and scales of 1 x 128 blocks by definition (f32 steps, rounded to nearest even), on the host."""
     x = x.float().cpu()
     m, k = x.shape
     kb = (k + 127) // 128
     full = torch.zeros(m, kb * 128)
     full[:, :k] = x
     blocks = full.reshape(m, kb, 128)
-    scale = torch.clamp(blocks.abs().amax(2) / 448.0, min=2.0 ** -126)
+    scale = torch.clamp(blocks.abs().amax(2) * INV_448, min=2.0 ** -126)
     return (blocks / scale[:, :, None]).to(F8).reshape(m, kb * 128)[:, :k], scale
 
 
@@ -411,7 +414,7 @@ def test_quantize_blocks(shape):
         for i in range(s3.shape[1]):
             for j in range(s3.shape[2]):
                 part = w3[e, i * 128:i * 128 + 128, j * 128:j * 128 + 128].float().cpu()
-                scale = torch.clamp(part.abs().amax() / 448.0, min=2.0 ** -126)
+                scale = torch.clamp(part.abs().amax() * INV_448, min=2.0 ** -126)
                 assert float(scale) == float(s3[e, i, j])
                 assert same_bits(q3[e, i * 128:i * 128 + 128, j * 128:j * 128 + 128], (part / scale).to(F8))
 
@@ -461,6 +464,74 @@ def test_grouped_linear_fp8(counts, extra, tokens, width, out, gather):
     y = km.grouped_linear_fp8(x, w, ws, offsets, r)
     near(y, want, mag, width + 3 * (width // 128 + 1), "y")
     assert y.dtype == torch.float16 and float(y[sum(counts):].abs().sum()) == 0.0
+
+
+# counts, K, N, tile: products large enough for the e4m3 matrix instruction, one for each of its kernels. The instruction aligns
+# the products of 8 consecutive indices to the largest of them and drops what lies more than 13 bits below: at most 8 x 2^-13
+# of the largest product, hence of the sum of their magnitudes, on top of the f32 sums' rounding
+LARGE_FP8 = [
+    ([40, 0, 100] + [41] * 61, 2064, 1032, "ring64x128/2 e4m3"),
+    ([90] * 14 + [3, 300], 2048, 2056, "ring128x128/2 e4m3"),
+    ([1030], 2064, 2056, "ring128x128/4 e4m3"),
+    ([1500, 77, 3000, 0], 1040, 2056, "pingpong256x256 e4m3"),
+    ([2500], 2048, 4096, "pingpong256x256 e4m3"),
+]
+
+
+@pytest.mark.parametrize("counts,width,out,tile", LARGE_FP8)
+def test_fp8_products_by_the_e4m3_instruction(counts, width, out, tile):
+    g = gen(width + out)
+    count = sum(counts) + 3
+    offsets, rows = make_order(counts, 3, 777, g)
+    grouped = len(counts) > 1
+    x = (randn(g, 777 if grouped else count, width) * torch.exp(randn(g, 1, width))).bfloat16()
+    w, ws = make_fp8(g, len(counts), out, width)
+    xq, xs = km.quantize_rows(x)
+    plan = K.LinearFp8(K.desc(x.shape, K.BF16), K.desc([len(counts), width, out], K.F8E4M3, "ACB"), K.desc([count, out], K.BF16), None, grouped, grouped)
+    assert plan.describe().endswith("tile=" + tile), plan.describe()
+    if grouped:
+        y = km.grouped_linear_fp8(x, w, ws, offsets, rows)
+        want, mag, *_ = grouped_plain(dequant(xq, xs), dequant(w, ws, 128), offsets, rows, count)
+        assert float(y[sum(counts):].abs().sum()) == 0.0
+    else:
+        y = km.linear_fp8(x, w[0], ws[0])
+        xd, wd = dequant(xq, xs), dequant(w[0], ws[0], 128)
+        want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+        exact = km.linear_fp8(x, w[0], ws[0], out_dtype=torch.float32)      # f32 results are formed exactly
+        near(exact, want, mag, width + 3 * (width // 128 + 1), "f32")
+    near(y, want, mag, width + 3 * (width // 128 + 1) + 2.0 ** 13, "y")
+    # in norm the drops are random and far below the rounding to bf16, 2^-8 / sqrt(12) of a value at most
+    assert float((y.double() - want).norm() / want.norm()) < 2.0 ** -9
+
+
+# counts, K, N, tile: 16-bit products of each forward kernel, at sizes where the rule takes it
+TILES = [
+    ([1] * 8, 2048, 520, "stream16x32/8"),
+    ([1, 2, 0, 1] * 16, 1024, 1032, "stream16x64/8"),
+    ([90], 2056, 4104, "stream64x64/8"),
+    ([20, 31, 0, 26, 22, 24, 30, 28], 1024, 4096, "stream64x64/4"),
+    ([30] * 60 + [0, 90, 5, 1], 520, 2056, "ring64x128/2"),
+    ([70] * 60 + [0, 290, 5, 1], 520, 2056, "ring128x128/2"),
+    ([500], 2056, 4104, "ring128x128/4"),
+    ([500, 1, 700, 900], 2056, 4104, "pingpong256x256"),
+]
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("counts,width,out,tile", TILES)
+def test_grouped_linear_by_each_kernel(counts, width, out, tile, dtype):
+    g = gen(width * 3 + out)
+    offsets, rows = make_order(counts, 2, 333, g)
+    count = sum(counts) + 2
+    x = randn(g, 333, width).to(HALF[dtype])
+    w = (randn(g, len(counts), out, width) * width ** -0.5).to(HALF[dtype])
+    d = K.BF16 if dtype == "bf16" else K.F16
+    plan = K.GroupedLinear(K.desc(x.shape, d), K.desc([len(counts), width, out], d, "ACB"), K.desc([count, out], d), True)
+    assert plan.describe().endswith("tile=" + tile), plan.describe()
+    y = km.grouped_linear(x, w, offsets, rows)
+    want, my, *_ = grouped_plain(x, w, offsets, rows, count)
+    near(y, want, my, width + 1, "y")
+    assert float(y[-2:].abs().sum()) == 0.0
 
 
 def test_fp8_nan_and_infinity_stay_in_their_row():
