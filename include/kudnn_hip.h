@@ -289,14 +289,16 @@ KUDNN_HIP_API int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const 
                                               const kudnn_tensor_desc *y, int gather, kudnn_grouped_linear_t *plan);
 KUDNN_HIP_API int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const void *x, const void *w,
                                            const int32_t *offsets, const int32_t *rows, void *y, void *stream);
+/* Workspace of the two gradients: 0 where N, K and the row pitches are multiples of 8, else room for rows packed to such. */
+KUDNN_HIP_API int64_t kudnn_grouped_linear_workspace_bytes(kudnn_grouped_linear_t plan);
 /* dx[r] = dy[r] x w[e]^T, {R, K} dense in the experts' order (with gather, a token's gradient is the sum over its slots:
  * kudnn_moe_combine_run with NULL weights). */
 KUDNN_HIP_API int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void *dy, const void *w,
-                                                      const int32_t *offsets, void *dx, void *stream);
+                                                      const int32_t *offsets, void *dx, void *workspace, void *stream);
 /* dw[e] = sum over the rows r of expert e of dy[r] x[r]^T, dense [E][N][K]; zero for an expert without rows. */
 KUDNN_HIP_API int kudnn_grouped_linear_backward_weight(kudnn_grouped_linear_t plan, const void *dy, const void *x,
                                                        const int32_t *offsets, const int32_t *rows, void *dw,
-                                                       void *stream);
+                                                       void *workspace, void *stream);
 KUDNN_HIP_API int kudnn_grouped_linear_destroy(kudnn_grouped_linear_t plan);
 
 /* Block scales. A row's block of 128 columns is held as e4m3 values q = round(x / s), s = max(amax * (1 / 448), 2^-126),

@@ -137,9 +137,10 @@ _SIGS = {
     "kudnn_moe_route_backward": ([_P] * 8, ctypes.c_int),
     "kudnn_moe_route_destroy": ([_P], ctypes.c_int),
     "kudnn_grouped_linear_create": ([_D, _D, _D, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "kudnn_grouped_linear_workspace_bytes": ([_P], ctypes.c_int64),
     "kudnn_grouped_linear_run": ([_P] * 7, ctypes.c_int),
-    "kudnn_grouped_linear_backward_input": ([_P] * 6, ctypes.c_int),
-    "kudnn_grouped_linear_backward_weight": ([_P] * 7, ctypes.c_int),
+    "kudnn_grouped_linear_backward_input": ([_P] * 7, ctypes.c_int),
+    "kudnn_grouped_linear_backward_weight": ([_P] * 8, ctypes.c_int),
     "kudnn_grouped_linear_destroy": ([_P], ctypes.c_int),
     "kudnn_quantize_rows": ([_D, _P, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
     "kudnn_quantize_blocks": ([_D, _P, _P, _P, _P], ctypes.c_int),
@@ -343,18 +344,19 @@ class GroupedLinear(_Plan):
     def __init__(self, x, w, y, gather=False):
         super().__init__()
         check(lib().kudnn_grouped_linear_create(_ref(x), _ref(w), _ref(y), int(gather), ctypes.byref(self.handle)))
+        self.workspace_bytes = lib().kudnn_grouped_linear_workspace_bytes(self.handle)
 
     def run(self, x, w, offsets, rows, y, stream=None):
         check(lib().kudnn_grouped_linear_run(self.handle, _ptr(x), _ptr(w), _ptr(offsets), _ptr(rows), _ptr(y),
                                              _stream(stream)))
 
-    def backward_input(self, dy, w, offsets, dx, stream=None):
+    def backward_input(self, dy, w, offsets, dx, stream=None, workspace=None):
         check(lib().kudnn_grouped_linear_backward_input(self.handle, _ptr(dy), _ptr(w), _ptr(offsets), _ptr(dx),
-                                                        _stream(stream)))
+                                                        _ptr(workspace), _stream(stream)))
 
-    def backward_weight(self, dy, x, offsets, rows, dw, stream=None):
+    def backward_weight(self, dy, x, offsets, rows, dw, stream=None, workspace=None):
         check(lib().kudnn_grouped_linear_backward_weight(self.handle, _ptr(dy), _ptr(x), _ptr(offsets), _ptr(rows), _ptr(dw),
-                                                         _stream(stream)))
+                                                         _ptr(workspace), _stream(stream)))
 
 
 class LinearFp8(_Plan):

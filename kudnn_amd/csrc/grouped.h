@@ -46,23 +46,26 @@ inline bool kudnn_grouped_native(int64_t R, int64_t N, int64_t K, int c_dt)
 // The figures are a fit to 322 products timed on MI355X on every kernel (1 to 128 groups of 1 to 4096 rows, K and N = 256 to
 // 8192, 16-bit and e4m3; weights rotated past the Infinity Cache): the choice takes 1.012 times the best kernel's time on average,
 // and more than 1.1 times in 14 of them (1.21 at most). Always 256 x 256 tiles, or one tile of 64 x 64, would take 2 to 5 times.
-inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int64_t K, int dt, int c_dt)
+// any: operands that are not whole 16-byte chunks. They pass through registers, which the 256 x 256 tiles and the 64 x 64 tiles
+// of 8 waves have none left for and the longer ring has no use for; the others stay in the order that the figures give them.
+inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int64_t K, int dt, int c_dt, bool any)
 {
     struct Kind {
         int kind, bm, bn, form, waves;   // waves: that split the sum
         double slots;
         double alone[3], full[3];        // 16-bit; e4m3 exact; e4m3 native (0: none)
         double ends;
+        bool any;
     };
     static const Kind kKinds[] = {
-        {GroupedTile::STREAM, 16, 32, 8, 8, 768, {0.06, 0.13, 0}, {0.26, 0.30, 0}, 1.53},
-        {GroupedTile::STREAM, 16, 64, 8, 8, 512, {0.19, 0.22, 0}, {0.32, 0.38, 0}, 0.91},
-        {GroupedTile::STREAM, 64, 64, 4, 4, 512, {0.29, 0.41, 0}, {0.59, 0.76, 0}, 1.78},
-        {GroupedTile::STREAM, 64, 64, 8, 8, 256, {0.19, 0.25, 0}, {0.31, 0.41, 0}, 2.11},
-        {GroupedTile::RING, 64, 128, 2, 1, 768, {0.78, 1.05, 0.49}, {1.25, 1.85, 1.82}, 1.12},
-        {GroupedTile::RING, 128, 128, 2, 1, 512, {0.84, 1.19, 0.85}, {1.18, 2.56, 1.51}, 0.79},
-        {GroupedTile::RING, 128, 128, 4, 1, 256, {0.53, 1.03, 0.72}, {0.62, 1.30, 0.99}, 2.37},
-        {GroupedTile::PINGPONG, 256, 256, 0, 1, 256, {1.11, 0, 1.44}, {1.11, 0, 2.15}, 1.88},
+        {GroupedTile::STREAM, 16, 32, 8, 8, 768, {0.06, 0.13, 0}, {0.26, 0.30, 0}, 1.53, true},
+        {GroupedTile::STREAM, 16, 64, 8, 8, 512, {0.19, 0.22, 0}, {0.32, 0.38, 0}, 0.91, true},
+        {GroupedTile::STREAM, 64, 64, 4, 4, 512, {0.29, 0.41, 0}, {0.59, 0.76, 0}, 1.78, true},
+        {GroupedTile::STREAM, 64, 64, 8, 8, 256, {0.19, 0.25, 0}, {0.31, 0.41, 0}, 2.11, false},
+        {GroupedTile::RING, 64, 128, 2, 1, 768, {0.78, 1.05, 0.49}, {1.25, 1.85, 1.82}, 1.12, true},
+        {GroupedTile::RING, 128, 128, 2, 1, 512, {0.84, 1.19, 0.85}, {1.18, 2.56, 1.51}, 0.79, true},
+        {GroupedTile::RING, 128, 128, 4, 1, 256, {0.53, 1.03, 0.72}, {0.62, 1.30, 0.99}, 2.37, false},
+        {GroupedTile::PINGPONG, 256, 256, 0, 1, 256, {1.11, 0, 1.44}, {1.11, 0, 2.15}, 1.88, false},
     };
     const bool f8 = dt == KUDNN_DT_F8E4M3, native = f8 && kudnn_grouped_native(R, N, K, c_dt);
     const int col = f8 ? (native ? 2 : 1) : 0;
@@ -72,7 +75,7 @@ inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int6
     GroupedTile best{GroupedTile::STREAM, 16, 64, 8, false, false};
     double bestUs = 0.0;
     for (const Kind &k : kKinds) {
-        if (k.full[col] == 0.0) {
+        if (k.full[col] == 0.0 || (any && !k.any)) {
             continue;
         }
         const double blocks = std::ceil(std::ceil(static_cast<double>(K) * es / 128.0) / k.waves) * k.waves;
@@ -90,24 +93,21 @@ inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int6
     return best;
 }
 
-inline GroupedTile kudnn_grouped_tile(const GroupedArgs &g)
-{
-    const int64_t groups = g.offsets == nullptr ? 1 : (g.E < g.R ? g.E : g.R);
-    return kudnn_grouped_rule(g.R, groups, g.J, g.C, g.dt, g.c_dt);
-}
-
 inline int kudnn_launch_grouped(const GroupedArgs &g, hipStream_t stream)
 {
-    if (!kudnn_grouped_tiled(g)) {
-        return kudnn_launch_grouped_generic(g, stream);
-    }
-    if (g.form != GROUPED_FWD) {
+    const bool whole = kudnn_grouped_tiled(g, true);
+    if (g.form != GROUPED_FWD && whole) {
         return kudnn_launch_grouped_pingpong(g, stream);
     }
-    const GroupedTile t = kudnn_grouped_tile(g);
+    const int64_t rowBytes = g.C * (g.dt == KUDNN_DT_F8E4M3 ? 1 : 2);
+    if (g.form != GROUPED_FWD || (!whole && (rowBytes < 16 || !kudnn_grouped_tiled(g, false)))) {
+        return kudnn_launch_grouped_generic(g, stream);
+    }
+    const int64_t groups = g.offsets == nullptr ? 1 : (g.E < g.R ? g.E : g.R);
+    const GroupedTile t = kudnn_grouped_rule(g.R, groups, g.J, g.C, g.dt, g.c_dt, !whole);
     switch (t.kind) {
-        case GroupedTile::STREAM: return kudnn_launch_grouped_stream(g, t.bm, t.bn, t.form, t.hint, stream);
-        case GroupedTile::RING: return kudnn_launch_grouped_ring(g, t.bm, t.form, t.native, t.hint, stream);
+        case GroupedTile::STREAM: return kudnn_launch_grouped_stream(g, t.bm, t.bn, t.form, t.hint, !whole, stream);
+        case GroupedTile::RING: return kudnn_launch_grouped_ring(g, t.bm, t.form, t.native, t.hint, !whole, stream);
         default: return kudnn_launch_grouped_pingpong(g, stream);
     }
 }

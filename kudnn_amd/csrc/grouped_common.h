@@ -46,6 +46,45 @@ __device__ __forceinline__ void copy_lds(i32x4_t rs, uint32_t voff, uint32_t sof
     }
 }
 
+// Orders LDS accesses of one wave to memory of its own.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 16 bytes at an address that is a multiple of the element size ES only.
+template <int ES>
+__device__ __forceinline__ u32x4_t load16_any(const uint8_t *p)
+{
+    struct __attribute__((packed, aligned(ES))) Any16 {
+        uint32_t w[4];
+    };
+    const Any16 v = *reinterpret_cast<const Any16 *>(p);
+    return u32x4_t{v.w[0], v.w[1], v.w[2], v.w[3]};
+}
+
+// The 16 bytes at p of which only the first `valid` (any number, also none) belong to the row, which is at least 16 long: the
+// rest are zeros. It reads the row's last 16 bytes and shifts them down, so no byte past the row's end is touched.
+template <int ES>
+__device__ __forceinline__ u32x4_t load16_tail(const uint8_t *p, int valid)
+{
+    if (valid >= 16) return load16_any<ES>(p);
+    if (valid <= 0) return u32x4_t{0u, 0u, 0u, 0u};
+    const u32x4_t v = load16_any<ES>(p + valid - 16);
+    uint64_t lo = v.x | static_cast<uint64_t>(v.y) << 32, hi = v.z | static_cast<uint64_t>(v.w) << 32;
+    const int drop = (16 - valid) * 8;      // bits of the row's earlier elements
+    if (drop >= 64) {
+        lo = hi >> (drop - 64);
+        hi = 0;
+    } else {
+        lo = lo >> drop | hi << (64 - drop);
+        hi >>= drop;
+    }
+    return u32x4_t{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32)};
+}
+
 // Four e4m3 bytes as four bf16, exactly.
 __device__ __forceinline__ uint2 widen4(uint32_t w)
 {

@@ -63,13 +63,6 @@ __device__ __forceinline__ uint32_t lds_addr(const uint4 *p)
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)p));
 }
 
-__device__ __forceinline__ void wave_sync()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Eight outputs of a row from column j: one or two 16-byte stores where the row allows it, else element by element.
 __device__ __forceinline__ void store8(const GroupedArgs &g, int64_t at, int64_t j, const float (&v)[8], bool wide)
 {
@@ -558,21 +551,22 @@ void launch_form(const GroupedArgs &g, hipStream_t stream)
 
 }  // namespace
 
-bool kudnn_grouped_tiled(const GroupedArgs &g)
+bool kudnn_grouped_tiled(const GroupedArgs &g, bool whole)
 {
-    const int64_t es = g.dt == KUDNN_DT_F8E4M3 ? 1 : 2, whole = 16 / es;
-    const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    // rows are whole 16-byte chunks apart, from aligned bases, and hold whole chunks
-    bool ok = aligned(g.a) && aligned(g.b) && g.lda % whole == 0 && g.ldb % whole == 0;
-    if (g.form == GROUPED_BWD_W) {
-        // the summed index counts rows: the chunks lie along both outputs' indices. 32-bit offsets of the rows of x (all that
-        // a row may come from) and of the expert's rows
-        const int64_t span = (int64_t(1) << 32) - (int64_t(1) << 20);
-        return ok && g.offsets != nullptr && g.I % whole == 0 && g.J % whole == 0 && g.R < span / (g.lda * es) &&
-               (g.S > g.R ? g.S : g.R) < span / (g.ldb * es);
-    }
-    ok = ok && g.be % whole == 0 && g.C % whole == 0 && (g.form == GROUPED_FWD || g.J % whole == 0);
+    const int64_t es = g.dt == KUDNN_DT_F8E4M3 ? 1 : 2, chunk = whole ? 16 / es : 1;
     const int64_t span = (int64_t(1) << 32) - (int64_t(1) << 20);
+    if (whole && (reinterpret_cast<uintptr_t>(g.a) % 16 != 0 || reinterpret_cast<uintptr_t>(g.b) % 16 != 0)) {
+        return false;
+    }
+    bool ok = g.lda % chunk == 0 && g.ldb % chunk == 0;
+    if (g.form == GROUPED_BWD_W) {
+        // the chunks lie along both of C's indices (of a last part chunk the columns past the end are not stored); offsets of any row
+        // of x and of the expert's rows
+        return ok && g.offsets != nullptr && (g.a_padded || g.I % chunk == 0) && (g.b_padded || g.J % chunk == 0) &&
+               g.R < span / (g.lda * es) && (g.S > g.R ? g.S : g.R) < span / (g.ldb * es);
+    }
+    // chunks of A lie along the sum; those of B too in the forward form, else along C's columns
+    ok = ok && g.be % chunk == 0 && (g.a_padded || g.C % chunk == 0) && (g.form == GROUPED_FWD || g.b_padded || g.J % chunk == 0);
     const int64_t rowsA = g.rows != nullptr ? g.S : 256, rowsB = g.form == GROUPED_FWD ? 256 : g.C;
     return ok && rowsA < span / (g.lda * es) && rowsB < span / (g.ldb * es);
 }

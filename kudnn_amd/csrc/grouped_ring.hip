@@ -29,7 +29,9 @@ __device__ __forceinline__ void copy_words(i32x4_t rs, uint32_t voff, uint32_t s
 }
 
 // HINT: the weights are read by one row tile (non-temporal). NATIVE: e4m3 products by the e4m3 matrix instruction.
-template <int CT, int BM, int WM, int WN, int S, bool HINT, bool NATIVE>
+// REG (two stages): rows of any alignment and length (16 bytes at least) go to LDS through registers, a block ahead, since a
+// copy moves whole aligned chunks only.
+template <int CT, int BM, int WM, int WN, int S, bool HINT, bool NATIVE, bool REG>
 __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs g, int tilesJ)
 {
     constexpr bool F8 = CT == KUDNN_DT_F8E4M3;
@@ -58,10 +60,10 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
     const uint32_t rowBytes = static_cast<uint32_t>(g.C) * ES;
     const int blocks = none ? 0 : static_cast<int>((rowBytes + 127) / 128);
     const bool gather = g.rows != nullptr;
-    const i32x4_t ra = gather ? resource(g.a, static_cast<uint64_t>(g.S) * lda)
-                              : resource(static_cast<const uint8_t *>(g.a) + static_cast<uint64_t>(t.r0) * lda, static_cast<uint64_t>(t.end - t.r0) * lda);
-    const i32x4_t rb = resource(static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES +
-                                    static_cast<uint64_t>(j0) * ldb, static_cast<uint64_t>(BN) * ldb);
+    const uint8_t *baseA = static_cast<const uint8_t *>(g.a) + (gather ? 0u : static_cast<uint64_t>(t.r0) * lda);
+    const uint8_t *baseB = static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES + static_cast<uint64_t>(j0) * ldb;
+    const i32x4_t ra = resource(baseA, static_cast<uint64_t>(gather ? g.S : t.end - t.r0) * lda);
+    const i32x4_t rb = resource(baseB, static_cast<uint64_t>(BN) * ldb);
     // copy q = wave kCopies + i has rows 8 q .. 8 q + 7 of the stage, A's before B's: lane -> row l / 8, slot l % 8, chunk
     // slot ^ ((row / 2) % 8)
     uint32_t vo[kCopies];
@@ -109,6 +111,30 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
         if constexpr (F8) {
             copy_words(rsc, vs, static_cast<uint32_t>(kb) * 4u, to + static_cast<uint32_t>((BM + BN) * 128 + (wave % (BM / 64)) * 256));
         }
+    };
+
+    // the same through registers
+    u32x4_t held[REG ? kCopies : 1];
+    float heldScale = 0.0f;
+    auto load = [&](int kb) __attribute__((always_inline)) {
+        const uint32_t at = static_cast<uint32_t>(kb) * 128u;
+        const bool tail = at + 128u > rowBytes;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int q = wave * kCopies + i;
+            const uint8_t *p = (q < BM / 8 ? baseA : baseB) + at + vo[i];
+            u32x4_t x{0u, 0u, 0u, 0u};
+            if (vo[i] != kOut) {
+                x = tail ? load16_tail<ES>(p, static_cast<int>(rowBytes) - static_cast<int>(at + (chunk0 ^ (4u * (q & 1))) * 16u)) : load16_any<ES>(p);
+            }
+            held[REG ? i : 0] = x;
+        }
+        if constexpr (F8) heldScale = vs != kOut ? g.a_scale[vs / 4u + static_cast<uint32_t>(kb)] : 0.0f;
+    };
+    auto put = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) lds[stage * kStage + (wave * kCopies + i) * 64 + lane] = __builtin_bit_cast(uint4, held[REG ? i : 0]);
+        if constexpr (F8) reinterpret_cast<float *>(lds + stage * kStage + (BM + BN) * 8)[(wave % (BM / 64)) * 64 + lane] = heldScale;
     };
 
     f32x4_t acc[NT][MT];
@@ -189,12 +215,26 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
         }
     };
 
+    if constexpr (REG) {
+        static_assert(S == 2, "one block in use, one written");
+        if (blocks > 0) {
+            load(0);
+            put(0);
+            if (blocks > 1) load(1);
+        }
+        for (int kb = 0; kb < blocks; ++kb) {
+            __syncthreads();     // block kb is written, block kb - 1 has been read
+            if (kb + 1 < blocks) put((kb + 1) & 1);
+            if (kb + 2 < blocks) load(kb + 2);
+            multiply(kb, kb & 1);
+        }
+    }
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) {
+    for (int s = 0; s < S - 1 && !REG; ++s) {
         if (s < blocks) copy(s, s);
     }
     int stage = 0;
-    for (int kb = 0; kb < blocks; ++kb) {
+    for (int kb = 0; kb < blocks && !REG; ++kb) {
         // blocks kb + 1 .. kb + S - 2 may still be on their way
         if (kb + S - 2 < blocks) {
             wait_copies<(S - 2) * kSent>();
@@ -224,22 +264,34 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
     }
 }
 
-template <int CT, int BM, int WM, int WN, int S, bool NATIVE = false>
+template <int CT, int BM, int WM, int WN, int S, bool NATIVE>
 void launch(const GroupedArgs &g, bool hint, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + 127) / 128;
     const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
     if (hint) {
-        grouped_ring_kernel<CT, BM, WM, WN, S, true, NATIVE><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_ring_kernel<CT, BM, WM, WN, S, true, NATIVE, false><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
     } else {
-        grouped_ring_kernel<CT, BM, WM, WN, S, false, NATIVE><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_ring_kernel<CT, BM, WM, WN, S, false, NATIVE, false><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
     }
 }
 
-template <int CT, bool NATIVE = false>
-void launch_tile(const GroupedArgs &g, int bm, int stages, bool hint, hipStream_t stream)
+template <int CT, int BM, int WM, int WN, bool NATIVE>
+void launch_any(const GroupedArgs &g, hipStream_t stream)
 {
-    if (bm == 64) {
+    const int64_t tilesJ = (g.J + 127) / 128;
+    const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    grouped_ring_kernel<CT, BM, WM, WN, 2, false, NATIVE, true><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+}
+
+template <int CT, bool NATIVE = false>
+void launch_tile(const GroupedArgs &g, int bm, int stages, bool hint, bool any, hipStream_t stream)
+{
+    if (any && bm == 64) {
+        launch_any<CT, 64, 2, 2, NATIVE>(g, stream);
+    } else if (any) {
+        launch_any<CT, 128, 2, 4, NATIVE>(g, stream);
+    } else if (bm == 64) {
         launch<CT, 64, 2, 2, 2, NATIVE>(g, hint, stream);
     } else if (stages == 2) {
         launch<CT, 128, 2, 4, 2, NATIVE>(g, hint, stream);
@@ -250,16 +302,16 @@ void launch_tile(const GroupedArgs &g, int bm, int stages, bool hint, hipStream_
 
 }  // namespace
 
-int kudnn_launch_grouped_ring(const GroupedArgs &g, int bm, int stages, bool native, bool hint, hipStream_t stream)
+int kudnn_launch_grouped_ring(const GroupedArgs &g, int bm, int stages, bool native, bool hint, bool any, hipStream_t stream)
 {
     switch (g.dt) {
-        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, stages, hint, stream); break;
-        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, stages, hint, stream); break;
+        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, stages, hint, any, stream); break;
+        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, stages, hint, any, stream); break;
         case KUDNN_DT_F8E4M3:
             if (native) {
-                launch_tile<KUDNN_DT_F8E4M3, true>(g, bm, stages, hint, stream);
+                launch_tile<KUDNN_DT_F8E4M3, true>(g, bm, stages, hint, any, stream);
             } else {
-                launch_tile<KUDNN_DT_F8E4M3>(g, bm, stages, hint, stream);
+                launch_tile<KUDNN_DT_F8E4M3>(g, bm, stages, hint, any, stream);
             }
             break;
         default: return -1;

@@ -31,8 +31,9 @@ using namespace kudnn_dev;
 
 namespace {
 
-// BM x BN tile, W waves. HINT: the weights are read by one row tile (non-temporal).
-template <int CT, int BM, int BN, int W, bool HINT>
+// BM x BN tile, W waves. HINT: the weights are read by one row tile (non-temporal). REG: rows of any alignment and length (16
+// bytes at least) go to LDS through registers, a block ahead, since a copy moves whole aligned chunks only.
+template <int CT, int BM, int BN, int W, bool HINT, bool REG>
 __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, int tilesJ)
 {
     constexpr bool F8 = CT == KUDNN_DT_F8E4M3;
@@ -59,10 +60,10 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     const uint32_t rowBytes = static_cast<uint32_t>(g.C) * ES;
     const int blocks = none ? 0 : static_cast<int>((rowBytes + 127) / 128);
     const bool gather = g.rows != nullptr;
-    const i32x4_t ra = gather ? resource(g.a, static_cast<uint64_t>(g.S) * lda)
-                              : resource(static_cast<const uint8_t *>(g.a) + static_cast<uint64_t>(t.r0) * lda, static_cast<uint64_t>(t.end - t.r0) * lda);
-    const i32x4_t rb = resource(static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES +
-                                    static_cast<uint64_t>(j0) * ldb, static_cast<uint64_t>(BN) * ldb);
+    const uint8_t *baseA = static_cast<const uint8_t *>(g.a) + (gather ? 0u : static_cast<uint64_t>(t.r0) * lda);
+    const uint8_t *baseB = static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES + static_cast<uint64_t>(j0) * ldb;
+    const i32x4_t ra = resource(baseA, static_cast<uint64_t>(gather ? g.S : t.end - t.r0) * lda);
+    const i32x4_t rb = resource(baseB, static_cast<uint64_t>(BN) * ldb);
     // copy i has rows 8 i .. 8 i + 7: lane -> row l / 8, slot l % 8, chunk slot ^ ((row / 2) % 8)
     uint32_t va[BM / 8], vb[BN / 8];
     const uint32_t chunk0 = static_cast<uint32_t>((lane & 7) ^ (lane >> 4));
@@ -92,6 +93,27 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
             const bool in = !tail || (chunk0 ^ (4u * (i & 1))) * 16u < left;
             copy_lds<false>(ra, in ? va[i] : kOut, at, stage + static_cast<uint32_t>(i) * 1024u);
         }
+    };
+    // the same through registers
+    constexpr int kCopies = (BM + BN) / 8;
+    u32x4_t held[REG ? kCopies : 1];
+    auto load = [&](int kb) __attribute__((always_inline)) {
+        const uint32_t at = static_cast<uint32_t>(kb) * 128u;
+        const bool tail = at + 128u > rowBytes;
+#pragma unroll
+        for (int q = 0; q < kCopies; ++q) {
+            const uint32_t v = q < BM / 8 ? va[q < BM / 8 ? q : 0] : vb[q < BM / 8 ? 0 : q - BM / 8];
+            const uint8_t *p = (q < BM / 8 ? baseA : baseB) + at + v;
+            u32x4_t x{0u, 0u, 0u, 0u};
+            if (v != kOut) {
+                x = tail ? load16_tail<ES>(p, static_cast<int>(rowBytes) - static_cast<int>(at + (chunk0 ^ (4u * (q & 1))) * 16u)) : load16_any<ES>(p);
+            }
+            held[REG ? q : 0] = x;
+        }
+    };
+    auto put = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < kCopies; ++q) lds[wave * kStage + q * 64 + lane] = __builtin_bit_cast(uint4, held[REG ? q : 0]);
     };
     // scales: lane l has the row of x that its results have, 16 i + l % 16
     const_float *sw = nullptr;
@@ -176,7 +198,19 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
             }
         }
     };
-    if (wave < blocks) {
+    if (REG && wave < blocks) {
+        load(wave);
+        for (int kb = wave; kb < blocks; kb += W) {
+            Block x;
+            scales(x, kb);
+            put();
+            wave_sync();
+            fetch(x);
+            wave_sync();
+            if (kb + W < blocks) load(kb + W);
+            multiply(x);
+        }
+    } else if (wave < blocks) {
         copy(wave);
         for (int kb = wave; kb < blocks; kb += W) {
             Block x;
@@ -215,40 +249,42 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     }
 }
 
-template <int CT, int BM, int BN, int W>
-void launch(const GroupedArgs &g, bool hint, hipStream_t stream)
+template <int CT, int BM, int BN, int W, bool ANY = true>
+void launch(const GroupedArgs &g, bool hint, bool any, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + BN - 1) / BN;
     const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
-    if (hint) {
-        grouped_stream_kernel<CT, BM, BN, W, true><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+    if (ANY && any) {
+        grouped_stream_kernel<CT, BM, BN, W, false, ANY><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+    } else if (hint) {
+        grouped_stream_kernel<CT, BM, BN, W, true, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
     } else {
-        grouped_stream_kernel<CT, BM, BN, W, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_stream_kernel<CT, BM, BN, W, false, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
     }
 }
 
 template <int CT>
-void launch_tile(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream)
+void launch_tile(const GroupedArgs &g, int bm, int bn, int waves, bool hint, bool any, hipStream_t stream)
 {
     if (bm == 16 && bn == 32) {
-        launch<CT, 16, 32, 8>(g, hint, stream);
+        launch<CT, 16, 32, 8>(g, hint, any, stream);
     } else if (bm == 16) {
-        launch<CT, 16, 64, 8>(g, hint, stream);
+        launch<CT, 16, 64, 8>(g, hint, any, stream);
     } else if (waves == 4) {
-        launch<CT, 64, 64, 4>(g, hint, stream);
+        launch<CT, 64, 64, 4>(g, hint, any, stream);
     } else {
-        launch<CT, 64, 64, 8>(g, hint, stream);
+        launch<CT, 64, 64, 8, false>(g, hint, any, stream);
     }
 }
 
 }  // namespace
 
-int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream)
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, bool any, hipStream_t stream)
 {
     switch (g.dt) {
-        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, waves, hint, stream); break;
-        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, waves, hint, stream); break;
-        case KUDNN_DT_F8E4M3: launch_tile<KUDNN_DT_F8E4M3>(g, bm, bn, waves, hint, stream); break;
+        case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, waves, hint, any, stream); break;
+        case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, waves, hint, any, stream); break;
+        case KUDNN_DT_F8E4M3: launch_tile<KUDNN_DT_F8E4M3>(g, bm, bn, waves, hint, any, stream); break;
         default: return -1;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;

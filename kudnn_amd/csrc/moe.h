@@ -80,19 +80,22 @@ struct GroupedArgs {
     int64_t lda, ldb, ldc;           // row pitches in elements
     int64_t be, ce;                  // pitch of an expert in B (first two forms), in C (last)
     int form, dt, c_dt;              // dt: BF16, F16 or F8E4M3 (GROUPED_FWD only)
+    bool a_padded, b_padded;         // the operand's rows (packed by the library) hold zeros up to a whole 16-byte chunk
 };
 
 // Any sizes, pitches and alignments (grouped_generic.hip).
 int kudnn_launch_grouped_generic(const GroupedArgs &g, hipStream_t stream);
-// Whether the operands are whole 16-byte chunks within 32-bit offsets, as the tiled kernels need them (grouped_pingpong.hip).
-bool kudnn_grouped_tiled(const GroupedArgs &g);
+// Whether offsets within an operand fit 32 bits, as every kernel but the generic one needs, and (`whole`) the operands are whole
+// 16-byte chunks, as the copies to LDS need (grouped_pingpong.hip).
+bool kudnn_grouped_tiled(const GroupedArgs &g, bool whole);
 // 256 x 256 tiles (grouped_pingpong.hip); e4m3 products by the e4m3 matrix instruction.
 int kudnn_launch_grouped_pingpong(const GroupedArgs &g, hipStream_t stream);
 // GROUPED_FWD of few rows, the sum dealt to the waves (grouped_stream.hip); products exact in f32. Tiles (bm, bn) and waves:
-// (16, 32) and (16, 64) with 8, (64, 64) with 4 or 8. hint: the weights are read by one row tile.
-int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, hipStream_t stream);
-// GROUPED_FWD on tiles of bm (64 or 128) rows and 128 columns, a ring of 2 or (128 rows) 4 stages (grouped_ring.hip). native:
-// e4m3 products by the e4m3 matrix instruction, else exact in f32.
-int kudnn_launch_grouped_ring(const GroupedArgs &g, int bm, int stages, bool native, bool hint, hipStream_t stream);
+// (16, 32) and (16, 64) with 8, (64, 64) with 4 or (not `any`) 8. hint: the weights are read by one row tile. any: operands that are not
+// whole chunks, of rows of 16 bytes or more.
+int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, bool any, hipStream_t stream);
+// GROUPED_FWD on tiles of bm (64 or 128) rows and 128 columns, a ring of 2 or (128 rows, not `any`) 4 stages (grouped_ring.hip).
+// native: e4m3 products by the e4m3 matrix instruction, else exact in f32.
+int kudnn_launch_grouped_ring(const GroupedArgs &g, int bm, int stages, bool native, bool hint, bool any, hipStream_t stream);
 
 #endif  // KUDNN_MOE_H

@@ -8,6 +8,7 @@
 
 #include "../../include/kudnn_hip.h"
 #include "grouped.h"
+#include "kernels.h"
 #include "moe.h"
 #include "plan_base.h"
 
@@ -25,6 +26,9 @@ struct kudnn_grouped_linear_plan : PlanBase {
     int64_t S = 0, R = 0, E = 0, K = 0, N = 0, ldx = 0, ldw = 0, we = 0, ldy = 0;
     int dt = 0;
     bool gather = false;
+    // gradients: rows that are not whole 16-byte chunks are packed to a pitch that is (0: read in place). Byte offsets in
+    // the workspace: dy at 0, then w (gradient of x) or x (gradient of w)
+    int64_t packDy = 0, packW = 0, packX = 0, second = 0, workspace = 0;
 };
 
 struct kudnn_linear_fp8_plan : PlanBase {
@@ -107,20 +111,41 @@ int CheckBuffers(const Buffer (&b)[N])
     return KUDNN_STATUS_SUCCESS;
 }
 
-// The forward kernel of a product whose operands are whole 16-byte chunks, for describe().
-std::string TileName(int64_t R, int64_t groups, int64_t N, int64_t K, int dt, int c_dt)
+// The forward kernel of a product from aligned bases, for describe().
+std::string TileName(int64_t R, int64_t groups, int64_t N, int64_t K, int64_t lda, int64_t ldb, int dt, int c_dt)
 {
     const int64_t whole = dt == KUDNN_DT_F8E4M3 ? 16 : 8;
     if (R == 0) {
         return "";
     }
-    if (K % whole != 0) {
+    if (K < whole) {
         return " tile=generic";
     }
-    const GroupedTile t = kudnn_grouped_rule(R, groups < R ? groups : R, N, K, dt, c_dt);
+    const bool any = K % whole != 0 || lda % whole != 0 || ldb % whole != 0;
+    const GroupedTile t = kudnn_grouped_rule(R, groups < R ? groups : R, N, K, dt, c_dt, any);
     return std::string(" tile=") + (t.kind == GroupedTile::STREAM ? "stream" : (t.kind == GroupedTile::RING ? "ring" : "pingpong")) +
-           std::to_string(t.bm) + "x" + std::to_string(t.bn) + (t.form > 0 ? "/" + std::to_string(t.form) : "") +
+           std::to_string(t.bm) + "x" + std::to_string(t.bn) + (t.form > 0 ? "/" + std::to_string(t.form) : "") + (any ? " any" : "") +
            (t.native || (dt == KUDNN_DT_F8E4M3 && t.kind == GroupedTile::PINGPONG) ? " e4m3" : "");
+}
+
+// Rows of a 16-bit operand packed to a pitch of `pitch` elements, zeros past the row.
+int Pack(const void *src, int dt, int64_t rows, int64_t cols, int64_t ld, int64_t batches, int64_t bs, void *dst, int64_t pitch,
+         hipStream_t stream)
+{
+    PackArgs p{};
+    p.src = src;
+    p.src_dt = p.dst_dt = dt;
+    p.rows = rows;
+    p.cols = cols;
+    p.s_r = ld;
+    p.s_k = 1;
+    p.bdim[0] = p.bdim[1] = 1;
+    p.bdim[2] = batches;
+    p.bs[2] = bs;
+    p.dst = dst;
+    p.kp = pitch;
+    p.dst_bstride = rows * pitch;
+    return rows == 0 ? 0 : kudnn_launch_pack(p, batches, stream);
 }
 
 int Launched(int rc, const char *what)
@@ -334,12 +359,24 @@ int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const kudnn_tensor_d
         p->ldy = ldy;
         p->dt = x->dtype;
         p->gather = gather != 0;
+        // few rows, or more experts than a launch of the pack takes, are left to the generic kernel
+        if (E <= 65535 && K >= 8 && N >= 8 && ldw < kMaxSide) {
+            const auto up = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
+            p->packDy = N % 8 != 0 ? up(N, 8) : 0;
+            p->packW = K % 8 != 0 || ldw % 8 != 0 || (E > 1 && we % 8 != 0) ? up(K, 8) : 0;
+            p->packX = K % 8 != 0 || (S > 1 && ldx % 8 != 0) ? up(K, 8) : 0;
+            p->second = up(R * p->packDy * 2, 256);
+            const int64_t w2 = E * N * p->packW * 2, x2 = S * p->packX * 2;
+            p->workspace = p->second + (w2 > x2 ? w2 : x2);
+        }
         p->desc = "grouped_linear E=" + std::to_string(E) + " R=" + std::to_string(R) + " N=" + std::to_string(N) + " K=" +
-                  std::to_string(K) + (p->gather ? " gather" : "") + TileName(R, E, N, K, p->dt, p->dt);
+                  std::to_string(K) + (p->gather ? " gather" : "") + TileName(R, E, N, K, ldx, ldw, p->dt, p->dt);
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });
 }
+
+int64_t kudnn_grouped_linear_workspace_bytes(kudnn_grouped_linear_t plan) { return plan == nullptr ? 0 : plan->workspace; }
 
 int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const void *x, const void *w, const int32_t *offsets,
                              const int32_t *rows, void *y, void *stream)
@@ -383,7 +420,7 @@ int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const void *x, const v
 }
 
 int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void *dy, const void *w, const int32_t *offsets,
-                                        void *dx, void *stream)
+                                        void *dx, void *workspace, void *stream)
 {
     if (plan == nullptr) {
         return Null("grouped Linear: null plan");
@@ -391,13 +428,18 @@ int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void 
     if (plan->R == 0) {
         return KUDNN_STATUS_SUCCESS;
     }
-    if (dy == nullptr || w == nullptr || offsets == nullptr || dx == nullptr) {
+    if (dy == nullptr || w == nullptr || offsets == nullptr || dx == nullptr || (plan->workspace > 0 && workspace == nullptr)) {
         return Null("grouped Linear: one of the buffers is nullptr");
     }
-    const int s = CheckBuffers({Buffer{dy, plan->dt}, Buffer{w, plan->dt}, Buffer{offsets, KUDNN_DT_S32}, Buffer{dx, plan->dt}});
+    const int s = CheckBuffers({Buffer{dy, plan->dt}, Buffer{w, plan->dt}, Buffer{offsets, KUDNN_DT_S32}, Buffer{dx, plan->dt},
+                                Buffer{workspace, KUDNN_DT_S32}});
     if (s != KUDNN_STATUS_SUCCESS) {
         return s;
     }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+        return Bad("grouped Linear: the workspace must be 16-byte aligned");
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
     GroupedArgs g{};
     g.a = dy;
     g.b = w;
@@ -413,28 +455,47 @@ int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void 
     g.be = plan->we;
     g.form = GROUPED_BWD_IN;
     g.dt = g.c_dt = plan->dt;
-    return Launched(kudnn_launch_grouped(g, static_cast<hipStream_t>(stream)), "grouped Linear: launch failed");
+    char *ws = static_cast<char *>(workspace);
+    int rc = 0;
+    if (plan->packDy > 0) {
+        rc = Pack(dy, plan->dt, plan->R, plan->N, plan->N, 1, 0, ws, plan->packDy, st);
+        g.a = ws;
+        g.lda = plan->packDy;
+        g.a_padded = true;
+    }
+    if (rc == 0 && plan->packW > 0) {
+        rc = Pack(w, plan->dt, plan->N, plan->K, plan->ldw, plan->E, plan->we, ws + plan->second, plan->packW, st);
+        g.b = ws + plan->second;
+        g.ldb = plan->packW;
+        g.be = plan->N * plan->packW;
+        g.b_padded = true;
+    }
+    return Launched(rc == 0 ? kudnn_launch_grouped(g, st) : rc, "grouped Linear: launch failed");
 }
 
 int kudnn_grouped_linear_backward_weight(kudnn_grouped_linear_t plan, const void *dy, const void *x, const int32_t *offsets,
-                                         const int32_t *rows, void *dw, void *stream)
+                                         const int32_t *rows, void *dw, void *workspace, void *stream)
 {
     if (plan == nullptr) {
         return Null("grouped Linear: null plan");
     }
     const bool some = plan->R > 0;
     if ((some && dy == nullptr) || (x == nullptr && some && plan->S > 0) || offsets == nullptr || dw == nullptr ||
-        (some && plan->gather && rows == nullptr)) {
+        (some && plan->gather && rows == nullptr) || (some && plan->workspace > 0 && workspace == nullptr)) {
         return Null("grouped Linear: one of the buffers is nullptr");
     }
     if (!plan->gather && rows != nullptr) {
         return Bad("grouped Linear: rows were given to a plan made without gather");
     }
     const int s = CheckBuffers({Buffer{dy, plan->dt}, Buffer{x, plan->dt}, Buffer{offsets, KUDNN_DT_S32},
-                                Buffer{rows, KUDNN_DT_S32}, Buffer{dw, plan->dt}});
+                                Buffer{rows, KUDNN_DT_S32}, Buffer{dw, plan->dt}, Buffer{workspace, KUDNN_DT_S32}});
     if (s != KUDNN_STATUS_SUCCESS) {
         return s;
     }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+        return Bad("grouped Linear: the workspace must be 16-byte aligned");
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
     GroupedArgs g{};
     g.a = dy;
     g.b = x;
@@ -452,7 +513,21 @@ int kudnn_grouped_linear_backward_weight(kudnn_grouped_linear_t plan, const void
     g.ce = plan->N * plan->K;
     g.form = GROUPED_BWD_W;
     g.dt = g.c_dt = plan->dt;
-    return Launched(kudnn_launch_grouped(g, static_cast<hipStream_t>(stream)), "grouped Linear: launch failed");
+    char *ws = static_cast<char *>(workspace);
+    int rc = 0;
+    if (some && plan->packDy > 0) {
+        rc = Pack(dy, plan->dt, plan->R, plan->N, plan->N, 1, 0, ws, plan->packDy, st);
+        g.a = ws;
+        g.lda = plan->packDy;
+        g.a_padded = true;
+    }
+    if (some && rc == 0 && plan->packX > 0) {
+        rc = Pack(x, plan->dt, plan->S, plan->K, plan->ldx, 1, 0, ws + plan->second, plan->packX, st);
+        g.b = ws + plan->second;
+        g.ldb = plan->packX;
+        g.b_padded = true;
+    }
+    return Launched(rc == 0 ? kudnn_launch_grouped(g, st) : rc, "grouped Linear: launch failed");
 }
 
 int kudnn_grouped_linear_destroy(kudnn_grouped_linear_t plan)
@@ -596,7 +671,7 @@ int kudnn_linear_fp8_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc 
             p->workspace = p->scaleOffset + S * ((K + 127) / 128) * static_cast<int64_t>(sizeof(float));
         }
         p->desc = "linear_fp8 E=" + std::to_string(E) + " R=" + std::to_string(R) + " N=" + std::to_string(N) + " K=" +
-                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "") + TileName(R, E, N, K, KUDNN_DT_F8E4M3, p->ydt);
+                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "") + TileName(R, E, N, K, p->xdt == KUDNN_DT_F8E4M3 ? ldx : kudnn_fp8_pitch(K), ldw, KUDNN_DT_F8E4M3, p->ydt);
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });

@@ -232,14 +232,15 @@ class _GroupedLinear(torch.autograd.Function):
         dx = dw = None
         with torch.cuda.device(device):
             stream = _stream(device.index)
+            ws = _workspace(plan, device)
             if ctx.needs_input_grad[0]:
                 dx = torch.empty((dy.shape[0], x.shape[1]), dtype=x.dtype, device=device)
-                plan.backward_input(dy, w, offsets, dx, stream)
+                plan.backward_input(dy, w, offsets, dx, stream, ws)
                 if rows is not None:
                     dx = _combine(dx, None, slots)
             if ctx.needs_input_grad[1]:
                 dw = torch.empty(w.shape, dtype=w.dtype, device=device)
-                plan.backward_weight(dy, x, offsets, rows, dw, stream)
+                plan.backward_weight(dy, x, offsets, rows, dw, stream, ws)
         return dx, dw, None, None, None
 
 

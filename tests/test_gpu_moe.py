@@ -268,8 +268,9 @@ def test_grouped_linear(counts, extra, tokens, width, out, gather, dtype):
                            K.desc([count, out], K.BF16 if dtype == "bf16" else K.F16), gather)
     stream = torch.cuda.current_stream()
     gx, gw = torch.full((count, width), math.nan, dtype=dt, device=DEV), torch.full(w.shape, math.nan, dtype=dt, device=DEV)
-    plan.backward_input(dy, w, offsets, gx, stream)
-    plan.backward_weight(dy, x, offsets, r, gw, stream)
+    ws = torch.full((plan.workspace_bytes,), 255, dtype=torch.uint8, device=DEV)     # NaN in 16 bits
+    plan.backward_input(dy, w, offsets, gx, stream, ws)
+    plan.backward_weight(dy, x, offsets, r, gw, stream, ws)
     near(gx, dxs, mx, out + 1, "dx")
     near(gw, dw, mw, max(counts) + 1, "dw")
 

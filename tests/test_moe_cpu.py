@@ -91,6 +91,10 @@ def test_runs_refuse_missing_and_host_buffers():
     refused(K.BAD_ARGUMENTS, lambda: g.run(at, at, at, None, at))
     refused(K.NULL_POINTER, lambda: g.backward_input(at, None, at, at))
     refused(K.NULL_POINTER, lambda: g.backward_weight(at, at, at, None, None))
+    odd = K.GroupedLinear(K.desc([4, 9], K.BF16), K.desc([2, 9, 11], K.BF16, "ACB"), K.desc([4, 11], K.BF16))
+    assert g.workspace_bytes == 0 and odd.workspace_bytes == 256 + 2 * 11 * 16 * 2
+    refused(K.NULL_POINTER, lambda: odd.backward_input(at, at, at, at))                      # no workspace
+    refused(K.NULL_POINTER, lambda: odd.backward_weight(at, at, at, None, at))
     f = K.LinearFp8(K.desc([4, 8], K.BF16), K.desc([8, 8], K.F8E4M3, "BA"), K.desc([4, 8], K.BF16))
     refused(K.NULL_POINTER, lambda: f.run(at, None, at, at, at))                             # no workspace
     refused(K.BAD_ARGUMENTS, lambda: f.run(at, at, at, at, at, workspace=at))                # a scale for bf16 x
