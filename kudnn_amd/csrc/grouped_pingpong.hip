@@ -107,10 +107,11 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     int e, aFirst, bFirst, begin, end, sumLen;
     if constexpr (FORM == GROUPED_BWD_W) {
         const int tilesI = static_cast<int>((ga.I + kBN - 1) / kBN), perExpert = tilesI * tilesJ;
-        const int lid = xcd_remap(blockIdx.x, gridDim.x);
-        e = lid / perExpert;
+        // all XCDs on one expert at a time: its tiles take as long as it has rows, so an expert of its own would leave the XCD
+        // of the fullest one behind (8 experts of 700 to 4000 rows, 4096 x 4096: 768 us that way)
+        e = static_cast<int>(blockIdx.x) / perExpert;
         int ti, tj;
-        grouped_tile(lid - e * perExpert, tilesI, tilesJ, order, ti, tj);
+        grouped_tile(xcd_remap(static_cast<int>(blockIdx.x) - e * perExpert, perExpert), tilesI, tilesJ, order, ti, tj);
         begin = clamp_row(ga.offsets[e], R);
         end = clamp_row(ga.offsets[e + 1], R);
         aFirst = tj * kBM;                          // columns of x, C's columns
@@ -222,21 +223,23 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             tailAt[1] = ((lane & 7) ^ (4 + (lane >> 4))) * static_cast<int>(16u / ES);
         }
     }
-    // Gathered rows of x in the weight's gradient change with the k-tile: lane l < 16 holds the byte offset of row l of the
-    // wave's 16 in the k-tile to come. Only group 0 loads them, which waits for all its copies in every phase anyway.
+    // Gathered rows of x in the weight's gradient change with the k-tile: lane l < 16 holds the row number of row l of the
+    // wave's 16 in the k-tile to come, as loaded: nothing is computed from it before the next memory phase, so the load has a
+    // whole phase to arrive. Only group 0 loads them, which waits for all its copies in every phase anyway.
     const bool gatherK = AK && ga.rows != nullptr;
-    uint32_t rowOff = kOut;
+    int rowNo = -1;
     auto load_rows = [&](int t) __attribute__((always_inline)) {
         if (gatherK && g == 0) {
             const int r = begin + t * 64 + p * 16 + (lane & 15);
-            const int64_t s = r < end ? source_row(ga, r) : -1;
-            rowOff = s >= 0 ? static_cast<uint32_t>(s) * ldb : kOut;
+            rowNo = -1;
+            if (r < end) rowNo = ga.rows[r];
         }
     };
     auto stream = [&](int t, uint32_t lds) __attribute__((always_inline)) {
         const uint32_t soff = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(t) * kStep);
         lds = __builtin_amdgcn_readfirstlane(lds + static_cast<uint32_t>(p * 8) * 1024u);
         if (AK && gatherK && g == 0) {
+            const uint32_t rowOff = static_cast<uint32_t>(rowNo) < static_cast<uint32_t>(ga.S) ? static_cast<uint32_t>(rowNo) * ldb : kOut;
             sfor<8>([&](auto jc) __attribute__((always_inline)) {
                 constexpr int j = decltype(jc)::value;
                 const uint32_t r0 = __builtin_amdgcn_readlane(rowOff, 2 * j), r1 = __builtin_amdgcn_readlane(rowOff, 2 * j + 1);
@@ -512,6 +515,14 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 }
             }
         }
+        // the bias of this lane's columns, the same for its rows
+        float bias[8];
+        if constexpr (F8) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                bias[q] = ga.bias != nullptr && colW + colU + col8 + q < ga.J ? load_elem(ga.bias, ga.c_dt, colW + colU + col8 + q) : 0.0f;
+            }
+        }
         wave_sync();
 #pragma unroll
         for (int ps = 0; ps < 4; ++ps) {
@@ -520,9 +531,9 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             const float4 lo = *reinterpret_cast<const float4 *>(sp), hi = *reinterpret_cast<const float4 *>(sp + 4);
             float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
             if (row < rowEnd && col < ga.J) {
-                if (F8 && ga.bias != nullptr) {
+                if constexpr (F8) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) v[q] += col + q < ga.J ? load_elem(ga.bias, ga.c_dt, col + q) : 0.0f;
+                    for (int q = 0; q < 8; ++q) v[q] += bias[q];
                 }
                 store8(ga, cBase + row * ga.ldc + col, col, v, wide);
             }

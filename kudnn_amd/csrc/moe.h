@@ -21,6 +21,7 @@ struct RouteArgs {
     int32_t *experts, *offsets, *rows, *slots;
     uint8_t *counts;              // [workgroups][counts_ld]: a workgroup's rows of each expert; unused with one workgroup
     int counts_ld;
+    bool wide;                    // set by the launcher: rows can be read 4 values at a time
 };
 int kudnn_launch_moe_route(const RouteArgs &a, hipStream_t stream);
 
@@ -32,6 +33,7 @@ struct RouteBackwardArgs {
     const float *weights, *dweights;
     const int32_t *experts;
     void *dlogits;                // dense [T][E]
+    bool wide, wide_out;          // set by the launcher: rows can be read and written 4 values at a time
 };
 int kudnn_launch_moe_route_backward(const RouteBackwardArgs &a, hipStream_t stream);
 

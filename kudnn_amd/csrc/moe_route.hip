@@ -1,9 +1,10 @@
 // Router of a mixture of experts: softmax over the experts of each token, its k largest, and the tokens in the order of
 // their experts; and the gradient of the weights.
 //
-// A workgroup takes 64 tokens. A group of L lanes holds a token's logits in registers (V = up to 16 a lane) and picks the
-// largest k times, each time by a butterfly over the L lanes of a 64-bit key: the logit's bits, made to order as signed
-// integers, above the complement of the expert's index, so that ties go to the lowest index and the result is unique.
+// A workgroup takes 64 tokens. A group of L lanes holds a token's logits in registers (V = up to 16 neighbours a lane, in
+// 16-byte loads where the rows allow it) and picks the largest k times, each time by a butterfly over the L lanes: the larger key
+// (the logit's bits, made to order as signed integers) wins, of equal ones the lower index, so the result is unique. Butterflies
+// within 16 lanes are DPP moves.
 //
 // The order by expert is a counting sort without atomics whose order could change the result. A token takes an expert at
 // most once, so a row's place among its workgroup's rows of one expert is the number of earlier tokens that took it: each
@@ -32,6 +33,87 @@ __device__ __forceinline__ int order_key(float x)
 __device__ __forceinline__ float key_value(int key)
 {
     return key == INT32_MAX ? u2f(0x7fc00000u) : u2f(static_cast<uint32_t>(key < 0 ? key ^ 0x7fffffff : key));
+}
+
+// The value of the lane across: distance 1 and 2 within a quad; at 4 and 8 the mirrored lane, which stands for the group across
+// once all lanes of each smaller group hold the same; 16 and 32 by the permute network.
+template <int D>
+__device__ __forceinline__ int across(int v)
+{
+    if constexpr (D == 1) {
+        return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, false);     // quad_perm [1, 0, 3, 2]
+    } else if constexpr (D == 2) {
+        return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, false);     // quad_perm [2, 3, 0, 1]
+    } else if constexpr (D == 4) {
+        return __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, false);    // row_half_mirror
+    } else if constexpr (D == 8) {
+        return __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, false);    // row_mirror
+    } else {
+        return __shfl_xor(v, D);
+    }
+}
+template <int D>
+__device__ __forceinline__ float across(float v) { return u2f(static_cast<uint32_t>(across<D>(static_cast<int>(f2u(v))))); }
+
+// f(distance) for the steps of a butterfly over L lanes.
+template <int L, int D = 1, typename F>
+__device__ __forceinline__ void butterfly(F &&f)
+{
+    if constexpr (D < L) {
+        f(std::integral_constant<int, D>{});
+        butterfly<L, 2 * D>(f);
+    }
+}
+
+// V logits of a row from index i0 on as f32 and whether each is there and open by the mask. wide: 16-byte loads of logits, and
+// loads of V mask bytes, are aligned and inside the row.
+template <int V>
+__device__ __forceinline__ void load_logits(const void *logits, int dt, int64_t row, int64_t ld, const uint8_t *mask, int64_t maskRow,
+                                            int64_t mask_se, int i0, int E, bool wide, float (&x)[V], bool (&open)[V])
+{
+    if (wide && i0 + V <= E) {
+        if constexpr (V >= 4) {
+            if (dt == KUDNN_DT_F32) {
+                const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(logits) + row * ld + i0);
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    const float4 r = p[q];
+                    x[4 * q] = r.x, x[4 * q + 1] = r.y, x[4 * q + 2] = r.z, x[4 * q + 3] = r.w;
+                }
+            } else {
+                const uint2 *p = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(logits) + row * ld + i0);
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    const uint2 r = p[q];
+                    const uint32_t w[4] = {r.x & 0xffffu, r.x >> 16, r.y & 0xffffu, r.y >> 16};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[4 * q + i] = dt == KUDNN_DT_BF16 ? u2f(w[i] << 16) : f16_to_f32(static_cast<uint16_t>(w[i]));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) open[i] = true;
+        if (mask != nullptr) {
+            if constexpr (V >= 4) {
+                const uint32_t *m = reinterpret_cast<const uint32_t *>(mask + maskRow + i0);
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    const uint32_t r = m[q];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) open[4 * q + i] = ((r >> (8 * i)) & 255u) != 0u;
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = i0 + i;
+        open[i] = e < E && (mask == nullptr || mask[maskRow + e * mask_se] != 0);
+        x[i] = open[i] ? load_elem(logits, dt, row * ld + e) : 0.0f;
+    }
 }
 
 struct Shared {
@@ -104,28 +186,23 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a, int single
     for (int t = threadIdx.x / L; t < n; t += kThreads / L) {
         const int64_t tok = t0 + t;
         int key[V];
+        {
+            float x[V];
+            bool open[V];
+            load_logits<V>(a.logits, a.dt, tok, a.ld, a.mask, tok * a.mask_st, a.mask_se, sub * V, a.E, a.wide, x, open);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = i * L + sub;
-            key[i] = kClosed;
-            if (e < a.E && (a.mask == nullptr || a.mask[tok * a.mask_st + e * a.mask_se] != 0)) {
-                const float x = load_elem(a.logits, a.dt, tok * a.ld + e);
-                key[i] = x == -__builtin_inff() ? kClosed : order_key(x);
-            }
+            for (int i = 0; i < V; ++i) key[i] = open[i] && x[i] != -__builtin_inff() ? order_key(x[i]) : kClosed;
         }
-        float top = 0.0f;
         if (!a.normalize) {
             int m = kClosed;
 #pragma unroll
             for (int i = 0; i < V; ++i) m = max(m, key[i]);
-#pragma unroll
-            for (int d = 1; d < L; d <<= 1) m = max(m, __shfl_xor(m, d));
-            top = key_value(m);
+            butterfly<L>([&](auto d) __attribute__((always_inline)) { m = max(m, across<decltype(d)::value>(m)); });
+            const float top = key_value(m);
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) s += key[i] == kClosed ? 0.0f : fast_exp(key_value(key[i]) - top);
-#pragma unroll
-            for (int d = 1; d < L; d <<= 1) s += __shfl_xor(s, d);
+            butterfly<L>([&](auto d) __attribute__((always_inline)) { s += across<decltype(d)::value>(s); });
             if (sub == 0) sh.sum[t] = s;
         }
         for (int j = 0; j < a.k; ++j) {
@@ -137,16 +214,15 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a, int single
                     bi = i;
                 }
             }
-            int be = bi * L + sub;
-#pragma unroll
-            for (int d = 1; d < L; d <<= 1) {
-                const int ok = __shfl_xor(bk, d), oe = __shfl_xor(be, d);
+            int be = sub * V + bi;
+            butterfly<L>([&](auto d) __attribute__((always_inline)) {
+                const int ok = across<decltype(d)::value>(bk), oe = across<decltype(d)::value>(be);
                 const bool take = ok > bk || (ok == bk && oe < be);
                 bk = take ? ok : bk;
                 be = take ? oe : be;
-            }
+            });
 #pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = i * L + sub == be ? kClosed : key[i];
+            for (int i = 0; i < V; ++i) key[i] = sub * V + i == be ? kClosed : key[i];
             if (sub == 0) {
                 sh.key[t * a.k + j] = bk;
                 sh.expert[t * a.k + j] = static_cast<short>(bk == kClosed ? -1 : be);
@@ -276,7 +352,7 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteBackwardA
         dot += g * w;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (i * L + sub == e) {
+            if (sub * V + i == e) {
                 d[i] = g;
                 p[i] = w;
             }
@@ -284,38 +360,65 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteBackwardA
     }
     if (!a.normalize) {
         float x[V], top = -__builtin_inff(), s = 0.0f;
+        bool open[V];
+        load_logits<V>(a.logits, a.dt, tok, a.ld, a.mask, tok * a.mask_st, a.mask_se, sub * V, a.E, a.wide, x, open);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int e = i * L + sub;
-            const bool open = e < a.E && (a.mask == nullptr || a.mask[tok * a.mask_st + e * a.mask_se] != 0);
-            x[i] = open ? load_elem(a.logits, a.dt, tok * a.ld + e) : -__builtin_inff();
+            x[i] = open[i] ? x[i] : -__builtin_inff();
             top = fmaxf(top, x[i]);
         }
-#pragma unroll
-        for (int m = 1; m < L; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+        butterfly<L>([&](auto m) __attribute__((always_inline)) { top = fmaxf(top, across<decltype(m)::value>(top)); });
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             p[i] = x[i] == -__builtin_inff() ? 0.0f : fast_exp(x[i] - top);
             s += p[i];
         }
-#pragma unroll
-        for (int m = 1; m < L; m <<= 1) s += __shfl_xor(s, m);
+        butterfly<L>([&](auto m) __attribute__((always_inline)) { s += across<decltype(m)::value>(s); });
         const float inv = s == 0.0f ? 0.0f : 1.0f / s;
 #pragma unroll
         for (int i = 0; i < V; ++i) p[i] = p[i] == 0.0f ? 0.0f : p[i] * inv;  // 0 stays 0 beside a NaN in the sum
     }
+    float dx[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) dx[i] = p[i] == 0.0f ? 0.0f : p[i] * (d[i] - dot);
+    const int e0 = sub * V;
+    if (V % 4 == 0 && a.wide_out && e0 + V <= a.E) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            if (a.dt == KUDNN_DT_F32) {
+                reinterpret_cast<float4 *>(static_cast<float *>(a.dlogits) + tok * a.E + e0)[q] =
+                    make_float4(dx[4 * q], dx[4 * q + 1], dx[4 * q + 2], dx[4 * q + 3]);
+            } else {
+                uint32_t w[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float lo = dx[4 * q + 2 * i], hi = dx[4 * q + 2 * i + 1];
+                    w[i] = a.dt == KUDNN_DT_BF16 ? pack_bf16x2_rne(lo, hi) : static_cast<uint32_t>(f32_to_f16_rne(lo)) | (static_cast<uint32_t>(f32_to_f16_rne(hi)) << 16);
+                }
+                reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.dlogits) + tok * a.E + e0)[q] = make_uint2(w[0], w[1]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int e = i * L + sub;
-        if (e < a.E) store_elem(a.dlogits, a.dt, tok * a.E + e, p[i] == 0.0f ? 0.0f : p[i] * (d[i] - dot));
+        if (e0 + i < a.E) store_elem(a.dlogits, a.dt, tok * a.E + e0 + i, dx[i]);
     }
+}
+
+// Whether a row's logits and mask bytes can be read 4 values at a time.
+bool wide_rows(const void *logits, int dt, int64_t ld, const uint8_t *mask, int64_t mask_st, int64_t mask_se)
+{
+    const uintptr_t size = dt == KUDNN_DT_F32 ? 16 : 8;
+    return reinterpret_cast<uintptr_t>(logits) % size == 0 && ld % 4 == 0 &&
+           (mask == nullptr || (reinterpret_cast<uintptr_t>(mask) % 4 == 0 && mask_st % 4 == 0 && mask_se == 1));
 }
 
 // The lanes and registers a token takes: 8 lanes up to 128 experts, so that a wave holds 8 tokens.
 template <typename F>
 int with_shape(int E, F &&f)
 {
-    if (E <= 16) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+    if (E <= 32) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
     if (E <= 64) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
     if (E <= 128) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
     if (E <= 256) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
@@ -325,8 +428,10 @@ int with_shape(int E, F &&f)
 
 }  // namespace
 
-int kudnn_launch_moe_route(const RouteArgs &a, hipStream_t stream)
+int kudnn_launch_moe_route(const RouteArgs &args, hipStream_t stream)
 {
+    RouteArgs a = args;
+    a.wide = wide_rows(a.logits, a.dt, a.ld, a.mask, a.mask_st, a.mask_se);
     const int blocks = a.T <= kTokens ? 1 : static_cast<int>((a.T + kTokens - 1) / kTokens);  // no tokens: zero offsets
     const int single = blocks <= 1 ? 1 : 0;
     with_shape(a.E, [&](auto l, auto v) {
@@ -339,8 +444,11 @@ int kudnn_launch_moe_route(const RouteArgs &a, hipStream_t stream)
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-int kudnn_launch_moe_route_backward(const RouteBackwardArgs &a, hipStream_t stream)
+int kudnn_launch_moe_route_backward(const RouteBackwardArgs &args, hipStream_t stream)
 {
+    RouteBackwardArgs a = args;
+    a.wide = wide_rows(a.logits, a.dt, a.ld, a.mask, a.mask_st, a.mask_se);
+    a.wide_out = a.E % 4 == 0 && reinterpret_cast<uintptr_t>(a.dlogits) % 16 == 0;
     with_shape(a.E, [&](auto l, auto v) {
         constexpr int perBlock = kThreads / decltype(l)::value;
         route_backward_kernel<decltype(l)::value, decltype(v)::value>
