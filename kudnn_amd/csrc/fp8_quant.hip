@@ -6,7 +6,7 @@
 // s is at most 2^-23 of itself off amax / 448, so |x / s| stays below 464, where e4m3 would leave its range: no clamp is needed. A NaN in a block
 // stays NaN and an infinity becomes one (inf / inf), which the product hands on.
 // Bound by HBM: x is read once, a byte an element is written.
-#include "device_common.h"
+#include "e4m3.h"
 #include "moe.h"
 
 using namespace kudnn_dev;
@@ -14,16 +14,6 @@ using namespace kudnn_dev;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kInvMax = 1.0f / 448.0f, kTiny = 1.17549435e-38f;
-
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax * kInvMax, kTiny); }
-
-// Four values as e4m3 bytes, lowest first.
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d)
-{
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
-}
 
 // 16 lanes a block of a row, 8 elements a lane; 16 blocks a workgroup.
 template <int DT, bool WIDE>
@@ -36,25 +26,8 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void *x, 
     const int64_t row = block / KB, kb = block - row * KB;
     const int64_t col = kb * 128 + (threadIdx.x % 16) * 8;
     float v[8];
+    load_eight<DT>(x, row * ldx + col, K - col, WIDE, v);
     float amax = 0.0f;
-    if (WIDE && col + 8 <= K) {
-        if constexpr (DT == KUDNN_DT_F32) {
-            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(x) + row * ldx + col);
-            const float4 lo = p[0], hi = p[1];
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-        } else {
-            const uint4 r = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(x) + row * ldx + col);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = DT == KUDNN_DT_BF16 ? u2f(w[i] << 16) : f16_to_f32(static_cast<uint16_t>(w[i]));
-                v[2 * i + 1] = DT == KUDNN_DT_BF16 ? u2f(w[i] & 0xffff0000u) : f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = col + i < K ? load_elem(x, DT, row * ldx + col + i) : 0.0f;
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll

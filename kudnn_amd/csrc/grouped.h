@@ -93,6 +93,18 @@ inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int6
     return best;
 }
 
+// Whether an e4m3 product of R rows leaves the quantisation of x to the workgroups: each takes the whole of its rows (up to 48 KB
+// of e4m3 in LDS) before its first block of weights has arrived, where a launch of its own and the wait for it cost 3.5 us of 15
+// (1 x 4096 x 14336).
+inline bool kudnn_grouped_fused(int64_t R, int64_t groups, int64_t N, int64_t K, int c_dt, bool any)
+{
+    if (R > 16 || K < 16 || R * kudnn_fp8_pitch(K) > 49152) {
+        return false;
+    }
+    const GroupedTile t = kudnn_grouped_rule(R, groups, N, K, KUDNN_DT_F8E4M3, c_dt, any);
+    return t.kind == GroupedTile::STREAM && t.bm == 16;
+}
+
 inline int kudnn_launch_grouped(const GroupedArgs &g, hipStream_t stream)
 {
     const bool whole = kudnn_grouped_tiled(g, true);

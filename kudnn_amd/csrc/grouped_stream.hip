@@ -25,6 +25,7 @@
 // the end of the sum have an offset outside and read as zeros.
 #include <type_traits>
 
+#include "e4m3.h"
 #include "grouped_common.h"
 
 using namespace kudnn_dev;
@@ -32,8 +33,9 @@ using namespace kudnn_dev;
 namespace {
 
 // BM x BN tile, W waves. HINT: the weights are read by one row tile (non-temporal). REG: rows of any alignment and length (16
-// bytes at least) go to LDS through registers, a block ahead, since a copy moves whole aligned chunks only.
-template <int CT, int BM, int BN, int W, bool HINT, bool REG>
+// bytes at least) go to LDS through registers, a block ahead, since a copy moves whole aligned chunks only. XDT (e4m3, 16 rows):
+// 0, or the type of rows of x that this workgroup quantises itself, into `rowsLds`, while its first weights are on their way.
+template <int CT, int BM, int BN, int W, bool HINT, bool REG, int XDT>
 __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, int tilesJ)
 {
     constexpr bool F8 = CT == KUDNN_DT_F8E4M3;
@@ -41,6 +43,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     constexpr int kStage = (BM + BN) * 8;                        // 16-byte chunks of a wave's block: A's rows, then B's
     constexpr int kSums = W * BM * kPitch / 4;                   // the sums reuse the stages
     __shared__ uint4 lds[W * kStage > kSums ? W * kStage : kSums];
+    extern __shared__ uint4 rowsLds[];                           // XDT: the tile's rows as e4m3, then their scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row16 = lane & 15, grp = lane >> 4;
 
@@ -60,6 +63,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     const uint32_t rowBytes = static_cast<uint32_t>(g.C) * ES;
     const int blocks = none ? 0 : static_cast<int>((rowBytes + 127) / 128);
     const bool gather = g.rows != nullptr;
+    // (XDT: A is not copied)
     const uint8_t *baseA = static_cast<const uint8_t *>(g.a) + (gather ? 0u : static_cast<uint64_t>(t.r0) * lda);
     const uint8_t *baseB = static_cast<const uint8_t *>(g.b) + static_cast<uint64_t>(e) * static_cast<uint64_t>(g.be) * ES + static_cast<uint64_t>(j0) * ldb;
     const i32x4_t ra = resource(baseA, static_cast<uint64_t>(gather ? g.S : t.end - t.r0) * lda);
@@ -89,7 +93,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
             copy_lds<HINT>(rb, in ? vb[i] : kOut, at, stage + static_cast<uint32_t>(BM / 8 + i) * 1024u);
         }
 #pragma unroll
-        for (int i = 0; i < BM / 8; ++i) {
+        for (int i = 0; i < (XDT ? 0 : BM / 8); ++i) {
             const bool in = !tail || (chunk0 ^ (4u * (i & 1))) * 16u < left;
             copy_lds<false>(ra, in ? va[i] : kOut, at, stage + static_cast<uint32_t>(i) * 1024u);
         }
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
         const uint32_t at = static_cast<uint32_t>(kb) * 128u;
         const bool tail = at + 128u > rowBytes;
 #pragma unroll
-        for (int q = 0; q < kCopies; ++q) {
+        for (int q = XDT ? BM / 8 : 0; q < kCopies; ++q) {
             const uint32_t v = q < BM / 8 ? va[q < BM / 8 ? q : 0] : vb[q < BM / 8 ? 0 : q - BM / 8];
             const uint8_t *p = (q < BM / 8 ? baseA : baseB) + at + v;
             u32x4_t x{0u, 0u, 0u, 0u};
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     };
     auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < kCopies; ++q) lds[wave * kStage + q * 64 + lane] = __builtin_bit_cast(uint4, held[REG ? q : 0]);
+        for (int q = XDT ? BM / 8 : 0; q < kCopies; ++q) lds[wave * kStage + q * 64 + lane] = __builtin_bit_cast(uint4, held[REG ? q : 0]);
     };
     // scales: lane l has the row of x that its results have, 16 i + l % 16
     const_float *sw = nullptr;
@@ -134,21 +138,62 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     };
     const uint4 *mine = lds + wave * kStage;
     const int sw16 = (row16 >> 1) & 7;
-    auto fetch = [&](Block &x) __attribute__((always_inline)) {
+    const int pitch = static_cast<int>(KB) * 8;                  // XDT: 16-byte chunks of a row
+    const int held16 = t.end - t.r0 < BM ? t.end - t.r0 : BM;     // rows of the tile
+    auto fetch = [&](Block &x, int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int slot = (grp + 4 * h) ^ sw16;
 #pragma unroll
             for (int j = 0; j < NT; ++j) x.b[j][h] = __builtin_bit_cast(u32x4_t, mine[(BM + j * 16 + row16) * 8 + slot]);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x.a[i][h] = __builtin_bit_cast(u32x4_t, mine[(i * 16 + row16) * 8 + slot]);
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (XDT != 0) {
+                    x.a[i][h] = u32x4_t{0u, 0u, 0u, 0u};
+                    if (row16 < held16) x.a[i][h] = __builtin_bit_cast(u32x4_t, rowsLds[row16 * pitch + kb * 8 + grp + 4 * h]);
+                } else {
+                    x.a[i][h] = __builtin_bit_cast(u32x4_t, mine[(i * 16 + row16) * 8 + slot]);
+                }
+            }
         }
     };
     auto scales = [&](Block &x, int kb) __attribute__((always_inline)) {
         if constexpr (F8) {
             x.sw = sw[kb];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x.sx[i] = sxAt[i] != kOut ? g.a_scale[sxAt[i] + static_cast<uint32_t>(kb)] : 0.0f;
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (XDT != 0) {
+                    const float *scale = reinterpret_cast<const float *>(rowsLds + g.R * pitch);
+                    x.sx[i] = row16 < held16 ? scale[row16 * KB + static_cast<uint32_t>(kb)] : 0.0f;
+                } else {
+                    x.sx[i] = sxAt[i] != kOut ? g.a_scale[sxAt[i] + static_cast<uint32_t>(kb)] : 0.0f;
+                }
+            }
+        }
+    };
+    // XDT: 16 lanes quantise a block of a row
+    auto quantize = [&]() __attribute__((always_inline)) {
+        if constexpr (XDT != 0) {
+            const bool aligned = g.lda % 8 == 0 && reinterpret_cast<uintptr_t>(g.a) % 16 == 0;
+            const int units = none ? 0 : held16 * static_cast<int>(KB), sub = threadIdx.x & 15;
+            for (int u = threadIdx.x >> 4; u < units; u += W * 4) {
+                const int r = u / static_cast<int>(KB), kb = u - r * static_cast<int>(KB);
+                const int64_t s = source_row(g, t.r0 + r), col = kb * 128 + sub * 8;
+                float v[8];
+                load_eight<XDT>(g.a, s * g.lda + col, s < 0 ? 0 : g.C - col, aligned, v);
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+                const float sc = block_scale(amax);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = v[i] / sc;
+                reinterpret_cast<uint2 *>(rowsLds)[(r * pitch + kb * 8) * 2 + sub] =
+                    make_uint2(pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7]));
+                if (sub == 0) reinterpret_cast<float *>(rowsLds + g.R * pitch)[r * KB + kb] = sc;
+            }
+            __syncthreads();
         }
     };
 
@@ -198,25 +243,31 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
             }
         }
     };
+    if (wave < blocks) {
+        if constexpr (REG) {
+            load(wave);
+        } else {
+            copy(wave);
+        }
+    }
+    quantize();
     if (REG && wave < blocks) {
-        load(wave);
         for (int kb = wave; kb < blocks; kb += W) {
             Block x;
             scales(x, kb);
             put();
             wave_sync();
-            fetch(x);
+            fetch(x, kb);
             wave_sync();
             if (kb + W < blocks) load(kb + W);
             multiply(x);
         }
     } else if (wave < blocks) {
-        copy(wave);
         for (int kb = wave; kb < blocks; kb += W) {
             Block x;
             scales(x, kb);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's copies of block kb have landed
-            fetch(x);
+            fetch(x, kb);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and left LDS before the next ones arrive there
             if (kb + W < blocks) copy(kb + W);
             multiply(x);
@@ -249,17 +300,19 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     }
 }
 
-template <int CT, int BM, int BN, int W, bool ANY = true>
+template <int CT, int BM, int BN, int W, bool ANY = true, int XDT = 0>
 void launch(const GroupedArgs &g, bool hint, bool any, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + BN - 1) / BN;
     const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    // the rows of a tile and their scales
+    const size_t lds = XDT != 0 ? static_cast<size_t>(g.R * (kudnn_fp8_pitch(g.C) + (g.C + 127) / 128 * 4)) : 0;
     if (ANY && any) {
-        grouped_stream_kernel<CT, BM, BN, W, false, ANY><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_stream_kernel<CT, BM, BN, W, false, ANY, XDT><<<tiles, W * 64, lds, stream>>>(g, static_cast<int>(tilesJ));
     } else if (hint) {
-        grouped_stream_kernel<CT, BM, BN, W, true, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_stream_kernel<CT, BM, BN, W, true, false, XDT><<<tiles, W * 64, lds, stream>>>(g, static_cast<int>(tilesJ));
     } else {
-        grouped_stream_kernel<CT, BM, BN, W, false, false><<<tiles, W * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
+        grouped_stream_kernel<CT, BM, BN, W, false, false, XDT><<<tiles, W * 64, lds, stream>>>(g, static_cast<int>(tilesJ));
     }
 }
 
@@ -277,10 +330,29 @@ void launch_tile(const GroupedArgs &g, int bm, int bn, int waves, bool hint, boo
     }
 }
 
+template <int XDT>
+void launch_fused(const GroupedArgs &g, int bn, bool any, hipStream_t stream)
+{
+    // at most 16 rows: the weights are read once
+    if (bn == 32) {
+        launch<KUDNN_DT_F8E4M3, 16, 32, 8, true, XDT>(g, true, any, stream);
+    } else {
+        launch<KUDNN_DT_F8E4M3, 16, 64, 8, true, XDT>(g, true, any, stream);
+    }
+}
+
 }  // namespace
 
 int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, bool any, hipStream_t stream)
 {
+    if (g.x_dt == KUDNN_DT_BF16) {
+        launch_fused<KUDNN_DT_BF16>(g, bn, any, stream);
+        return hipGetLastError() == hipSuccess ? 0 : -1;
+    }
+    if (g.x_dt == KUDNN_DT_F16) {
+        launch_fused<KUDNN_DT_F16>(g, bn, any, stream);
+        return hipGetLastError() == hipSuccess ? 0 : -1;
+    }
     switch (g.dt) {
         case KUDNN_DT_BF16: launch_tile<KUDNN_DT_BF16>(g, bm, bn, waves, hint, any, stream); break;
         case KUDNN_DT_F16: launch_tile<KUDNN_DT_F16>(g, bm, bn, waves, hint, any, stream); break;

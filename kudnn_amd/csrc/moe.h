@@ -82,6 +82,7 @@ struct GroupedArgs {
     int64_t lda, ldb, ldc;           // row pitches in elements
     int64_t be, ce;                  // pitch of an expert in B (first two forms), in C (last)
     int form, dt, c_dt;              // dt: BF16, F16 or F8E4M3 (GROUPED_FWD only)
+    int x_dt;                        // not 0: A is not quantised yet but of this 16-bit type (a_scale unused); see below
     bool a_padded, b_padded;         // the operand's rows (packed by the library) hold zeros up to a whole 16-byte chunk
 };
 
@@ -95,6 +96,7 @@ int kudnn_launch_grouped_pingpong(const GroupedArgs &g, hipStream_t stream);
 // GROUPED_FWD of few rows, the sum dealt to the waves (grouped_stream.hip); products exact in f32. Tiles (bm, bn) and waves:
 // (16, 32) and (16, 64) with 8, (64, 64) with 4 or (not `any`) 8. hint: the weights are read by one row tile. any: operands that are not
 // whole chunks, of rows of 16 bytes or more.
+// With g.x_dt: e4m3 products whose workgroups quantise their rows of x themselves, 16 rows a tile (kudnn_grouped_fused).
 int kudnn_launch_grouped_stream(const GroupedArgs &g, int bm, int bn, int waves, bool hint, bool any, hipStream_t stream);
 // GROUPED_FWD on tiles of bm (64 or 128) rows and 128 columns, a ring of 2 or (128 rows, not `any`) 4 stages (grouped_ring.hip).
 // native: e4m3 products by the e4m3 matrix instruction, else exact in f32.

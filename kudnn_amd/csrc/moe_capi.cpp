@@ -35,7 +35,7 @@ struct kudnn_linear_fp8_plan : PlanBase {
     kudnn_linear_fp8_plan() : PlanBase(PLAN_LINEAR_FP8) {}
     int64_t S = 0, R = 0, E = 0, K = 0, N = 0, ldx = 0, ldw = 0, we = 0, ldy = 0, scaleOffset = 0, workspace = 0;
     int xdt = 0, ydt = 0;
-    bool grouped = false, gather = false, hasBias = false;
+    bool grouped = false, gather = false, hasBias = false, fused = false;   // fused: the product quantises x itself
 };
 
 struct kudnn_moe_combine_plan : PlanBase {
@@ -666,12 +666,15 @@ int kudnn_linear_fp8_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc 
         p->grouped = grouped != 0;
         p->gather = gather != 0;
         p->hasBias = hasBias;
-        if (p->xdt != KUDNN_DT_F8E4M3) {
+        // weights that 32-bit offsets do not reach go through the generic kernel, which takes e4m3 rows
+        p->fused = R > 0 && p->xdt != KUDNN_DT_F8E4M3 && ldw < kMaxSide &&
+                   kudnn_grouped_fused(R, p->grouped ? (E < R ? E : R) : 1, N, K, p->ydt, K % 16 != 0 || ldw % 16 != 0);
+        if (p->xdt != KUDNN_DT_F8E4M3 && !p->fused) {
             p->scaleOffset = S * kudnn_fp8_pitch(K);
             p->workspace = p->scaleOffset + S * ((K + 127) / 128) * static_cast<int64_t>(sizeof(float));
         }
         p->desc = "linear_fp8 E=" + std::to_string(E) + " R=" + std::to_string(R) + " N=" + std::to_string(N) + " K=" +
-                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "") + TileName(R, E, N, K, p->xdt == KUDNN_DT_F8E4M3 ? ldx : kudnn_fp8_pitch(K), ldw, KUDNN_DT_F8E4M3, p->ydt);
+                  std::to_string(K) + (p->grouped ? (p->gather ? " grouped gather" : " grouped") : "") + (p->fused ? " fused" : "") + TileName(R, E, N, K, p->xdt == KUDNN_DT_F8E4M3 ? ldx : kudnn_fp8_pitch(K), ldw, KUDNN_DT_F8E4M3, p->ydt);
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });
@@ -712,7 +715,9 @@ int kudnn_linear_fp8_run(kudnn_linear_fp8_t plan, const void *x, const float *x_
     g.a = x;
     g.a_scale = x_scale;
     g.lda = plan->ldx;
-    if (!quantized) {
+    if (plan->fused) {
+        g.x_dt = plan->xdt;
+    } else if (!quantized) {
         char *ws = static_cast<char *>(workspace);
         float *scale = reinterpret_cast<float *>(ws + plan->scaleOffset);
         if (plan->S > 0 &&
@@ -740,6 +745,11 @@ int kudnn_linear_fp8_run(kudnn_linear_fp8_t plan, const void *x, const float *x_
     g.form = GROUPED_FWD;
     g.dt = KUDNN_DT_F8E4M3;
     g.c_dt = plan->ydt;
+    if (plan->fused) {
+        const bool any = plan->K % 16 != 0 || plan->ldw % 16 != 0 || (plan->E > 1 && plan->we % 16 != 0) || reinterpret_cast<uintptr_t>(w) % 16 != 0;
+        const GroupedTile t = kudnn_grouped_rule(g.R, plan->grouped ? (g.E < g.R ? g.E : g.R) : 1, g.J, g.C, g.dt, g.c_dt, any);
+        return Launched(kudnn_launch_grouped_stream(g, 16, t.bm == 16 ? t.bn : 64, 8, true, any, st), "8-bit Linear: launch failed");
+    }
     return Launched(kudnn_launch_grouped(g, st), "8-bit Linear: launch failed");
 }
 

@@ -535,6 +535,27 @@ def test_grouped_linear_by_each_kernel(counts, width, out, tile, dtype):
     assert float(y[-2:].abs().sum()) == 0.0
 
 
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_fp8_rows_quantised_by_the_product(dtype):
+    """Few rows are quantised by the product itself: the same values, and the same bits as from quantize_rows."""
+    g = gen(31)
+    for m, k, n, pad, e in [(1, 4096, 1040, 0, 0), (16, 2048, 96, 0, 0), (7, 203, 50, 5, 0), (3, 16, 16, 1, 0), (5, 1000, 70, 0, 6), (9, 384, 300, 8, 40)]:
+        wide = (randn(g, m, k + pad) * torch.exp(randn(g, 1, k + pad))).to(HALF[dtype])
+        x = wide[:, pad:] if pad != 8 else wide[:, :k]
+        x[0, :min(k, 128)] = 0
+        w, ws = make_fp8(g, max(1, e), n, k)
+        xq, xs = km.quantize_rows(x)
+        if e:
+            rows = torch.randint(-1, m, (12,), generator=g, device=DEV, dtype=torch.int32)
+            offsets = torch.tensor([0] + sorted(torch.randint(0, 12, (e,), generator=torch.Generator().manual_seed(m)).tolist()), dtype=torch.int32, device=DEV)
+            got = km.grouped_linear_fp8(x, w, ws, offsets, rows, out_dtype=torch.float32)
+            same = km.grouped_linear_fp8(xq, w, ws, offsets, rows, x_scale=xs, out_dtype=torch.float32)
+        else:
+            got = km.linear_fp8(x, w[0], ws[0], out_dtype=torch.float32)
+            same = km.linear_fp8(xq, w[0], ws[0], x_scale=xs, out_dtype=torch.float32)
+        assert torch.equal(got, same)
+
+
 def test_fp8_nan_and_infinity_stay_in_their_row():
     g = gen(8)
     for m, k, n in [(4, 256, 64), (40, 256, 64), (300, 512, 512)]:

@@ -50,7 +50,9 @@ def test_linear_fp8_refusals():
     f8 = K.F8E4M3
     x, w, y = K.desc([6, 200], K.BF16), K.desc([200, 24], f8, "BA"), K.desc([6, 24], K.F32)
     p = K.LinearFp8(x, w, y)
-    assert p.workspace_bytes == 6 * 256 + 6 * 2 * 4
+    assert p.workspace_bytes == 0 and " fused" in p.describe()                              # few rows: quantised by the product
+    p = K.LinearFp8(K.desc([60, 200], K.BF16), w, K.desc([60, 24], K.F32))
+    assert p.workspace_bytes == 60 * 256 + 60 * 2 * 4 and " fused" not in p.describe()
     assert K.LinearFp8(K.desc([6, 200], f8), w, y, K.desc([1, 24], K.F32)).workspace_bytes == 0
     wg = K.desc([3, 200, 24], f8, "ACB")
     K.LinearFp8(x, wg, y, None, True), K.LinearFp8(x, wg, K.desc([12, 24], K.F16), None, True, True)
@@ -95,7 +97,7 @@ def test_runs_refuse_missing_and_host_buffers():
     assert g.workspace_bytes == 0 and odd.workspace_bytes == 256 + 2 * 11 * 16 * 2
     refused(K.NULL_POINTER, lambda: odd.backward_input(at, at, at, at))                      # no workspace
     refused(K.NULL_POINTER, lambda: odd.backward_weight(at, at, at, None, at))
-    f = K.LinearFp8(K.desc([4, 8], K.BF16), K.desc([8, 8], K.F8E4M3, "BA"), K.desc([4, 8], K.BF16))
+    f = K.LinearFp8(K.desc([40, 8], K.BF16), K.desc([8, 8], K.F8E4M3, "BA"), K.desc([40, 8], K.BF16))
     refused(K.NULL_POINTER, lambda: f.run(at, None, at, at, at))                             # no workspace
     refused(K.BAD_ARGUMENTS, lambda: f.run(at, at, at, at, at, workspace=at))                # a scale for bf16 x
     refused(K.BAD_ARGUMENTS, lambda: f.run(at, None, at, at, at, workspace=at))
