@@ -5,6 +5,9 @@
 // A thread holds 16 bytes of a row (8 16-bit or 4 f32 values) and walks the token's k rows, so every access is a whole
 // line of consecutive lanes; rows that are not whole 16-byte pieces take the same kernel with one element a thread.
 // Sums over j run in j's order and dot products in a fixed tree, so results do not depend on timing.
+// What passes through once is read and written non-temporally: 8192 tokens x 4 rows of 4096 bf16 take 60 us forward
+// (335 MB, 5.6 TB/s; 73 us with cached accesses) and 130 us backward (604 MB, 4.6 TB/s; 144 us cached), where a plain copy
+// of 2 GiB reaches 4.9 TB/s.
 #include "device_common.h"
 #include "moe.h"
 
@@ -14,16 +17,22 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int DT, int VEC>
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
+
+// STREAM: read or written once, so it need not stay in the caches (non-temporal).
+template <int DT, int VEC, bool STREAM>
 __device__ __forceinline__ void load_vec(const void *p, int64_t i, float (&v)[VEC])
 {
     if constexpr (VEC == 1) {
         v[0] = load_elem(p, DT, i);
     } else if constexpr (DT == KUDNN_DT_F32) {
-        const float4 r = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        const v4f_t *at = reinterpret_cast<const v4f_t *>(static_cast<const float *>(p) + i);
+        const v4f_t r = STREAM ? __builtin_nontemporal_load(at) : *at;
         v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
     } else {
-        const uint4 r = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        const v4u_t *at = reinterpret_cast<const v4u_t *>(static_cast<const uint16_t *>(p) + i);
+        const v4u_t r = STREAM ? __builtin_nontemporal_load(at) : *at;
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -39,7 +48,7 @@ __device__ __forceinline__ void store_vec(void *p, int64_t i, const float (&v)[V
     if constexpr (VEC == 1) {
         store_elem(p, DT, i, v[0]);
     } else if constexpr (DT == KUDNN_DT_F32) {
-        *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+        __builtin_nontemporal_store(v4f_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<v4f_t *>(static_cast<float *>(p) + i));
     } else {
         uint32_t w[4];
 #pragma unroll
@@ -48,7 +57,7 @@ __device__ __forceinline__ void store_vec(void *p, int64_t i, const float (&v)[V
                                        : static_cast<uint32_t>(f32_to_f16_rne(v[2 * q])) |
                                              (static_cast<uint32_t>(f32_to_f16_rne(v[2 * q + 1])) << 16);
         }
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        __builtin_nontemporal_store(v4u_t{w[0], w[1], w[2], w[3]}, reinterpret_cast<v4u_t *>(static_cast<uint16_t *>(p) + i));
     }
 }
 
@@ -72,15 +81,27 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a)
         float sum[VEC];
 #pragma unroll
         for (int q = 0; q < VEC; ++q) sum[q] = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t s = slot_of(a, t, j);
-            if (s < 0) continue;
-            const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
-            float v[VEC];
-            load_vec<DT, VEC>(a.y, s * a.ldy + col, v);
+        // four rows at a time on their way; a row without a slot is not read
+        for (int j0 = 0; j0 < a.k; j0 += 4) {
+            float v[4][VEC], w[4];
+            bool there[4];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) sum[q] = fmaf(w, v[q], sum[q]);
+            for (int j = 0; j < 4; ++j) {
+                const int64_t s = j0 + j < a.k ? slot_of(a, t, j0 + j) : -1;
+                there[j] = s >= 0;
+                w[j] = 1.0f;
+                if (there[j]) {
+                    if (a.weights != nullptr) w[j] = a.weights[t * a.k + j0 + j];
+                    load_vec<DT, VEC, true>(a.y, s * a.ldy + col, v[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (there[j]) {
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) sum[q] = fmaf(w[j], v[j][q], sum[q]);
+                }
+            }
         }
         store_vec<DT, VEC>(a.out, t * a.ldo + col, sum);
     }
@@ -119,9 +140,9 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs 
         if (s >= 0) {
             for (int64_t col = threadIdx.x * VEC; col < a.N; col += kThreads * VEC) {
                 float g[VEC], v[VEC];
-                load_vec<DT, VEC>(a.dout, t * a.N + col, g);
+                load_vec<DT, VEC, false>(a.dout, t * a.N + col, g);
                 if (a.dweights != nullptr) {
-                    load_vec<DT, VEC>(a.y, s * a.ldy + col, v);
+                    load_vec<DT, VEC, true>(a.y, s * a.ldy + col, v);
 #pragma unroll
                     for (int q = 0; q < VEC; ++q) dot = fmaf(g[q], v[q], dot);
                 }
