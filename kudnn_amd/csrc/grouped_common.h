@@ -137,12 +137,15 @@ __device__ __forceinline__ int clamp_row(int v, int R) { return v < 0 ? 0 : (v >
 
 // Row tiles of all experts and of the rest, as one wave sees them: 64 experts at a time, a scan over the lanes. Offsets are
 // clamped to [0, R], so any contents stay inside the buffers. With up to 64 experts the offsets are read once.
+// HALVES: an expert's last tile, if it has at most bm / 2 rows, is not counted among the tiles but among the halves.
+template <bool HALVES = false>
 class RowTiles {
 public:
     __device__ __forceinline__ RowTiles(const int32_t *offsets, int E, int R, int bm) : offsets_(offsets), E_(E), R_(R), bm_(bm)
     {
         if (offsets == nullptr) {   // one group of all rows
-            total_ = experts_ = (R + bm - 1) / bm;
+            total_ = experts_ = whole(R);
+            halves_ = half(R) ? 1 : 0;
             return;
         }
         for (int base = 0; base < E; base += 64) experts_ = scan(base, experts_);
@@ -151,6 +154,29 @@ public:
         total_ = experts_ + (R - rest_ + bm - 1) / bm;
     }
     __device__ __forceinline__ int total() const { return total_; }
+    __device__ __forceinline__ int halves() const { return halves_; }
+    // Half number `want` < halves().
+    __device__ __forceinline__ RowTile find_half(int want)
+    {
+        RowTile t{0, 0, R_, whole(R_) * bm_};
+        for (int base = 0; offsets_ != nullptr && base < E_; base += 64) {
+            if (E_ > 64) scan(base, 0);
+            const bool mine = half(hi_ - lo_);
+            const unsigned long long who = __ballot(mine);
+            const int before = __builtin_popcountll(who & ((1ull << (threadIdx.x & 63)) - 1ull));
+            const unsigned long long is = __ballot(mine && before == want);
+            if (is != 0ull) {
+                const int src = __ffsll(is) - 1;
+                t.e = base + src;
+                t.begin = __builtin_amdgcn_readlane(lo_, src);
+                t.end = __builtin_amdgcn_readlane(hi_, src);
+                t.r0 = t.begin + whole(t.end - t.begin) * bm_;
+                break;
+            }
+            want -= __builtin_popcountll(who);
+        }
+        return t;
+    }
     // Tile number `want` < total(). Its members are the same in every lane.
     __device__ __forceinline__ RowTile find(int want)
     {
@@ -175,6 +201,8 @@ public:
     }
 
 private:
+    __device__ __forceinline__ bool half(int n) const { return HALVES && n > 0 && (n - 1) % bm_ < bm_ / 2; }
+    __device__ __forceinline__ int whole(int n) const { return n <= 0 ? 0 : (n + bm_ - 1) / bm_ - (half(n) ? 1 : 0); }
     // Expert base + lane: its rows, its tiles, and the number of tiles before; returns the number up to the 64th.
     __device__ __forceinline__ int scan(int base, int before)
     {
@@ -184,7 +212,8 @@ private:
             lo_ = clamp_row(offsets_[e], R_);
             hi_ = clamp_row(offsets_[e + 1], R_);
         }
-        tiles_ = hi_ > lo_ ? (hi_ - lo_ + bm_ - 1) / bm_ : 0;
+        tiles_ = whole(hi_ - lo_);
+        if constexpr (HALVES) halves_ += __builtin_popcountll(__ballot(half(hi_ - lo_)));
         int incl = tiles_;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -195,7 +224,7 @@ private:
         return before + __shfl(incl, 63);
     }
     const int32_t *offsets_;
-    int E_, R_, bm_, total_ = 0, experts_ = 0, rest_ = 0;
+    int E_, R_, bm_, total_ = 0, experts_ = 0, rest_ = 0, halves_ = 0;
     int lo_ = 0, hi_ = 0, tiles_ = 0, first_ = 0;
 };
 

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void grouped_generic_kernel(GroupedArgs g, int
         c0 = g.offsets == nullptr ? 0 : clamp_row(g.offsets[e], R);
         cEnd = g.offsets == nullptr ? R : clamp_row(g.offsets[e + 1], R);
     } else {
-        RowTiles tiles(g.offsets, static_cast<int>(g.E), static_cast<int>(g.R), kT);
+        RowTiles<> tiles(g.offsets, static_cast<int>(g.E), static_cast<int>(g.R), kT);
         const int want = static_cast<int>(blockIdx.x) / tilesJ;
         if (want >= tiles.total()) return;
         const RowTile t = tiles.find(want);

@@ -9,7 +9,7 @@
 //
 //   GROUPED_FWD     A = rows of x (gathered), B = rows of W[e]; both contiguous along the sum.
 //   GROUPED_BWD_IN  A = rows of dy, B = W[e] with the summed index as rows: read from LDS by transposing reads.
-//   GROUPED_BWD_W   A = x (gathered), B = dy, both with the summed index, the expert's rows, as rows. Any count of rows: those
+//   GROUPED_BWD_W   A = dy, B = x (gathered), both with the summed index, the expert's rows, as rows. Any count of rows: those
 //                   past the expert's last read as zero.
 //
 // Every copy is a buffer load into LDS of 64 x 16 bytes. A lane's row and chunk are its vector offset, the k-tile is the
@@ -37,6 +37,7 @@ namespace {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kBM = 256, kBN = 256, kKC = 8, kTile = 256 * kKC;  // kTile: 16-byte chunks of a buffer (32 KB)
+constexpr int kCUs = 256;         // of which each holds one workgroup
 constexpr int kPitch = 68;                                        // epilogue staging: 64 columns + 4 (floats)
 
 template <int... I, typename F>
@@ -96,6 +97,8 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     constexpr uint32_t ES = F8 ? 1u : 2u;
     constexpr bool AK = FORM == GROUPED_BWD_W;      // A is read with the summed index as rows
     constexpr bool BK = FORM != GROUPED_FWD;        // so is B
+    // tiles of at most 128 rows, or columns, take less than a whole one's time (e4m3 has no registers left for it)
+    constexpr bool PARTS = !F8 && FORM != GROUPED_BWD_W;
     __shared__ uint4 a0[kTile], a1[kTile], b0[kTile], b1[kTile], b2[kTile];
 
     const int lane = threadIdx.x & 63;
@@ -105,8 +108,9 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
 
     // ---- which tile: A's and B's first index, the group's rows, the k-tiles
     int e, aFirst, bFirst, begin, end, sumLen;
+    bool half = false;   // at most 128 of A's indices are the tile's
     if constexpr (FORM == GROUPED_BWD_W) {
-        const int tilesI = static_cast<int>((ga.I + kBN - 1) / kBN), perExpert = tilesI * tilesJ;
+        const int tilesI = static_cast<int>((ga.I + kBM - 1) / kBM), perExpert = tilesI * tilesJ;
         // all XCDs on one expert at a time: its tiles take as long as it has rows, so an expert of its own would leave the XCD
         // of the fullest one behind (8 experts of 700 to 4000 rows, 4096 x 4096: 768 us that way)
         e = static_cast<int>(blockIdx.x) / perExpert;
@@ -114,16 +118,33 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         grouped_tile(xcd_remap(static_cast<int>(blockIdx.x) - e * perExpert, perExpert), tilesI, tilesJ, order, ti, tj);
         begin = clamp_row(ga.offsets[e], R);
         end = clamp_row(ga.offsets[e + 1], R);
-        aFirst = tj * kBM;                          // columns of x, C's columns
-        bFirst = ti * kBN;                          // columns of dy, C's rows
+        aFirst = ti * kBM;                          // columns of dy, C's rows
+        bFirst = tj * kBN;                          // columns of x, C's columns
         sumLen = end > begin ? end - begin : 0;
     } else {
-        RowTiles tiles(ga.offsets, E, R, kBM);
-        const int actual = tiles.total() * tilesJ;
-        if (static_cast<int>(blockIdx.x) >= actual) return;
-        int ti, tj;
-        grouped_tile(xcd_remap(blockIdx.x, actual), tiles.total(), tilesJ, order, ti, tj);
-        const RowTile t = tiles.find(ti);
+        RowTiles<PARTS> tiles(ga.offsets, E, R, kBM);
+        // The halves come last, where they fill what the whole tiles' last round leaves free. If that round's tiles, cut in two,
+        // and the halves fit into one round together, they are cut: a round of halves takes 0.66 of the time.
+        const int whole = tiles.total() * tilesJ, halves = tiles.halves() * tilesJ, last = whole % kCUs;
+        const int cut = PARTS && 2 * last + halves <= kCUs ? last : 0, uncut = whole - cut;
+        int lid = static_cast<int>(blockIdx.x), ti, tj;
+        if (lid >= uncut + 2 * cut + halves) return;
+        half = PARTS && lid >= uncut;
+        RowTile t;
+        if (lid >= uncut + 2 * cut) {
+            grouped_tile(xcd_remap(lid - uncut - 2 * cut, halves), tiles.halves(), tilesJ, order, ti, tj);
+            t = tiles.find_half(ti);
+        } else {
+            const int part = lid < uncut ? 0 : lid >= uncut + cut;
+            lid -= part * cut;
+            const int place = lid < uncut ? xcd_remap(lid, uncut) : uncut + xcd_remap(lid - uncut, cut);
+            grouped_tile(place, tiles.total(), tilesJ, order, ti, tj);
+            t = tiles.find(ti);
+            if (half) {
+                t.r0 += part * 128;
+                t.end = t.end < t.r0 + 128 ? t.end : t.r0 + 128;
+            }
+        }
         e = t.e;
         begin = t.r0;
         end = t.end;
@@ -134,6 +155,13 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     constexpr int kPerTile = BK && AK ? 64 : static_cast<int>(128u / ES);       // summed indices of a k-tile
     const int nk = (sumLen + kPerTile - 1) / kPerTile;
     const int tailLen = sumLen - (nk - 1) * kPerTile;                            // summed indices of the last k-tile
+    // a wave's part of the tile: from A's index aWave on and B's bWave
+    const int aWave = (half ? p & 1 : p) * 64, bWave = g * 128 + (half ? (p >> 1) * 64 : 0);
+    // group 1 has nothing to multiply where the tile has at most 128 of B's indices
+    const int bLeft = static_cast<int>(ga.J) - bFirst;
+    const bool active = !PARTS || g == 0 || bLeft > 128;
+    // and the operand rows past 128 need no copies
+    const bool copies = !PARTS || (g == 0 ? !half || p < 2 : BK || bLeft > 128 || p < 2);
 
     // ---- this wave's stream: group 0 copies A, group 1 copies B; wave p copies pieces 8 p .. 8 p + 7 of a tile.
     // Contiguous along the sum: piece q holds rows 8 q .. 8 q + 7, 128 bytes each; lane -> row l / 8, LDS slot l % 8, source
@@ -150,15 +178,15 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         const uint8_t *base;
         uint64_t bytes;
         if constexpr (AK) {
-            // x [rows][K]: the expert's rows, or rows of all tokens when gathered
-            base = bx + (ga.rows == nullptr ? static_cast<uint64_t>(begin) * ldb : 0u);
-            bytes = ga.rows == nullptr ? static_cast<uint64_t>(sumLen) * ldb : static_cast<uint64_t>(ga.S) * ldb;
-            kStep = ga.rows == nullptr ? 64u * ldb : 0u;
+            // dy [rows][N], the expert's rows
+            base = ax + static_cast<uint64_t>(begin) * lda;
+            bytes = static_cast<uint64_t>(sumLen) * lda;
+            kStep = 64u * lda;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t q = static_cast<uint32_t>(p * 8 + j), row = 2u * q + (static_cast<uint32_t>(lane) >> 5);
                 const uint32_t col = static_cast<uint32_t>(aFirst) + (((static_cast<uint32_t>(lane) & 31u) ^ (4u * (row & 3u))) * 8u);
-                vo[j] = col < static_cast<uint32_t>(ga.J) ? (ga.rows == nullptr ? row * ldb : 0u) + col * ES : kOut;
+                vo[j] = col < static_cast<uint32_t>(ga.I) ? row * lda + col * ES : kOut;
             }
             tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
         } else {
@@ -187,14 +215,15 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         rs = resource(base, bytes);
     } else {
         if constexpr (AK) {
-            // dy [rows][N], the expert's rows
-            rs = resource(ax + static_cast<uint64_t>(begin) * lda, static_cast<uint64_t>(sumLen) * lda);
-            kStep = 64u * lda;
+            // x [rows][K]: the expert's rows, or rows of all tokens when gathered
+            const bool gather = ga.rows != nullptr;
+            rs = resource(bx + (gather ? 0u : static_cast<uint64_t>(begin) * ldb), static_cast<uint64_t>(gather ? ga.S : sumLen) * ldb);
+            kStep = gather ? 0u : 64u * ldb;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t q = static_cast<uint32_t>(p * 8 + j), row = 2u * q + (static_cast<uint32_t>(lane) >> 5);
                 const uint32_t col = static_cast<uint32_t>(bFirst) + (((static_cast<uint32_t>(lane) & 31u) ^ (4u * (row & 3u))) * 8u);
-                vo[j] = col < static_cast<uint32_t>(ga.I) ? row * lda + col * ES : kOut;
+                vo[j] = col < static_cast<uint32_t>(ga.J) ? (gather ? 0u : row * ldb) + col * ES : kOut;
             }
             tailAt[0] = tailAt[1] = 2 * p * 8 + (lane >> 5);
         } else if constexpr (BK) {
@@ -223,28 +252,32 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             tailAt[1] = ((lane & 7) ^ (4 + (lane >> 4))) * static_cast<int>(16u / ES);
         }
     }
-    // Gathered rows of x in the weight's gradient change with the k-tile: lane l < 16 holds the row number of row l of the
-    // wave's 16 in the k-tile to come, as loaded: nothing is computed from it before the next memory phase, so the load has a
-    // whole phase to arrive. Only group 0 loads them, which waits for all its copies in every phase anyway.
-    const bool gatherK = AK && ga.rows != nullptr;
-    int rowNo = -1;
-    auto load_rows = [&](int t) __attribute__((always_inline)) {
-        if (gatherK && g == 0) {
-            const int r = begin + t * 64 + p * 16 + (lane & 15);
-            rowNo = -1;
-            if (r < end) rowNo = ga.rows[r];
-        }
+    // Gathered rows of x in the weight's gradient change with the k-tile. Lane l holds the offset of row l % 16 of the wave's 16 in
+    // k-tile l / 16 of four; the numbers of the next four are loaded meanwhile.
+    const bool gatherK = AK && g == 1 && ga.rows != nullptr;
+    uint32_t rowOff = kOut;
+    int rowNext = -1;
+    auto load_rows = [&](int four) __attribute__((always_inline)) {
+        const int r = begin + (four * 4 + (lane >> 4)) * 64 + p * 16 + (lane & 15);
+        rowNext = -1;
+        if (r < end) rowNext = ga.rows[r];
+    };
+    auto next_rows = [&]() __attribute__((always_inline)) {
+        rowOff = static_cast<uint32_t>(rowNext) < static_cast<uint32_t>(ga.S) ? static_cast<uint32_t>(rowNext) * ldb : kOut;
     };
     auto stream = [&](int t, uint32_t lds) __attribute__((always_inline)) {
+        if (!copies) return;
         const uint32_t soff = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(t) * kStep);
         lds = __builtin_amdgcn_readfirstlane(lds + static_cast<uint32_t>(p * 8) * 1024u);
-        if (AK && gatherK && g == 0) {
-            const uint32_t rowOff = static_cast<uint32_t>(rowNo) < static_cast<uint32_t>(ga.S) ? static_cast<uint32_t>(rowNo) * ldb : kOut;
+        if (AK && gatherK) {
+            const int from = ((t & 3) * 16 + (lane >> 5)) * 4;
+            uint32_t at[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at[j] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from + 8 * j, static_cast<int>(rowOff)));
             sfor<8>([&](auto jc) __attribute__((always_inline)) {
                 constexpr int j = decltype(jc)::value;
-                const uint32_t r0 = __builtin_amdgcn_readlane(rowOff, 2 * j), r1 = __builtin_amdgcn_readlane(rowOff, 2 * j + 1);
-                const uint32_t r = lane < 32 ? r0 : r1;
-                copy_lds<false>(rs, r == kOut || vo[j] == kOut ? kOut : r + vo[j], soff, lds + static_cast<uint32_t>(j) * 1024u);
+                // the sum of offsets saturates: kOut stays kOut
+                copy_lds<false>(rs, __builtin_elementwise_add_sat(at[j], vo[j]), soff, lds + static_cast<uint32_t>(j) * 1024u);
             });
         } else if (t == nk - 1 && tailLen < kPerTile) {
             // past the end of the sum: rows (2 apart from piece to piece), or chunks (whole ones: the sum is a multiple of one)
@@ -268,7 +301,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     uint32_t sxAt = kOut;
     const_float *sw = nullptr;
     if constexpr (F8) {
-        const int r = aFirst + p * 64 + lane;
+        const int r = aFirst + aWave + lane;
         const int64_t s = r < end ? source_row(ga, r) : -1;
         sxAt = s >= 0 ? static_cast<uint32_t>(s) * static_cast<uint32_t>(KB) : kOut;
         const int64_t NB = (ga.J + 127) / 128;
@@ -296,7 +329,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
         return make_uint4(l2.x, l2.y, h2.x, h2.y);
     };
-    const int offA = (p * 64 + lrow) * kKC, offB = (g * 128 + lrow) * kKC;
+    const int offA = (aWave + lrow) * kKC, offB = (bWave + lrow) * kKC;
     // e4m3: 16 rows, lane group l / 16 has chunks 2 (l / 16) and + 1
     const int row16 = lane & 15, c16 = (lane >> 4) * 2, sw16 = (row16 >> 1) & 7;
     auto read16 = [&](const uint4 *buf, int row0) __attribute__((always_inline)) -> i32x8_t {
@@ -323,18 +356,23 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         }
     }
 
-    auto step = [&](auto ic, int t) __attribute__((always_inline)) {
+    // HALF: of A's 128 indices and B's 256, a wave has 64 and 64, and A is triple-buffered as well: its tiles take half the room,
+    // and half the products do not cover a copy's latency
+    auto step = [&](auto ic, int t, auto halfc) __attribute__((always_inline)) {
         constexpr int I = decltype(ic)::value;
-        const uint4 *at = I % 2 == 0 ? a0 : a1;
+        constexpr bool HALF = decltype(halfc)::value;
+        constexpr int NB = HALF ? 2 : 4, NB8 = 2 * NB;      // strips of B
+        const uint4 *at = HALF ? (I % 3 == 0 ? a0 : (I % 3 == 1 ? a0 + kTile / 2 : a1)) : (I % 2 == 0 ? a0 : a1);
         const uint4 *bt = I % 3 == 0 ? b0 : (I % 3 == 1 ? b1 : b2);
-        const uint32_t la = lds_addr(I % 2 == 0 ? a1 : a0), lb = lds_addr(I % 3 == 0 ? b2 : (I % 3 == 1 ? b0 : b1));
+        const uint32_t la = lds_addr(HALF ? (I % 3 == 0 ? a1 : (I % 3 == 1 ? a0 : a0 + kTile / 2)) : (I % 2 == 0 ? a1 : a0));
+        const uint32_t lb = lds_addr(I % 3 == 0 ? b2 : (I % 3 == 1 ? b0 : b1));
         // ---- memory phase
         uint4 fa[4][2], fb[2][4];
         i32x8_t fa8[4], fb8[2];
         float s8[4];
         if constexpr (F8) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa8[i] = read16(at, p * 64 + i * 16);
+            for (int i = 0; i < 4; ++i) fa8[i] = read16(at, aWave + i * 16);
             const float swt = sw[t];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -353,7 +391,10 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 }
             }
         }
-        const int tt = t + 1 + g;  // group 0 copies A(t + 1), group 1 copies B(t + 2)
+        const int tt = HALF ? t + 2 : t + 1 + g;  // group 0 copies A(t + 1), or A(t + 2) of a half, group 1 copies B(t + 2)
+        if (AK && gatherK && (tt & 3) == 0) {
+            next_rows();
+        }
         if (tt < nk) {
             stream(tt, g == 0 ? la : lb);
         }
@@ -369,20 +410,22 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         if constexpr (F8) {
             sx[I % 3] = load_sx(t + 3);
         }
-        load_rows(t + 2);
+        if (AK && gatherK && (tt & 3) == 0) {
+            load_rows((tt >> 2) + 1);
+        }
         auto read_b = [&](auto slotc, auto stepc) __attribute__((always_inline)) {
             constexpr int slot = decltype(slotc)::value, s = decltype(stepc)::value;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < NB; ++j) {
                 if constexpr (BK) {
-                    fb[slot][j] = read_tr(bt, static_cast<uint32_t>(g * 4 + j), s);
+                    fb[slot][j] = read_tr(bt, static_cast<uint32_t>(bWave / 32 + j), s);
                 } else {
                     fb[slot][j] = bt[offB + j * 32 * kKC + ((2 * s + lh) ^ fsw)];
                 }
             }
         };
         if constexpr (F8) {
-            fb8[0] = read16(bt, g * 128);
+            fb8[0] = read16(bt, bWave);
         } else {
             read_b(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
         }
@@ -392,13 +435,14 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         __builtin_amdgcn_sched_barrier(0);
         // ---- compute phase, at raised wave priority
         __builtin_amdgcn_s_setprio(1);
-        if constexpr (F8) {
+        if (!active) {
+        } else if constexpr (F8) {
             // product m = 4 j + i of strips j of B and i of A; the sums of product m - 2 run under it
             f32x4_t part[4];
-            sfor<8>([&](auto jc) __attribute__((always_inline)) {
+            sfor<NB8>([&](auto jc) __attribute__((always_inline)) {
                 constexpr int j = decltype(jc)::value;
-                if constexpr (j + 1 < 8) {
-                    fb8[(j + 1) & 1] = read16(bt, g * 128 + (j + 1) * 16);
+                if constexpr (j + 1 < NB8) {
+                    fb8[(j + 1) & 1] = read16(bt, bWave + (j + 1) * 16);
                 }
                 asm volatile("" ::: "memory");   // keeps the later strips' reads, and their registers, behind this one's
                 __builtin_amdgcn_sched_barrier(0);
@@ -418,8 +462,8 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
 #pragma unroll
             for (int i = 2; i < 4; ++i) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc8[7][i][r] = fmaf(s8[i], part[i][r], acc8[7][i][r]);
-                asm volatile("" : "+v"(acc8[7][i]));
+                for (int r = 0; r < 4; ++r) acc8[NB8 - 1][i][r] = fmaf(s8[i], part[i][r], acc8[NB8 - 1][i][r]);
+                asm volatile("" : "+v"(acc8[NB8 - 1][i]));
             }
         } else {
             sfor<4>([&](auto sc) __attribute__((always_inline)) {
@@ -429,11 +473,11 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < NB; ++j) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         // the first operand's index runs over a lane's registers: the one that is contiguous in C
-                        const uint4 first = AK ? fa[s][i] : fb[s & 1][j], second = AK ? fb[s & 1][j] : fa[s][i];
+                        const uint4 first = fb[s & 1][j], second = fa[s][i];
                         if constexpr (CT == KUDNN_DT_BF16) {
                             acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, first),
                                                                                 __builtin_bit_cast(bf16x8_t, second), acc[j][i], 0, 0, 0);
@@ -447,8 +491,12 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             });
         }
         __builtin_amdgcn_s_setprio(0);
-        if (g == 0) {
-            wait_vmcnt<0>();   // A(t + 1), which this group reads in the next phase
+        if (g == 0) {          // A(t + 1), which this group reads in the next phase
+            if (HALF && t + 2 < nk) {
+                wait_vmcnt<8>();
+            } else {
+                wait_vmcnt<0>();
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
@@ -459,11 +507,14 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         if constexpr (F8) {
             sfor<3>([&](auto ic) __attribute__((always_inline)) { sx[decltype(ic)::value] = load_sx(decltype(ic)::value); });
         }
-        load_rows(0);
+        if (AK && gatherK) {
+            load_rows(0);
+            next_rows();
+            load_rows(1);
+        }
         stream(0, g == 0 ? lds_addr(a0) : lds_addr(b0));
-        load_rows(1);
-        if (g == 1 && nk > 1) {
-            stream(1, lds_addr(b1));
+        if ((g == 1 || (PARTS && half)) && nk > 1) {
+            stream(1, g == 0 ? lds_addr(a0 + kTile / 2) : lds_addr(b1));
             wait_vmcnt<8>();
         } else {
             wait_vmcnt<0>();
@@ -472,10 +523,21 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         if (g == 1) {
             __builtin_amdgcn_s_barrier();  // group 1 runs one phase behind
         }
-        for (int t = 0; t < nk; t += 6) {
-            sfor<6>([&](auto ic) __attribute__((always_inline)) {
-                if (t + decltype(ic)::value < nk) step(ic, t + decltype(ic)::value);
-            });
+        auto run = [&](auto halfc) __attribute__((always_inline)) {
+            for (int t = 0; t < nk; t += 6) {
+                sfor<6>([&](auto ic) __attribute__((always_inline)) {
+                    if (t + decltype(ic)::value < nk) step(ic, t + decltype(ic)::value, halfc);
+                });
+            }
+        };
+        if constexpr (PARTS) {
+            if (half) {
+                run(std::true_type{});
+            } else {
+                run(std::false_type{});
+            }
+        } else {
+            run(std::false_type{});
         }
         if (g == 0) {
             __builtin_amdgcn_s_barrier();  // matches group 1's extra barrier at the start
@@ -486,15 +548,15 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
     // back 8 columns a lane: stores of whole 128-byte lines
     __syncthreads();   // every wave is done with the tile buffers
     float *stage = reinterpret_cast<float *>(wave < 3 ? a0 : (wave < 6 ? a1 : b0)) + (wave % 3) * (32 * kPitch);
-    const int64_t rowW = FORM == GROUPED_BWD_W ? bFirst + g * 128 : aFirst + p * 64;
-    const int64_t colW = FORM == GROUPED_BWD_W ? aFirst + p * 64 : bFirst + g * 128;
+    const int64_t rowW = aFirst + aWave, colW = bFirst + bWave;
     const int64_t rowEnd = FORM == GROUPED_BWD_W ? ga.I : end;
     const int64_t cBase = FORM == GROUPED_BWD_W ? e * ga.ce : 0;
     const bool wide = ga.ldc % 8 == 0 && ga.ce % 8 == 0 && reinterpret_cast<uintptr_t>(ga.c) % 16 == 0;
     const int col8 = (lane & 7) * 8, rl = lane >> 3;
     sfor<4>([&](auto uc) __attribute__((always_inline)) {
         constexpr int u = decltype(uc)::value;
-        constexpr int rowU = FORM == GROUPED_BWD_W ? u * 32 : (u % 2) * 32, colU = FORM == GROUPED_BWD_W ? 0 : (u / 2) * 64;
+        if (PARTS && u >= 2 && half) return;
+        constexpr int rowU = (u % 2) * 32, colU = (u / 2) * 64;
         if constexpr (F8) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -507,7 +569,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         } else {
 #pragma unroll
             for (int sh = 0; sh < 2; ++sh) {
-                const f32x16_t &v = FORM == GROUPED_BWD_W ? acc[u][sh] : acc[2 * (u / 2) + sh][u % 2];
+                const f32x16_t &v = acc[2 * (u / 2) + sh][u % 2];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     *reinterpret_cast<float4 *>(stage + lrow * kPitch + sh * 32 + q * 8 + lh * 4) =
@@ -547,7 +609,9 @@ void launch(const GroupedArgs &g, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + 255) / 256;
     const int64_t tiles = FORM == GROUPED_BWD_W ? g.E * ((g.I + 255) / 256) : max_row_tiles(g.R, g.E, 256, g.offsets != nullptr);
-    grouped_pingpong_kernel<CT, FORM><<<static_cast<unsigned>(tiles * tilesJ), 512, 0, stream>>>(g, static_cast<int>(tilesJ), 4);
+    // up to a round of tiles may be cut in two
+    const int64_t grid = tiles * tilesJ + (CT != KUDNN_DT_F8E4M3 && FORM != GROUPED_BWD_W ? (tiles * tilesJ < kCUs / 2 ? tiles * tilesJ : kCUs / 2) : 0);
+    grouped_pingpong_kernel<CT, FORM><<<static_cast<unsigned>(grid), 512, 0, stream>>>(g, static_cast<int>(tilesJ), 4);
 }
 
 template <int CT>

@@ -14,11 +14,12 @@ using namespace kudnn_dev;
 
 namespace {
 
-// s_waitcnt vmcnt(N) that no LDS access moves across.
+// Waits until at most N of this wave's copies are on their way and its LDS reads are done (a block's products may sink below
+// the barrier, and their reads' wait with them; the stage is overwritten after it). No LDS access moves across.
 template <int N>
 __device__ __forceinline__ void wait_copies()
 {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
 }
 
 // One word a lane to LDS: lane l's 4 bytes land at lds + 4 l.
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
     const int wm = wave / WN, wn = wave % WN, row16 = lane & 15, grp = lane >> 4;
 
     const int E = static_cast<int>(g.E);
-    RowTiles tiles(g.offsets, E, static_cast<int>(g.R), BM);
+    RowTiles<> tiles(g.offsets, E, static_cast<int>(g.R), BM);
     const int actual = tiles.total() * tilesJ;
     if (static_cast<int>(blockIdx.x) >= actual) return;
     const int lid = xcd_remap(blockIdx.x, actual);

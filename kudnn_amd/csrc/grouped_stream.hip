@@ -48,7 +48,7 @@ __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedArgs g, i
     const int row16 = lane & 15, grp = lane >> 4;
 
     const int E = static_cast<int>(g.E);
-    RowTiles tiles(g.offsets, E, static_cast<int>(g.R), BM);
+    RowTiles<> tiles(g.offsets, E, static_cast<int>(g.R), BM);
     const int actual = tiles.total() * tilesJ;
     if (static_cast<int>(blockIdx.x) >= actual) return;
     // the row tiles of one block of columns are neighbours: those of one expert read the same weights
