@@ -79,6 +79,16 @@ def _at(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _first_order(backward):
+    """A backward that is not differentiable itself: as torch's own wrapper, which is only taken where a graph is being made."""
+    again = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, grad):
+        return again(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+
+    return run
+
+
 def _workspace(plan, device: torch.device) -> Optional[torch.Tensor]:
     n = plan.workspace_bytes
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
@@ -145,6 +155,19 @@ def _route(logits, mask, top_k, normalize):
     return weights, chosen, offsets, rows, slots
 
 
+def _route_backward(logits, mask, top_k, normalize, weights, experts, dweights):
+    device = logits.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _route_backward(logits, mask, top_k, normalize, weights, experts, dweights)
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    rc = lib().kudnn_moe_route_backward(_route_plan(logits, mask, top_k, normalize).handle, logits.data_ptr(), _at(mask),
+                                        weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), _stream(device.index))
+    if rc:
+        check(rc)
+    return dlogits
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, mask, top_k, normalize, rest):
@@ -155,17 +178,10 @@ class _Route(torch.autograd.Function):
         return weights
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dweights):
         logits, mask, weights, experts = ctx.saved_tensors
-        plan = _route_plan(logits, mask, ctx.top_k, ctx.normalize)
-        dweights = dweights.contiguous()
-        device = logits.device
-        with torch.cuda.device(device):
-            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-            check(lib().kudnn_moe_route_backward(plan.handle, logits.data_ptr(), _at(mask), weights.data_ptr(), experts.data_ptr(),
-                                                 dweights.data_ptr(), dlogits.data_ptr(), _stream(device.index)))
-        return dlogits, None, None, None, None
+        return _route_backward(logits, mask, ctx.top_k, ctx.normalize, weights, experts, dweights.contiguous()), None, None, None, None
 
 
 def route(logits: torch.Tensor, top_k: int, normalize: bool = True, mask: Optional[torch.Tensor] = None) -> Routing:
@@ -216,6 +232,25 @@ def _grouped(x, w, offsets, rows):
     return y
 
 
+def _grouped_backward(x, w, offsets, rows, slots, dy, wants_dx, wants_dw):
+    device = x.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _grouped_backward(x, w, offsets, rows, slots, dy, wants_dx, wants_dw)
+    plan = _grouped_plan(x, w, dy.shape[0], rows is not None)
+    stream, ws = _stream(device.index), _workspace(plan, device)
+    dx = dw = None
+    if wants_dx:
+        dx = torch.empty((dy.shape[0], x.shape[1]), dtype=x.dtype, device=device)
+        plan.backward_input(dy, w, offsets, dx, stream, ws)
+        if rows is not None:
+            dx = _combine(dx, None, slots)
+    if wants_dw:
+        dw = torch.empty(w.shape, dtype=w.dtype, device=device)
+        plan.backward_weight(dy, x, offsets, rows, dw, stream, ws)
+    return dx, dw
+
+
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, rows, slots):
@@ -223,25 +258,9 @@ class _GroupedLinear(torch.autograd.Function):
         return _grouped(x, w, offsets, rows)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dy):
-        x, w, offsets, rows, slots = ctx.saved_tensors
-        dy = dy.contiguous()
-        device = x.device
-        plan = _grouped_plan(x, w, dy.shape[0], rows is not None)
-        dx = dw = None
-        with torch.cuda.device(device):
-            stream = _stream(device.index)
-            ws = _workspace(plan, device)
-            if ctx.needs_input_grad[0]:
-                dx = torch.empty((dy.shape[0], x.shape[1]), dtype=x.dtype, device=device)
-                plan.backward_input(dy, w, offsets, dx, stream, ws)
-                if rows is not None:
-                    dx = _combine(dx, None, slots)
-            if ctx.needs_input_grad[1]:
-                dw = torch.empty(w.shape, dtype=w.dtype, device=device)
-                plan.backward_weight(dy, x, offsets, rows, dw, stream, ws)
-        return dx, dw, None, None, None
+        return *_grouped_backward(*ctx.saved_tensors, dy.contiguous(), *ctx.needs_input_grad[:2]), None, None, None
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
@@ -395,6 +414,20 @@ def _combine(y, weights, slots):
     return out
 
 
+def _combine_backward(y, weights, slots, dout, wants_dy, wants_dw):
+    device = y.device
+    if _current() != device.index:
+        with torch.cuda.device(device):
+            return _combine_backward(y, weights, slots, dout, wants_dy, wants_dw)
+    dy = torch.empty(y.shape, dtype=y.dtype, device=device) if wants_dy else None
+    dw = torch.empty(slots.shape, dtype=torch.float32, device=device) if wants_dw else None
+    rc = lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
+                                          dout.data_ptr(), _at(dy), _at(dw), _stream(device.index))
+    if rc:
+        check(rc)
+    return dy, dw
+
+
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, slots):
@@ -402,17 +435,9 @@ class _Combine(torch.autograd.Function):
         return _combine(y, weights, slots)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dout):
-        y, weights, slots = ctx.saved_tensors
-        device = y.device
-        dout = dout.contiguous()
-        with torch.cuda.device(device):
-            dy = torch.empty(y.shape, dtype=y.dtype, device=device) if ctx.needs_input_grad[0] else None
-            dw = torch.empty(slots.shape, dtype=torch.float32, device=device) if ctx.needs_input_grad[1] else None
-            check(lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
-                                                   dout.data_ptr(), _at(dy), _at(dw), _stream(device.index)))
-        return dy, dw, None
+        return *_combine_backward(*ctx.saved_tensors, dout.contiguous(), *ctx.needs_input_grad[:2]), None
 
 
 def combine(y: torch.Tensor, weights: Optional[torch.Tensor], slots: torch.Tensor) -> torch.Tensor:

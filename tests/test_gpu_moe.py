@@ -694,3 +694,19 @@ def test_streams_and_graphs():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+
+
+def test_gradients_of_gradients_are_refused():
+    """A graph of the backward pass may be made, but nothing is differentiated through it silently."""
+    offsets, rows = make_order([3, 5], 0, 4, gen(5))
+    x = torch.randn(4, 64, device=DEV).bfloat16().requires_grad_(True)
+    w = torch.randn(2, 32, 64, device=DEV).bfloat16().requires_grad_(True)
+    y = torch.randn(8, 48, device=DEV).requires_grad_(True)
+    weights = torch.rand(4, 2, device=DEV).requires_grad_(True)
+    slots = torch.arange(8, dtype=torch.int32, device=DEV).reshape(4, 2)
+    logits = torch.randn(4, 8, device=DEV).requires_grad_(True)
+    for out, of in ((km.grouped_linear(x, w, offsets, rows, slots), w), (km.combine(y, weights, slots), weights),
+                    (km.route(logits, 2).weights, logits)):
+        (first,) = torch.autograd.grad(out.float().square().sum(), of, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad(first.float().sum(), of)
