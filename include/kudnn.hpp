@@ -20,5 +20,6 @@
 #include "operations/kudnn_linear_activationlayer.hpp"
 #include "operations/kudnn_linear_postops.hpp"
 #include "operations/kudnn_linear_res.hpp"
+#include "operations/kudnn_moe.hpp"
 
 #endif  // KUDNN_HPP

@@ -18,7 +18,8 @@ using IntType = std::int64_t;
 
 namespace Element {
 
-enum class TypeT { UNDEFINED = 0, F32, F16, BF16, S32, S8, U8 };
+// F8E4M3 is an addition after KuDNN's values, for the 8-bit Linear operators only.
+enum class TypeT { UNDEFINED = 0, F32, F16, BF16, S32, S8, U8, F8E4M3 };
 
 // Run-time description of an element type: its enumerator plus its storage size in bytes.
 struct Type final {
@@ -33,7 +34,7 @@ public:
     SizeType GetSize() const noexcept { return size; }
     SizeType GetBitwidth() const noexcept { return size * 8u; }
     operator TypeT() const noexcept { return type; }
-    bool IsFP() const noexcept { return type == TypeT::F32 || type == TypeT::F16 || type == TypeT::BF16; }
+    bool IsFP() const noexcept { return type == TypeT::F32 || type == TypeT::F16 || type == TypeT::BF16 || type == TypeT::F8E4M3; }
     bool IsIntegral() const noexcept { return !IsFP(); }
     bool IsSigned() const noexcept { return type != TypeT::U8; }
     bool IsUnsigned() const noexcept { return !IsSigned(); }
@@ -44,7 +45,7 @@ private:
         switch (t) {
             case TypeT::F32: case TypeT::S32: return 4;
             case TypeT::F16: case TypeT::BF16: return 2;
-            case TypeT::S8: case TypeT::U8: return 1;
+            case TypeT::S8: case TypeT::U8: case TypeT::F8E4M3: return 1;
             default: return 0;
         }
     }

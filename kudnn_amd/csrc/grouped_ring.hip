@@ -6,8 +6,13 @@
 // (wm, wn) has 1 / WM of the rows and 1 / WN of the columns. Per block: wait for this wave's own copies of it, one barrier (now
 // everyone's have landed, and everyone is done with the block before), send the copies of the block S - 1 ahead into the
 // stage that the barrier freed, read the fragments, multiply.
-// Fragments, swizzle, e4m3 (exact, by bf16 MFMAs) and what lies outside the operands: as in grouped_stream.hip. The row scales
+// Fragments, swizzle, exact e4m3 (by bf16 MFMAs) and what lies outside the operands: as in grouped_stream.hip. The row scales
 // come with a block's copies, a word a row, so that no load of the compiler's own waits for the ring.
+//
+// Two blocks leave room for three workgroups of 64-row tiles a CU or two of 128, whose starts and ends hide under one another's
+// blocks; four blocks (one workgroup a CU) pay where there are fewer tiles than that. Measured: 64 experts of 64 rows on
+// average, 2048 x 4096 e4m3 (537 MB): 152 us on 128 x 128 tiles of two blocks, 171 of four; a block takes 1.5 us, HBM's
+// latency under this load.
 #include "grouped_common.h"
 
 using namespace kudnn_dev;

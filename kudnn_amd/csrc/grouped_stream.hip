@@ -1,5 +1,4 @@
-// Grouped products of few rows: the experts' Linear layers of one token or a decode batch, e4m3 products of any size that does
-// not fill the chip with 256 x 256 tiles, and every e4m3 product into f32.
+// Grouped products of few rows: the experts' Linear layers of one token or a decode batch, in 16 bits or e4m3.
 //
 // A workgroup has a tile of BM rows of one expert and BN columns; its waves split the sum: wave w of W takes the blocks
 // w, w + W, ... of 128 bytes of each row and accumulates the whole tile over them. A wave copies a block's rows into LDS of
@@ -10,7 +9,7 @@
 // What bounds it is the weight's way from HBM. A copy covers 8 rows of whole 128-byte lines: reading 16 rows of 64 bytes, the
 // layout the MFMAs want, straight into registers streamed 90 MB at 4.4 TB/s where this pattern gave 5.2, and 5.7 with
 // the non-temporal hint (1 GB: 6.2, 6.1 and 7.0; a plain read of whole rows 7.1). The hint is for weights that one row tile
-// reads.
+// reads. Measured: 8 experts of one row each, 2048 x 4096 bf16 (134 MB): 21.4 us a call back to back (6.3 TB/s).
 //
 // v_mfma_f32_16x16x32: lane l has row l % 16 of an operand and 8 of its 32 summed indices. A block's row is 8 chunks of 16
 // bytes; lane group l / 16 takes chunks g and g + 4. Which index of the sum a lane has does not matter as long as both operands

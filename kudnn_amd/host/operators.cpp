@@ -6,31 +6,16 @@
 // KuDNN throws (Service::ThrowOnStatus, src/dnn/src/service.cpp:32-46):
 //   UNSUPPORTED -> Service::Unsupported, BAD_ARGUMENTS / null pointers -> Service::LogicError,
 //   allocation failure -> Service::BadAlloc, HIP runtime errors -> std::runtime_error.
-#include <cstring>
-#include <string>
-
 #include "../../include/kudnn.hpp"
 #include "../../include/kudnn_hip.h"
+#include "abi.h"
 
 namespace KuDNN {
 
 namespace {
 
-kudnn_tensor_desc ToDesc(const TensorInfo &t)
-{
-    kudnn_tensor_desc d;
-    std::memset(&d, 0, sizeof(d));
-    const Shape dims = t.GetDims();
-    const Shape strides = t.GetStrides();
-    d.ndims = static_cast<int32_t>(dims.GetNumDims());
-    d.dtype = static_cast<int32_t>(static_cast<Element::TypeT>(t.GetType()));
-    d.layout = static_cast<int32_t>(t.GetLayout());
-    for (SizeType i = 0; i < dims.GetNumDims(); ++i) {
-        d.dims[i] = static_cast<int64_t>(dims[i]);
-        d.strides[i] = i < strides.GetNumDims() ? static_cast<int64_t>(strides[i]) : 0;
-    }
-    return d;
-}
+using Abi::Check;
+using Abi::ToDesc;
 
 // KuDNN's "no bias" descriptor: a 1-D tensor of size 0 (kudnn_gemm.cpp:895-898).
 TensorInfo NoTensor(const TensorInfo &like) { return TensorInfo(Shape{0}, like.GetType(), Layout::A); }
@@ -41,18 +26,6 @@ Status ToStatus(int s) noexcept
         case KUDNN_STATUS_SUCCESS: return Status::SUCCESS;
         case KUDNN_STATUS_UNSUPPORTED: return Status::UNSUPPORTED;
         default: return Status::BAD_ARGUMENTS;
-    }
-}
-
-void Check(int s)
-{
-    switch (s) {
-        case KUDNN_STATUS_SUCCESS: return;
-        case KUDNN_STATUS_UNSUPPORTED: throw Service::Unsupported{kudnn_last_error()};
-        case KUDNN_STATUS_BAD_ARGUMENTS:
-        case KUDNN_STATUS_NULL_POINTER: throw Service::LogicError{kudnn_last_error()};
-        case KUDNN_STATUS_ALLOC_FAILED: throw Service::BadAlloc{};
-        default: throw std::runtime_error{kudnn_last_error()};
     }
 }
 

@@ -709,4 +709,4 @@ def test_gradients_of_gradients_are_refused():
                     (km.route(logits, 2).weights, logits)):
         (first,) = torch.autograd.grad(out.float().square().sum(), of, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
-            torch.autograd.grad(first.float().sum(), of)
+            first.float().sum().backward()
