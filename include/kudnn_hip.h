@@ -291,10 +291,12 @@ KUDNN_HIP_API int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const vo
                                            const int32_t *offsets, const int32_t *rows, void *y, void *stream);
 /* Workspace of the two gradients: 0 where N, K and the row pitches are multiples of 8, else room for rows packed to such. */
 KUDNN_HIP_API int64_t kudnn_grouped_linear_workspace_bytes(kudnn_grouped_linear_t plan);
-/* dx[r] = dy[r] x w[e]^T, {R, K} dense in the experts' order (with gather, a token's gradient is the sum over its slots:
- * kudnn_moe_combine_run with NULL weights). */
+/* dx[r] = dy[r] x w[e]^T, {R, K} dense in the experts' order, of dx_dt: the operands' type (or KUDNN_DT_UNDEFINED for it), or f32.
+ * With gather, a token's gradient is the sum over its slots: kudnn_moe_combine_run with NULL weights, of f32 rows where the
+ * sum is to be rounded once. */
 KUDNN_HIP_API int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void *dy, const void *w,
-                                                      const int32_t *offsets, void *dx, void *workspace, void *stream);
+                                                      const int32_t *offsets, void *dx, int dx_dt, void *workspace,
+                                                      void *stream);
 /* dw[e] = sum over the rows r of expert e of dy[r] x[r]^T, dense [E][N][K]; zero for an expert without rows. */
 KUDNN_HIP_API int kudnn_grouped_linear_backward_weight(kudnn_grouped_linear_t plan, const void *dy, const void *x,
                                                        const int32_t *offsets, const int32_t *rows, void *dw,
@@ -329,7 +331,8 @@ KUDNN_HIP_API int kudnn_linear_fp8_run(kudnn_linear_fp8_t plan, const void *x, c
 KUDNN_HIP_API int kudnn_linear_fp8_destroy(kudnn_linear_fp8_t plan);
 
 /* Weighted sum: out[t] = sum over j of weights[t][j] y[slots[t][j]], in f32, rounded once; j without a slot adds nothing.
- * y {R, N} AB, out {T, N} AB, one type of f32 / bf16 / f16; weights f32[T][k], or NULL for ones. top_k <= 64. */
+ * y {R, N} AB, out {T, N} AB, one type of f32 / bf16 / f16, or y of f32 and out of 16 bits (no gradients then); weights f32[T][k], or
+ * NULL for ones. top_k <= 64. */
 KUDNN_HIP_API int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kudnn_tensor_desc *out, int top_k,
                                            kudnn_moe_combine_t *plan);
 KUDNN_HIP_API int kudnn_moe_combine_run(kudnn_moe_combine_t plan, const void *y, const float *weights,

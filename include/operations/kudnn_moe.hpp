@@ -62,9 +62,10 @@ public:
     std::int64_t WorkspaceBytes() const noexcept(false);
     void Run(const void *x, const void *w, const std::int32_t *offsets, const std::int32_t *rows, void *y,
              void *stream = nullptr) const noexcept(false);
-    // dx {R, K} dense, in the experts' order; with gather, MoeCombine without weights adds a token's rows.
-    void BackwardInput(const void *dy, const void *w, const std::int32_t *offsets, void *dx, void *workspace,
-                       void *stream = nullptr) const noexcept(false);
+    // dx {R, K} dense, in the experts' order, of the operands' type (UNDEFINED) or F32; with gather, MoeCombine without weights adds a
+    // token's rows.
+    void BackwardInput(const void *dy, const void *w, const std::int32_t *offsets, void *dx, void *workspace, void *stream = nullptr,
+                       Element::TypeT dxType = Element::TypeT::UNDEFINED) const noexcept(false);
     // dw dense [E][N][K].
     void BackwardWeight(const void *dy, const void *x, const std::int32_t *offsets, const std::int32_t *rows, void *dw, void *workspace,
                         void *stream = nullptr) const noexcept(false);
@@ -100,7 +101,7 @@ private:
 // out[t] = sum over j of weights[t][j] y[slots[t][j]] (weights nullptr: ones).
 class KUDNN_API_PUBLIC MoeCombine final {
 public:
-    // y {R, N} AB and out {T, N} AB of one type: F32, BF16 or F16.
+    // y {R, N} AB and out {T, N} AB of one type: F32, BF16 or F16; or y of F32 and out of 16 bits (Run only).
     MoeCombine(const TensorInfo &y, const TensorInfo &out, int topK) noexcept(false);
     MoeCombine(const MoeCombine &other) = delete;
     MoeCombine(MoeCombine &&other) noexcept;

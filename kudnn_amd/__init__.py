@@ -139,7 +139,7 @@ _SIGS = {
     "kudnn_grouped_linear_create": ([_D, _D, _D, ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
     "kudnn_grouped_linear_workspace_bytes": ([_P], ctypes.c_int64),
     "kudnn_grouped_linear_run": ([_P] * 7, ctypes.c_int),
-    "kudnn_grouped_linear_backward_input": ([_P] * 7, ctypes.c_int),
+    "kudnn_grouped_linear_backward_input": ([_P] * 5 + [ctypes.c_int] + [_P] * 2, ctypes.c_int),
     "kudnn_grouped_linear_backward_weight": ([_P] * 8, ctypes.c_int),
     "kudnn_grouped_linear_destroy": ([_P], ctypes.c_int),
     "kudnn_quantize_rows": ([_D, _P, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
@@ -350,8 +350,9 @@ class GroupedLinear(_Plan):
         check(lib().kudnn_grouped_linear_run(self.handle, _ptr(x), _ptr(w), _ptr(offsets), _ptr(rows), _ptr(y),
                                              _stream(stream)))
 
-    def backward_input(self, dy, w, offsets, dx, stream=None, workspace=None):
-        check(lib().kudnn_grouped_linear_backward_input(self.handle, _ptr(dy), _ptr(w), _ptr(offsets), _ptr(dx),
+    def backward_input(self, dy, w, offsets, dx, stream=None, workspace=None, dx_dtype=DT_UNDEFINED):
+        """dx: of the operands' type (DT_UNDEFINED) or F32."""
+        check(lib().kudnn_grouped_linear_backward_input(self.handle, _ptr(dy), _ptr(w), _ptr(offsets), _ptr(dx), dx_dtype,
                                                         _ptr(workspace), _stream(stream)))
 
     def backward_weight(self, dy, x, offsets, rows, dw, stream=None, workspace=None):

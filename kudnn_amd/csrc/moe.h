@@ -46,7 +46,7 @@ struct CombineArgs {
     void *out, *dy;
     float *dweights;
     int64_t T, R, N, ldy, ldo;    // ldo: row pitch of out (dout and dy are dense)
-    int k, dt;
+    int k, dt, out_dt;            // out_dt: dt, or 16 bits of f32 rows (forward)
 };
 int kudnn_launch_moe_combine(const CombineArgs &a, hipStream_t stream);
 int kudnn_launch_moe_combine_backward(const CombineArgs &a, hipStream_t stream);

@@ -41,7 +41,7 @@ struct kudnn_linear_fp8_plan : PlanBase {
 struct kudnn_moe_combine_plan : PlanBase {
     kudnn_moe_combine_plan() : PlanBase(PLAN_MOE_COMBINE) {}
     int64_t T = 0, R = 0, N = 0, ldy = 0, ldo = 0;
-    int k = 0, dt = 0;
+    int k = 0, dt = 0, outDt = 0;
 };
 
 namespace {
@@ -420,10 +420,16 @@ int kudnn_grouped_linear_run(kudnn_grouped_linear_t plan, const void *x, const v
 }
 
 int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void *dy, const void *w, const int32_t *offsets,
-                                        void *dx, void *workspace, void *stream)
+                                        void *dx, int dx_dt, void *workspace, void *stream)
 {
     if (plan == nullptr) {
         return Null("grouped Linear: null plan");
+    }
+    if (dx_dt == KUDNN_DT_UNDEFINED) {
+        dx_dt = plan->dt;
+    }
+    if (dx_dt != plan->dt && dx_dt != KUDNN_DT_F32) {
+        return Unsupported("grouped Linear: dx must be of the operands' type or f32");
     }
     if (plan->R == 0) {
         return KUDNN_STATUS_SUCCESS;
@@ -431,7 +437,7 @@ int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void 
     if (dy == nullptr || w == nullptr || offsets == nullptr || dx == nullptr || (plan->workspace > 0 && workspace == nullptr)) {
         return Null("grouped Linear: one of the buffers is nullptr");
     }
-    const int s = CheckBuffers({Buffer{dy, plan->dt}, Buffer{w, plan->dt}, Buffer{offsets, KUDNN_DT_S32}, Buffer{dx, plan->dt},
+    const int s = CheckBuffers({Buffer{dy, plan->dt}, Buffer{w, plan->dt}, Buffer{offsets, KUDNN_DT_S32}, Buffer{dx, dx_dt},
                                 Buffer{workspace, KUDNN_DT_S32}});
     if (s != KUDNN_STATUS_SUCCESS) {
         return s;
@@ -454,7 +460,8 @@ int kudnn_grouped_linear_backward_input(kudnn_grouped_linear_t plan, const void 
     g.ldc = plan->K;
     g.be = plan->we;
     g.form = GROUPED_BWD_IN;
-    g.dt = g.c_dt = plan->dt;
+    g.dt = plan->dt;
+    g.c_dt = dx_dt;
     char *ws = static_cast<char *>(workspace);
     int rc = 0;
     if (plan->packDy > 0) {
@@ -772,8 +779,8 @@ int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kudnn_tensor_desc
         if (ldy < 0 || ldo < 0) {
             return Bad("weighted sum: y and out must be matrices with contiguous rows");
         }
-        if (!IsFloat(y->dtype) || out->dtype != y->dtype) {
-            return Unsupported("weighted sum: y and out must be of one type, f32, bf16 or f16");
+        if (!IsFloat(y->dtype) || !(out->dtype == y->dtype || (y->dtype == KUDNN_DT_F32 && IsFloat(out->dtype)))) {
+            return Unsupported("weighted sum: y and out must be of one type, f32, bf16 or f16, or y of f32 and out of 16 bits");
         }
         if (y->dims[1] != out->dims[1]) {
             return Bad("weighted sum: y and out have different widths");
@@ -793,6 +800,7 @@ int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kudnn_tensor_desc
         p->ldo = ldo;
         p->k = top_k;
         p->dt = y->dtype;
+        p->outDt = out->dtype;
         p->desc = "moe_combine T=" + std::to_string(p->T) + " R=" + std::to_string(p->R) + " N=" + std::to_string(p->N) +
                   " k=" + std::to_string(top_k);
         *plan = p;
@@ -812,7 +820,7 @@ int kudnn_moe_combine_run(kudnn_moe_combine_t plan, const void *y, const float *
     if ((y == nullptr && plan->R > 0) || slots == nullptr || out == nullptr) {
         return Null("weighted sum: one of the buffers is nullptr");
     }
-    const int s = CheckBuffers({Buffer{y, plan->dt}, Buffer{weights, KUDNN_DT_F32}, Buffer{slots, KUDNN_DT_S32}, Buffer{out, plan->dt}});
+    const int s = CheckBuffers({Buffer{y, plan->dt}, Buffer{weights, KUDNN_DT_F32}, Buffer{slots, KUDNN_DT_S32}, Buffer{out, plan->outDt}});
     if (s != KUDNN_STATUS_SUCCESS) {
         return s;
     }
@@ -828,6 +836,7 @@ int kudnn_moe_combine_run(kudnn_moe_combine_t plan, const void *y, const float *
     a.ldo = plan->ldo;
     a.k = plan->k;
     a.dt = plan->dt;
+    a.out_dt = plan->outDt;
     return Launched(kudnn_launch_moe_combine(a, static_cast<hipStream_t>(stream)), "weighted sum: launch failed");
 }
 
@@ -836,6 +845,9 @@ int kudnn_moe_combine_backward(kudnn_moe_combine_t plan, const void *y, const fl
 {
     if (plan == nullptr) {
         return Null("weighted sum: null plan");
+    }
+    if (plan->outDt != plan->dt) {
+        return Unsupported("weighted sum: the gradients need y and out of one type");
     }
     if (dy == nullptr && dweights == nullptr) {
         return KUDNN_STATUS_SUCCESS;
@@ -861,7 +873,7 @@ int kudnn_moe_combine_backward(kudnn_moe_combine_t plan, const void *y, const fl
     a.ldy = plan->ldy;
     a.ldo = plan->N;
     a.k = plan->k;
-    a.dt = plan->dt;
+    a.dt = a.out_dt = plan->dt;
     return Launched(kudnn_launch_moe_combine_backward(a, static_cast<hipStream_t>(stream)), "weighted sum: launch failed");
 }
 

@@ -79,9 +79,9 @@ void GroupedLinear::Run(const void *x, const void *w, const std::int32_t *offset
     Abi::Check(kudnn_grouped_linear_run(Get(pImpl), x, w, offsets, rows, y, stream));
 }
 void GroupedLinear::BackwardInput(const void *dy, const void *w, const std::int32_t *offsets, void *dx, void *workspace,
-                                  void *stream) const noexcept(false)
+                                  void *stream, Element::TypeT dxType) const noexcept(false)
 {
-    Abi::Check(kudnn_grouped_linear_backward_input(Get(pImpl), dy, w, offsets, dx, workspace, stream));
+    Abi::Check(kudnn_grouped_linear_backward_input(Get(pImpl), dy, w, offsets, dx, static_cast<int>(dxType), workspace, stream));
 }
 void GroupedLinear::BackwardWeight(const void *dy, const void *x, const std::int32_t *offsets, const std::int32_t *rows, void *dw,
                                    void *workspace, void *stream) const noexcept(false)

@@ -240,11 +240,15 @@ def _grouped_backward(x, w, offsets, rows, slots, dy, wants_dx, wants_dw):
     plan = _grouped_plan(x, w, dy.shape[0], rows is not None)
     stream, ws = _stream(device.index), _workspace(plan, device)
     dx = dw = None
-    if wants_dx:
+    if wants_dx and rows is None:
         dx = torch.empty((dy.shape[0], x.shape[1]), dtype=x.dtype, device=device)
         plan.backward_input(dy, w, offsets, dx, stream, ws)
-        if rows is not None:
-            dx = _combine(dx, None, slots)
+    elif wants_dx:
+        # a token's gradient is one sum over its slots: f32 rows until it is whole. Rows of 16 bits save 1 to 2 % of forward and
+        # backward (8192 tokens, 2 of 8 experts, 4096 x 4096: 1520 against 1537 us) and leave 1.4 times the error.
+        dx = torch.empty((dy.shape[0], x.shape[1]), dtype=torch.float32, device=device)
+        plan.backward_input(dy, w, offsets, dx, stream, ws, F32)
+        dx = _combine(dx, None, slots, x.dtype)
     if wants_dw:
         dw = torch.empty(w.shape, dtype=w.dtype, device=device)
         plan.backward_weight(dy, x, offsets, rows, dw, stream, ws)
@@ -394,20 +398,19 @@ def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torc
 
 # ---- weighted sum
 
-def _combine_plan(y, tokens, k) -> MoeCombine:
-    dt = _FLOAT[y.dtype]
-    return _plan(("combine", y.shape, y.stride(), y.dtype, tokens, k),
-                 lambda: MoeCombine(_matrix_desc(y, dt), desc([tokens, y.shape[1]], dt), k))
+def _combine_plan(y, tokens, k, dtype) -> MoeCombine:
+    return _plan(("combine", y.shape, y.stride(), y.dtype, tokens, k, dtype),
+                 lambda: MoeCombine(_matrix_desc(y, _FLOAT[y.dtype]), desc([tokens, y.shape[1]], _FLOAT[dtype]), k))
 
 
-def _combine(y, weights, slots):
+def _combine(y, weights, slots, dtype):
     device = y.device
     if _current() != device.index:
         with torch.cuda.device(device):
-            return _combine(y, weights, slots)
+            return _combine(y, weights, slots, dtype)
     tokens, k = slots.shape
-    out = torch.empty((tokens, y.shape[1]), dtype=y.dtype, device=device)
-    rc = lib().kudnn_moe_combine_run(_combine_plan(y, tokens, k).handle, y.data_ptr(), _at(weights), slots.data_ptr(), out.data_ptr(),
+    out = torch.empty((tokens, y.shape[1]), dtype=dtype, device=device)
+    rc = lib().kudnn_moe_combine_run(_combine_plan(y, tokens, k, dtype).handle, y.data_ptr(), _at(weights), slots.data_ptr(), out.data_ptr(),
                                      _stream(device.index))
     if rc:
         check(rc)
@@ -421,7 +424,7 @@ def _combine_backward(y, weights, slots, dout, wants_dy, wants_dw):
             return _combine_backward(y, weights, slots, dout, wants_dy, wants_dw)
     dy = torch.empty(y.shape, dtype=y.dtype, device=device) if wants_dy else None
     dw = torch.empty(slots.shape, dtype=torch.float32, device=device) if wants_dw else None
-    rc = lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
+    rc = lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape, y.dtype).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
                                           dout.data_ptr(), _at(dy), _at(dw), _stream(device.index))
     if rc:
         check(rc)
@@ -432,7 +435,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, slots):
         ctx.save_for_backward(y, weights, slots)
-        return _combine(y, weights, slots)
+        return _combine(y, weights, slots, y.dtype)
 
     @staticmethod
     @_first_order
@@ -458,7 +461,7 @@ def combine(y: torch.Tensor, weights: Optional[torch.Tensor], slots: torch.Tenso
     w = None if weights is None else weights.contiguous()
     if (y.requires_grad or (w is not None and w.requires_grad)) and torch.is_grad_enabled():
         return _Combine.apply(ym, w, slots)
-    return _combine(ym, w, slots)
+    return _combine(ym, w, slots, y.dtype)
 
 
 # ---- the operators together

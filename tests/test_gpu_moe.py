@@ -710,3 +710,42 @@ def test_gradients_of_gradients_are_refused():
         (first,) = torch.autograd.grad(out.float().square().sum(), of, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             first.float().sum().backward()
+
+
+@pytest.mark.parametrize("counts,extra,tokens,width,out", SHAPES)
+def test_input_gradient_in_f32(counts, extra, tokens, width, out):
+    g = gen(width + out + 2)
+    offsets, _ = make_order(counts, extra, tokens, g)
+    count = sum(counts) + extra
+    w = (randn(g, len(counts), out, width) * width ** -0.5).half()
+    dy = randn(g, count, out).half()
+    x = torch.zeros(count, width, dtype=torch.float16, device=DEV)
+    _, _, dxs, mx, *_ = grouped_plain(x, w, offsets, None, count, dy)
+    plan = K.GroupedLinear(K.desc(x.shape, K.F16), K.desc([len(counts), width, out], K.F16, "ACB"), K.desc([count, out], K.F16))
+    dx = torch.full((count, width), math.nan, device=DEV)
+    ws = torch.full((plan.workspace_bytes,), 255, dtype=torch.uint8, device=DEV)
+    plan.backward_input(dy, w, offsets, dx, torch.cuda.current_stream(), ws, K.F32)
+    near(dx, dxs, mx, out + 1, "dx")
+    assert float(dx[sum(counts):].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("tokens,k,width,pitch", [(1, 1, 8, 8), (37, 5, 1000, 1000), (60, 8, 41, 41), (9, 4, 2056, 2064), (300, 3, 64, 66), (5, 2, 7, 9)])
+def test_combine_of_f32_rows_into_16_bits(tokens, k, width, pitch, dtype):
+    g = gen(width + k)
+    dt = HALF[dtype]
+    y = randn(g, tokens * k, pitch)[:, :width]
+    weights = randn(g, tokens, k)
+    slots = torch.randperm(tokens * k, generator=g, device=DEV).int().reshape(tokens, k)
+    slots[torch.rand(tokens, k, generator=g, device=DEV) < 0.2] = -1
+    slots[tokens // 2] = -1                                     # a token without any
+    kind = K.BF16 if dtype == "bf16" else K.F16
+    plan = K.MoeCombine(K.desc(y.shape, K.F32, "AB", y.stride()), K.desc([tokens, width], kind), k)
+    rows = torch.where((slots >= 0)[:, :, None], y.double()[slots.long().clamp_min(0)], 0.0)
+    for w in (weights, None):
+        out = torch.full((tokens, width), math.nan, dtype=dt, device=DEV)
+        plan.run(y, w, slots, out, torch.cuda.current_stream())
+        scale = torch.ones_like(weights).double() if w is None else w.double()
+        near(out, (rows * scale[:, :, None]).sum(1), (rows * scale[:, :, None]).abs().sum(1), k + 1, "out")
+    with pytest.raises(RuntimeError):
+        plan.backward(y, weights, slots, out, None, torch.empty(tokens, k, device=DEV), torch.cuda.current_stream())

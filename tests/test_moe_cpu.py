@@ -141,3 +141,15 @@ def test_torch_entry_points_refuse_host_tensors():
                  lambda: km.linear_fp8(x, w[0].to(torch.float8_e4m3fn), torch.ones(1, 1))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_types_of_the_input_gradient_and_of_f32_rows():
+    host = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(host) // 64 * 64 + 64
+    g = K.GroupedLinear(K.desc([4, 8], K.BF16), K.desc([2, 8, 8], K.BF16, "ACB"), K.desc([4, 8], K.BF16))
+    refused(K.UNSUPPORTED, lambda: g.backward_input(at, at, at, at, dx_dtype=K.F16))
+    refused(K.BAD_ARGUMENTS, lambda: g.backward_input(at, at, at, at, dx_dtype=K.F32))       # host memory
+    c = K.MoeCombine(K.desc([12, 40], K.F32), K.desc([5, 40], K.F16), 2)
+    refused(K.UNSUPPORTED, lambda: c.backward(at, at, at, at, at))
+    refused(K.UNSUPPORTED, lambda: K.MoeCombine(K.desc([12, 40], K.BF16), K.desc([5, 40], K.F16), 2))
+    refused(K.UNSUPPORTED, lambda: K.MoeCombine(K.desc([12, 40], K.F32), K.desc([5, 40], K.S32), 2))
