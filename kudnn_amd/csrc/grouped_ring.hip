@@ -7,7 +7,7 @@
 // everyone's have landed, and everyone is done with the block before), send the copies of the block S - 1 ahead into the
 // stage that the barrier freed, read the fragments, multiply.
 // Fragments, swizzle, exact e4m3 (by bf16 MFMAs) and what lies outside the operands: as in grouped_stream.hip. The row scales
-// come with a block's copies, a word a row, so that no load of the compiler's own waits for the ring.
+// are copied to LDS as well, so that no load of the compiler's own waits for the ring.
 //
 // Two blocks leave room for three workgroups of 64-row tiles a CU or two of 128, whose starts and ends hide under one another's
 // blocks; four blocks (one workgroup a CU) pay where there are fewer tiles than that. Measured: 64 experts of 64 rows on
@@ -27,13 +27,6 @@ __device__ __forceinline__ void wait_copies()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
 }
 
-// One word a lane to LDS: lane l's 4 bytes land at lds + 4 l.
-__device__ __forceinline__ void copy_words(i32x4_t rs, uint32_t voff, uint32_t soff, uint32_t lds)
-{
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %3 offen lds"
-                 ::"v"(voff), "s"(rs), "s"(lds), "s"(soff) : "memory");
-}
-
 // HINT: the weights are read by one row tile (non-temporal). NATIVE: e4m3 products by the e4m3 matrix instruction.
 // REG (two stages): rows of any alignment and length (16 bytes at least) go to LDS through registers, a block ahead, since a
 // copy moves whole aligned chunks only.
@@ -45,9 +38,10 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
     constexpr int MT = BM / WM / 16, NT = BN / WN / 16;            // 16 x 16 results of a wave
     constexpr int kRows = (BM + BN) / 8, kCopies = kRows / W;       // 8-row copies of a block, and of a wave
     static_assert(kRows % W == 0, "copies are dealt evenly");
-    constexpr int kSent = kCopies + (F8 ? 1 : 0);                   // vector memory operations of a wave and block
-    constexpr int kScales = F8 ? BM / 4 : 0, kStage = (BM + BN) * 8 + kScales;   // 16-byte chunks of a stage
+    constexpr int kScaleWaves = F8 ? BM / 64 : 0;                   // each copies the scales of 64 rows
+    constexpr int kStage = (BM + BN) * 8;                           // 16-byte chunks of a stage
     __shared__ uint4 lds[S * kStage];
+    __shared__ uint4 scales[F8 ? 2 * BM : 1];                       // [two runs of four blocks][row]: a word a block
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, row16 = lane & 15, grp = lane >> 4;
 
@@ -86,14 +80,18 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
             vo[i] = j0 + row - BM < g.J ? static_cast<uint32_t>(row - BM) * ldb + c : kOut;
         }
     }
-    // row scales of a block: wave w copies those of 64 rows from 64 (w % (BM / 64)), some of them twice
+    // Row scales: those of four blocks at once (of the row's last four at its end), by one lane a row. A word a block and row, copied
+    // by every wave, were more requests than the operands' copies: 64 experts of 64 rows on average, 2048 x 4096, took 152 us
+    // instead of 137.
     const uint32_t KB = static_cast<uint32_t>((g.C + 127) / 128);
+    const int lastRun = KB > 4u ? static_cast<int>(KB) - 4 : 0;
+    auto run_of = [&](int kb) __attribute__((always_inline)) { return (kb & ~3) < lastRun ? kb & ~3 : lastRun; };   // its first block
     uint32_t vs = kOut;
     i32x4_t rsc = ra;
     const_float *sw = nullptr;
     if constexpr (F8) {
-        const int r = t.r0 + (wave % (BM / 64)) * 64 + lane;
-        const int64_t s = r < t.end ? source_row(g, r) : -1;
+        const int r = t.r0 + wave * 64 + lane;
+        const int64_t s = wave < kScaleWaves && r < t.end ? source_row(g, r) : -1;
         vs = s < 0 ? kOut : static_cast<uint32_t>(s) * KB * 4u;
         rsc = resource(g.a_scale, static_cast<uint64_t>(g.S) * KB * 4u);
         sw = (const_float *)(g.b_scale + (static_cast<int64_t>(e) * ((g.J + 127) / 128) + tj) * KB);
@@ -114,14 +112,22 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
                 copy_lds<HINT>(rb, v, at, at16);
             }
         }
-        if constexpr (F8) {
-            copy_words(rsc, vs, static_cast<uint32_t>(kb) * 4u, to + static_cast<uint32_t>((BM + BN) * 128 + (wave % (BM / 64)) * 256));
+    };
+    const uint32_t baseScales = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)scales));
+    auto copy_scales = [&](int kb) __attribute__((always_inline)) {
+        if (wave >= kScaleWaves) return;
+        const int buffer = ((kb >> 2) & 1) * BM + wave * 64;
+        if (KB >= 4u) {
+            copy_lds<false>(rsc, vs, static_cast<uint32_t>(run_of(kb)) * 4u, baseScales + static_cast<uint32_t>(buffer) * 16u);
+        } else {                                                    // rows of less than 16 bytes
+            float *to = reinterpret_cast<float *>(scales + buffer + lane);
+            for (uint32_t q = 0; q < KB; ++q) to[q] = vs != kOut ? g.a_scale[vs / 4u + q] : 0.0f;
         }
     };
 
     // the same through registers
     u32x4_t held[REG ? kCopies : 1];
-    float heldScale = 0.0f;
+    u32x4_t heldScales{0u, 0u, 0u, 0u};
     auto load = [&](int kb) __attribute__((always_inline)) {
         const uint32_t at = static_cast<uint32_t>(kb) * 128u;
         const bool tail = at + 128u > rowBytes;
@@ -135,12 +141,21 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
             }
             held[REG ? i : 0] = x;
         }
-        if constexpr (F8) heldScale = vs != kOut ? g.a_scale[vs / 4u + static_cast<uint32_t>(kb)] : 0.0f;
+        if constexpr (F8) {
+            if (vs != kOut && (kb & 3) == 0) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (static_cast<uint32_t>(run_of(kb) + q) < KB) heldScales[q] = f2u(g.a_scale[vs / 4u + static_cast<uint32_t>(run_of(kb) + q)]);
+                }
+            }
+        }
     };
-    auto put = [&](int stage) __attribute__((always_inline)) {
+    auto put = [&](int kb, int stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) lds[stage * kStage + (wave * kCopies + i) * 64 + lane] = __builtin_bit_cast(uint4, held[REG ? i : 0]);
-        if constexpr (F8) reinterpret_cast<float *>(lds + stage * kStage + (BM + BN) * 8)[(wave % (BM / 64)) * 64 + lane] = heldScale;
+        if constexpr (F8) {
+            if (wave < kScaleWaves && (kb & 3) == 0) scales[((kb >> 2) & 1) * BM + wave * 64 + lane] = __builtin_bit_cast(uint4, heldScales);
+        }
     };
 
     f32x4_t acc[NT][MT];
@@ -159,11 +174,11 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
             for (int i = 0; i < MT; ++i) a[i][h] = __builtin_bit_cast(u32x4_t, at[((wm * MT + i) * 16 + row16) * 8 + ((grp + 4 * h) ^ sw16)]);
         }
         if constexpr (F8) {
-            const float *sx = reinterpret_cast<const float *>(at + (BM + BN) * 8);
+            const float *sx = reinterpret_cast<const float *>(scales + ((kb >> 2) & 1) * BM) + (kb - run_of(kb));
             const float swb = sw[kb];
             float s[MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) s[i] = sx[(wm * MT + i) * 16 + row16] * swb;
+            for (int i = 0; i < MT; ++i) s[i] = sx[((wm * MT + i) * 16 + row16) * 4] * swb;
             if constexpr (NATIVE) {
                 // one instruction a block and 16 x 16 results; lane group g has the 16 indices of chunk g and those of g + 4
 #pragma unroll
@@ -225,31 +240,33 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_ring_kernel(GroupedArgs 
         static_assert(S == 2, "one block in use, one written");
         if (blocks > 0) {
             load(0);
-            put(0);
+            put(0, 0);
             if (blocks > 1) load(1);
         }
         for (int kb = 0; kb < blocks; ++kb) {
             __syncthreads();     // block kb is written, block kb - 1 has been read
-            if (kb + 1 < blocks) put((kb + 1) & 1);
+            if (kb + 1 < blocks) put(kb + 1, (kb + 1) & 1);
             if (kb + 2 < blocks) load(kb + 2);
             multiply(kb, kb & 1);
         }
     }
+    if (F8 && !REG && blocks > 0) copy_scales(0);
 #pragma unroll
     for (int s = 0; s < S - 1 && !REG; ++s) {
         if (s < blocks) copy(s, s);
     }
     int stage = 0;
     for (int kb = 0; kb < blocks && !REG; ++kb) {
-        // blocks kb + 1 .. kb + S - 2 may still be on their way
+        // blocks kb + 1 .. kb + S - 2 may still be on their way (scales were sent at least S - 1 blocks ago)
         if (kb + S - 2 < blocks) {
-            wait_copies<(S - 2) * kSent>();
+            wait_copies<(S - 2) * kCopies>();
         } else {
             wait_copies<0>();
         }
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const int freed = stage == 0 ? S - 1 : stage - 1;
+        if (F8 && (kb & 3) == 0 && kb + 4 < blocks) copy_scales(kb + 4);
         if (kb + S - 1 < blocks) copy(kb + S - 1, freed);
         multiply(kb, stage);
         stage = stage == S - 1 ? 0 : stage + 1;

@@ -749,3 +749,18 @@ def test_combine_of_f32_rows_into_16_bits(tokens, k, width, pitch, dtype):
         near(out, (rows * scale[:, :, None]).sum(1), (rows * scale[:, :, None]).abs().sum(1), k + 1, "out")
     with pytest.raises(RuntimeError):
         plan.backward(y, weights, slots, out, None, torch.empty(tokens, k, device=DEV), torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 3, 4, 5, 7, 9])
+@pytest.mark.parametrize("any_row", [0, 1])
+def test_fp8_scales_of_short_and_odd_rows(blocks, any_row):
+    """As many rows as the ring tiles take, whose row scales are read four blocks at a time; no scale past the last row's."""
+    g = gen(blocks)
+    counts, width, out = [70, 0, 61, 90, 33] * 6, blocks * 128 - 16 + any_row, 264
+    offsets, rows = make_order(counts, 0, 200, g)
+    x = (randn(g, 200, width) * torch.exp(randn(g, 200, 1))).bfloat16()
+    w, ws = make_fp8(g, len(counts), out, width)
+    q, s = km.quantize_rows(x)
+    y = km.grouped_linear_fp8(q, w, ws, offsets, rows, x_scale=s, out_dtype=torch.float32)
+    want, mag, *_ = grouped_plain(dequant(q, s), dequant(w, ws, 128), offsets, rows, sum(counts))
+    near(y, want, mag, width + 3 * (width // 128 + 1), "y")
