@@ -19,7 +19,7 @@
 //
 // e4m3: one v_mfma_*_16x16x128 covers a block of 128 for 16 x 16 outputs; its result is added to the running f32 sum times
 // sx[row] sw[block]. A lane's four results share the row of x, so a k-tile costs a wave 32 MFMAs (1024 cycles), 128 fused
-// multiply-adds (512) and 4 products of scales. The row scales are loaded three k-tiles ahead, a lane a row, and pass to the
+// multiply-adds (512) and 4 products of scales. The row scales are loaded for three k-tiles at once, a lane a row, and pass to the
 // lanes that need them through ds_bpermute.
 //
 // Tiles of at most 128 rows ("halves") have a form of their own: their waves lie 2 x 4 over 128 x 256, and A takes half the room,
@@ -301,9 +301,9 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         }
     };
 
-    // ---- scales (e4m3): lane l holds sx of row 64 p + l for the three k-tiles to come
+    // ---- scales (e4m3): lane l holds sx of row 64 p + l for these three k-tiles and the next
     const int KB = static_cast<int>((ga.C + 127) / 128);
-    float sx[3];
+    float sx[2][3];
     uint32_t sxAt = kOut;
     const_float *sw = nullptr;
     if constexpr (F8) {
@@ -315,7 +315,19 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
         nb = nb < NB ? nb : NB - 1;                 // a half tile past the last column: its results are not stored
         sw = (const_float *)(ga.b_scale + ((e < E ? e : 0) * NB + nb) * KB);
     }
-    auto load_sx = [&](int t) __attribute__((always_inline)) { return sxAt != kOut && t < nk ? ga.a_scale[sxAt + static_cast<uint32_t>(t)] : 0.0f; };
+    auto load_sx = [&](int t, float (&v)[3]) __attribute__((always_inline)) {
+        v[0] = v[1] = v[2] = 0.0f;
+        if (sxAt == kOut) return;
+        const float *at = ga.a_scale + sxAt + static_cast<uint32_t>(t);
+        if (t + 2 < nk) {
+            v[0] = at[0], v[1] = at[1], v[2] = at[2];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (t + q < nk) v[q] = at[q];
+            }
+        }
+    };
 
     // ---- fragments
     const int lrow = lane & 31, lh = lane >> 5;
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
             const float swt = sw[t];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s8[i] = u2f(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute((i * 16 + row16) * 4, static_cast<int>(f2u(sx[I % 3]))))) * swt;
+                s8[i] = u2f(static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute((i * 16 + row16) * 4, static_cast<int>(f2u(sx[I / 3][I % 3]))))) * swt;
             }
         } else {
 #pragma unroll
@@ -413,8 +425,8 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
                 wait_vmcnt<0>();
             }
         }
-        if constexpr (F8) {
-            sx[I % 3] = load_sx(t + 3);
+        if constexpr (F8 && I % 3 == 0) {
+            load_sx(t + 3, sx[1 - I / 3]);
         }
         if (AK && gatherK && (tt & 3) == 0) {
             load_rows((tt >> 2) + 1);
@@ -511,7 +523,7 @@ __global__ __launch_bounds__(512, 1) void grouped_pingpong_kernel(GroupedArgs ga
 
     if (nk > 0) {
         if constexpr (F8) {
-            sfor<3>([&](auto ic) __attribute__((always_inline)) { sx[decltype(ic)::value] = load_sx(decltype(ic)::value); });
+            load_sx(0, sx[0]);
         }
         if (AK && gatherK) {
             load_rows(0);
