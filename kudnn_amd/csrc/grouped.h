@@ -45,7 +45,8 @@ inline bool kudnn_grouped_native(int64_t R, int64_t N, int64_t K, int c_dt)
 // of an average of r, and half a tile more than r rows fill.
 // The figures are a fit to 322 products timed on MI355X on every kernel (1 to 128 groups of 1 to 4096 rows, K and N = 256 to
 // 8192, 16-bit and e4m3; weights rotated past the Infinity Cache): the choice takes 1.012 times the best kernel's time on average,
-// and more than 1.1 times in 14 of them (1.21 at most); on 144 more with skewed sizes (a softmax over normal numbers) 1.038 times.
+// and more than 1.1 times in 14 of them (1.21 at most); on 144 more with skewed sizes (a softmax over normal numbers) 1.037 times
+// (timed after the ring's e4m3 tiles had become a tenth faster than the fit has them).
 // Always 256 x 256 tiles, or one tile of 64 x 64, would take 2 to 5 times.
 // any: operands that are not whole 16-byte chunks. They pass through registers, which the 256 x 256 tiles and the 64 x 64 tiles
 // of 8 waves have none left for and the longer ring has no use for; the others stay in the order that the figures give them.
