@@ -28,13 +28,15 @@ struct GroupedTile {
 
 // e4m3 operands. The e4m3 matrix instruction aligns the products of 8 consecutive indices to the largest of them and drops
 // what lies more than 13 bits below it (measured: beside 2^16 a product of 2^2 is lost, at a distance of 8 indices it is kept);
-// bf16 holds e4m3 exactly, and its instruction sums in f32, at half the rate and with the widening to do. Products into f32
+// bf16 holds e4m3 exactly, and its instruction sums in f32, at half the rate and with the widening to do. Products into f32 and f16
 // are formed that way, and so are those of less than 2^33 operations, whose time is the weight's way from HBM and the launch
-// (8 experts of 32 rows, 2048 x 4096: 21 us exact, 18 us native). Larger ones into 16 bits, whose rounding is 32 times coarser than what
-// is dropped, take the native instruction (4096 x 4096 x 4096: 66 us native, 166 exact; 64 experts of 64 rows, 2048 x 4096: 144 and 207).
+// (8 experts of 32 rows, 2048 x 4096: 21 us exact, 18 us native). Larger ones into bf16, whose rounding is 32 times coarser than what
+// is dropped, take the native instruction (4096 x 4096 x 4096: 66 us native, 166 exact; 64 experts of 64 rows, 2048 x 4096: 144 and 207):
+// the error against 64 bits in norm is 0.001658 either way at 4096 x 4096 x 11008 (203 us native, 425 exact). f16's rounding is only 4 times
+// coarser, and there it grew from 2.072e-4 to 2.098e-4.
 inline bool kudnn_grouped_native(int64_t R, int64_t N, int64_t K, int c_dt)
 {
-    return c_dt != KUDNN_DT_F32 && static_cast<double>(R) * static_cast<double>(N) * static_cast<double>(K) >= 4294967296.0;
+    return c_dt == KUDNN_DT_BF16 && static_cast<double>(R) * static_cast<double>(N) * static_cast<double>(K) >= 4294967296.0;
 }
 
 // The tile with the least estimate for R rows in `groups` groups of weights N x K (rows of `es` bytes an element). A tile's

@@ -368,6 +368,10 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
                x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y = x @ weight.T + bias with e4m3 operands and a scale for each block of 128, summed in f32, rounded once.
 
+    The products of a block are exact in f32, except that bfloat16 results of 2**33 operations or more come from the e4m3 matrix
+    instruction, which drops what lies more than 13 bits below the largest of 8 products, some 32 times below bfloat16's rounding.
+    out_dtype=torch.float32 has exact products at every size.
+
     x: [..., K], bfloat16 or float16 (quantised here as ``quantize_rows`` does), or e4m3 with x_scale; weight: [N, K] and
     weight_scale as ``quantize_blocks`` gives them; bias: [N] of the output's type. out_dtype: x's type, bfloat16 for e4m3 x.
     """
