@@ -339,8 +339,8 @@ KUDNN_HIP_API int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kud
 KUDNN_HIP_API int kudnn_moe_combine_run(kudnn_moe_combine_t plan, const void *y, const float *weights,
                                         const int32_t *slots, void *out, void *stream);
 /* dy[slots[t][j]] = weights[t][j] dout[t] (dense {R, N}) and dweights[t][j] = dout[t] . y[slots[t][j]] (f32, 0 without a
- * slot). The slots are the router's: each row of 0 .. n - 1 once, n the number of slots that are not -1; the rows from n on
- * are set to zero. Either output may be NULL. */
+ * slot). Slots name a row at most once, as the router's do; rows of dy that none names are zero, wherever they lie (a caller may take
+ * choices out by -1). Either output may be NULL. */
 KUDNN_HIP_API int kudnn_moe_combine_backward(kudnn_moe_combine_t plan, const void *y, const float *weights,
                                              const int32_t *slots, const void *dout, void *dy, float *dweights,
                                              void *stream);

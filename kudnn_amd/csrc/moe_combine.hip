@@ -6,8 +6,8 @@
 // line of consecutive lanes; rows that are not whole 16-byte pieces take the same kernel with one element a thread.
 // Sums over j run in j's order and dot products in a fixed tree, so results do not depend on timing.
 // What passes through once is read and written non-temporally: 8192 tokens x 4 rows of 4096 bf16 take 60 us forward
-// (335 MB, 5.6 TB/s; 73 us with cached accesses) and 130 us backward (604 MB, 4.6 TB/s; 144 us cached), where a plain copy
-// of 2 GiB reaches 4.9 TB/s.
+// (335 MB, 5.6 TB/s; 73 us with cached accesses) and 116 us backward (604 MB, 5.2 TB/s), where a plain copy of 2 GiB reaches 4.9
+// TB/s.
 #include "device_common.h"
 #include "moe.h"
 
@@ -111,32 +111,68 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a)
     }
 }
 
-// A workgroup a token (the last one: the rows that no slot takes). Thread partials of the k dot products meet in LDS.
+// Rows of dy that no slot names are zero: workgroup `id` of `1 << shift` has the rows r with r % (1 << shift) == id, marks in LDS those that
+// are named, and clears the others. Rows are dealt in turn, since a router leaves its unused rows together at the end. These workgroups
+// start first and read under the others' traffic: 8192 x 4 rows of 4096 bf16 with 0, a 16th and half of the tokens without experts take 116, 111
+// and 89 us (130, 231 and 956 where one workgroup counted the slots and cleared the rows past the count).
+constexpr int kMarks = 131072;       // rows of a workgroup that one reading of the slots can mark: 2^25 rows of y in one
+
+template <int DT, int VEC>
+__device__ __forceinline__ void clear_unnamed(const CombineArgs &a, uint32_t id, int shift, uint32_t *named)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t slots = a.T * a.k, mine = ((a.R - 1 - id) >> shift) + 1;   // id < R
+    const bool quads = reinterpret_cast<uintptr_t>(a.slots) % 16 == 0;
+    float zero[VEC];
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) zero[q] = 0.0f;
+    for (int64_t base = 0; base < mine; base += kMarks) {
+        const int rows = static_cast<int>(mine - base < kMarks ? mine - base : kMarks), words = (rows + 31) / 32;
+        for (int w = threadIdx.x; w < words; w += kThreads) named[w] = 0u;
+        __syncthreads();
+        auto mark = [&](int s) __attribute__((always_inline)) {
+            const int64_t at = (static_cast<int64_t>(s) >> shift) - base;
+            if (s >= 0 && s < a.R && (static_cast<uint32_t>(s) & ((1u << shift) - 1u)) == id && at >= 0 && at < rows) {
+                atomicOr(&named[at >> 5], 1u << (at & 31));
+            }
+        };
+        const int64_t whole = quads ? slots / 4 : 0;
+        const int4 *four = reinterpret_cast<const int4 *>(a.slots);
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < whole; i += kThreads) {
+            const int4 s = four[i];
+            mark(s.x), mark(s.y), mark(s.z), mark(s.w);
+        }
+        for (int64_t i = whole * 4 + threadIdx.x; i < slots; i += kThreads) mark(a.slots[i]);
+        __syncthreads();
+        for (int w = wave; w < words; w += kThreads / 64) {
+            uint32_t free = ~named[w] & (rows - w * 32 >= 32 ? ~0u : (1u << (rows - w * 32)) - 1u);
+            while (free != 0u) {
+                const int64_t row = ((base + w * 32 + __ffs(free) - 1) << shift) + id;
+                free &= free - 1u;
+                for (int64_t col = lane * VEC; col < a.N; col += 64 * VEC) store_vec<DT, VEC>(a.dy, row * a.N + col, zero);
+            }
+        }
+        __syncthreads();   // before the next marks
+    }
+}
+
+// The first `1 << shift` workgroups (none with shift < 0) clear the rows that no slot names, as long as the others take; then a workgroup
+// a token. Thread partials of the k dot products meet in LDS.
 template <int DT, bool WIDE>
-__global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs a)
+__global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs a, int shift)
 {
     constexpr int VEC = vec_of<DT, WIDE>();
     constexpr int kWaves = kThreads / 64;
     __shared__ float part[64][kWaves];
-    __shared__ int count;
+    __shared__ uint32_t named[kMarks / 32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (blockIdx.x == gridDim.x - 1) {
-        // rows n .. R - 1 have no slot: zero
-        if (a.dy == nullptr) return;
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        int mine = 0;
-        for (int64_t i = threadIdx.x; i < a.T * a.k; i += kThreads) mine += a.slots[i] >= 0 ? 1 : 0;
-        atomicAdd(&count, mine);
-        __syncthreads();
-        const int64_t all = a.R * a.N;
-        float zero[VEC];
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) zero[q] = 0.0f;
-        for (int64_t i = count * a.N + threadIdx.x * VEC; i < all; i += kThreads * VEC) store_vec<DT, VEC>(a.dy, i, zero);
+    const uint32_t clearing = shift < 0 ? 0u : 1u << shift;
+    if (blockIdx.x < clearing) {
+        clear_unnamed<DT, VEC>(a, blockIdx.x, shift, named);
         return;
     }
-    const int64_t t = blockIdx.x;
+    const int64_t t = blockIdx.x - clearing;
     for (int j = 0; j < a.k; ++j) {
         const int64_t s = slot_of(a, t, j);
         const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
@@ -189,11 +225,17 @@ int launch(const CombineArgs &a, bool wide, hipStream_t stream)
 template <int DT>
 int launch_backward(const CombineArgs &a, bool wide, hipStream_t stream)
 {
-    const unsigned grid = static_cast<unsigned>(a.T + 1);
+    // clearing workgroups: a power of two, up to 256, of 64 rows each or more where there are that few
+    int shift = a.dy != nullptr && a.R > 0 && a.N > 0 ? 0 : -1;
+    while (shift >= 0 && shift < 8 && (int64_t(64) << shift) < a.R) ++shift;
+    const unsigned grid = static_cast<unsigned>(a.T + (shift < 0 ? 0 : 1 << shift));
+    if (grid == 0) {
+        return 0;
+    }
     if (wide) {
-        combine_backward_kernel<DT, true><<<grid, kThreads, 0, stream>>>(a);
+        combine_backward_kernel<DT, true><<<grid, kThreads, 0, stream>>>(a, shift);
     } else {
-        combine_backward_kernel<DT, false><<<grid, kThreads, 0, stream>>>(a);
+        combine_backward_kernel<DT, false><<<grid, kThreads, 0, stream>>>(a, shift);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

@@ -451,8 +451,8 @@ def combine(y: torch.Tensor, weights: Optional[torch.Tensor], slots: torch.Tenso
     """out[t] = sum over j of weights[t, j] * y[slots[t, j]], summed in f32, rounded once to y's type.
 
     y: [R, N], float32, bfloat16 or float16; weights: float32 [T, k], or None for ones; slots: int32 [T, k] as ``route`` gives
-    them, -1 adds nothing. Differentiable in y and weights; the rows of y that no slot takes are the last ones, and get a
-    gradient of zero.
+    them, no row twice; any of them may be set to -1 (as may what names no row of y), which adds nothing. Differentiable in y and
+    weights; the rows of y that no slot names get a gradient of zero.
     """
     if y.dim() != 2 or y.dtype not in _FLOAT:
         raise ValueError("kudnn combine: y must be a matrix of float32, bfloat16 or float16")

@@ -35,3 +35,67 @@ def test_large_fp8_products_into_f16_are_rounded_once(counts, width, out):
     near(y, want, mag, width + 3 * (width // 128 + 1), "y")
     off = lambda v: float((v.double() - want).norm() / want.norm())
     assert off(y) <= 1.003 * off(want.half())
+
+
+def combine_gradients(slots, rows, width, dtype, g, weighted=True):
+    """Gradients of the weighted sum, written over NaN, against the formula."""
+    tokens, k = slots.shape
+    y = randn(g, rows, width).to(dtype)
+    w = randn(g, tokens, k) if weighted else None
+    dout = randn(g, tokens, width).to(dtype)
+    kind = {torch.float32: K.F32, torch.bfloat16: K.BF16, torch.float16: K.F16}[dtype]
+    dy, dw = torch.full((rows, width), math.nan, dtype=dtype, device=DEV), torch.full((tokens, k), math.nan, device=DEV)
+    K.MoeCombine(K.desc([rows, width], kind), K.desc([tokens, width], kind), k).backward(y, w, slots, dout, dy, dw, torch.cuda.current_stream())
+    named = (slots >= 0) & (slots < rows)
+    want = torch.zeros(rows, width, dtype=torch.float64, device=DEV)
+    scale = torch.ones(tokens, k, device=DEV) if w is None else w
+    for j in range(k):
+        at = named[:, j].nonzero()[:, 0]
+        want[slots[at, j].long()] = scale[at, j, None].double() * dout[at].double()
+    near(dy, want, want.abs(), 1, "dy")
+    for j in range(k):
+        picked = torch.where(named[:, j, None], y.double()[torch.where(named[:, j], slots[:, j], 0).long()], 0.0) * dout.double()
+        near(dw[:, j], picked.sum(1), picked.abs().sum(1), width, "dweights")
+    return dy
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,k,width,rows", [(1, 1, 8, 1), (1, 2, 7, 300), (40, 3, 1000, 120), (40, 3, 129, 63), (300, 8, 64, 2400), (3000, 4, 16, 9000),
+                                                 (5000, 2, 3, 40000)])
+def test_combine_gradients_of_any_slots(tokens, k, width, rows, dtype):
+    """Slots taken out anywhere, more rows than slots and fewer, slots past the last row: the rows that none names are zero."""
+    g = gen(rows + width)
+    for out in (0.0, 0.3, 0.97):
+        order = torch.randperm(max(rows, tokens * k) + 50, generator=g, device=DEV)[:tokens * k].int().reshape(tokens, k)   # some past the last
+        slots = torch.where(torch.rand(tokens, k, generator=g, device=DEV) < out, torch.full_like(order, -1), order)
+        combine_gradients(slots, rows, width, dtype, g, out == 0.3)
+    combine_gradients(torch.full((tokens, k), -1, dtype=torch.int32, device=DEV), rows, width, dtype, g)
+    odd = torch.empty(tokens * k + 1, dtype=torch.int32, device=DEV)[1:].reshape(tokens, k)      # off 16 bytes
+    odd.copy_(order)
+    combine_gradients(odd, rows, width, dtype, g)
+
+
+def test_combine_gradient_of_more_rows_than_one_reading_marks():
+    rows = (1 << 25) + 777
+    g = gen(7)
+    slots = torch.randint(0, rows, (900, 2), generator=g, device=DEV, dtype=torch.int32)
+    slots[0], slots[1, 0] = torch.tensor([rows - 1, rows - 2]), 0
+    slots = torch.unique(slots.flatten())[-1700:].reshape(850, 2).contiguous()
+    combine_gradients(slots, rows, 1, torch.float16, g)
+
+
+def test_combine_after_choices_are_dropped():
+    """Choices over an expert's capacity set to -1 by the caller: gradients through torch, against differences of the output's formula."""
+    g = gen(17)
+    tokens, experts, k, width = 50, 6, 2, 40
+    r = km.route(randn(g, tokens, experts), k)
+    place = r.slots - r.offsets[:-1][r.experts.long()]
+    slots = torch.where(place < 8, r.slots, -1).int()
+    assert int((slots < 0).sum()) > 0
+    y = randn(g, tokens * k, width).requires_grad_(True)
+    dout = randn(g, tokens, width)
+    dy, = torch.autograd.grad(km.combine(y, r.weights, slots), y, dout)
+    want = torch.zeros(tokens * k, width, dtype=torch.float64, device=DEV)
+    keep = slots >= 0
+    want[slots[keep].long()] = (r.weights.double()[:, :, None] * dout.double()[:, None, :])[keep]
+    near(dy, want, want.abs(), 1, "dy")
