@@ -43,7 +43,7 @@ def _plan(key, make):
             return plan
         plan = _plans[key] = make()
         while len(_plans) > MAX_CACHED_PLANS:
-            _plans.popitem(last=False)  # destroyed once no caller holds it
+            _plans.popitem(last=False)  # destroyed once no caller holds it: callers keep the plan, not its handle alone
         return plan
 
 
@@ -160,9 +160,10 @@ def _route_backward(logits, mask, top_k, normalize, weights, experts, dweights):
     if _current() != device.index:
         with torch.cuda.device(device):
             return _route_backward(logits, mask, top_k, normalize, weights, experts, dweights)
+    plan = _route_plan(logits, mask, top_k, normalize)
     dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    rc = lib().kudnn_moe_route_backward(_route_plan(logits, mask, top_k, normalize).handle, logits.data_ptr(), _at(mask),
-                                        weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), _stream(device.index))
+    rc = lib().kudnn_moe_route_backward(plan.handle, logits.data_ptr(), _at(mask), weights.data_ptr(), experts.data_ptr(),
+                                        dweights.data_ptr(), dlogits.data_ptr(), _stream(device.index))
     if rc:
         check(rc)
     return dlogits
@@ -224,9 +225,10 @@ def _grouped(x, w, offsets, rows):
         with torch.cuda.device(device):
             return _grouped(x, w, offsets, rows)
     count = x.shape[0] if rows is None else rows.shape[0]
+    plan = _grouped_plan(x, w, count, rows is not None)
     y = torch.empty((count, w.shape[1]), dtype=x.dtype, device=device)
-    rc = lib().kudnn_grouped_linear_run(_grouped_plan(x, w, count, rows is not None).handle, x.data_ptr(), w.data_ptr(),
-                                        offsets.data_ptr(), _at(rows), y.data_ptr(), _stream(device.index))
+    rc = lib().kudnn_grouped_linear_run(plan.handle, x.data_ptr(), w.data_ptr(), offsets.data_ptr(), _at(rows), y.data_ptr(),
+                                        _stream(device.index))
     if rc:
         check(rc)
     return y
@@ -413,9 +415,9 @@ def _combine(y, weights, slots, dtype):
         with torch.cuda.device(device):
             return _combine(y, weights, slots, dtype)
     tokens, k = slots.shape
+    plan = _combine_plan(y, tokens, k, dtype)
     out = torch.empty((tokens, y.shape[1]), dtype=dtype, device=device)
-    rc = lib().kudnn_moe_combine_run(_combine_plan(y, tokens, k, dtype).handle, y.data_ptr(), _at(weights), slots.data_ptr(), out.data_ptr(),
-                                     _stream(device.index))
+    rc = lib().kudnn_moe_combine_run(plan.handle, y.data_ptr(), _at(weights), slots.data_ptr(), out.data_ptr(), _stream(device.index))
     if rc:
         check(rc)
     return out
@@ -426,10 +428,11 @@ def _combine_backward(y, weights, slots, dout, wants_dy, wants_dw):
     if _current() != device.index:
         with torch.cuda.device(device):
             return _combine_backward(y, weights, slots, dout, wants_dy, wants_dw)
+    plan = _combine_plan(y, *slots.shape, y.dtype)
     dy = torch.empty(y.shape, dtype=y.dtype, device=device) if wants_dy else None
     dw = torch.empty(slots.shape, dtype=torch.float32, device=device) if wants_dw else None
-    rc = lib().kudnn_moe_combine_backward(_combine_plan(y, *slots.shape, y.dtype).handle, y.data_ptr(), _at(weights), slots.data_ptr(),
-                                          dout.data_ptr(), _at(dy), _at(dw), _stream(device.index))
+    rc = lib().kudnn_moe_combine_backward(plan.handle, y.data_ptr(), _at(weights), slots.data_ptr(), dout.data_ptr(), _at(dy), _at(dw),
+                                          _stream(device.index))
     if rc:
         check(rc)
     return dy, dw
