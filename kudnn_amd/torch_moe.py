@@ -148,8 +148,9 @@ def _route(logits, mask, top_k, normalize):
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
     rows = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
     slots = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    ws = _workspace(plan, device)   # held until the call returns
     rc = lib().kudnn_moe_route_run(plan.handle, logits.data_ptr(), _at(mask), weights.data_ptr(), chosen.data_ptr(), offsets.data_ptr(),
-                                   rows.data_ptr(), slots.data_ptr(), _at(_workspace(plan, device)), _stream(device.index))
+                                   rows.data_ptr(), slots.data_ptr(), _at(ws), _stream(device.index))
     if rc:
         check(rc)
     return weights, chosen, offsets, rows, slots

@@ -74,3 +74,26 @@ def test_plans_outlive_their_calls(calls, monkeypatch):
     run_everything()
     assert {n.replace("kudnn_", "") for n in seen} == {"moe_route_run", "moe_route_backward", "grouped_linear_run", "grouped_linear_backward_input",
                                                        "grouped_linear_backward_weight", "moe_combine_run", "moe_combine_backward", "linear_fp8_run"}
+
+
+def test_workspaces_outlive_their_calls(calls, monkeypatch):
+    inside, seen = calls
+    given, had = [], set()
+    workspace_of = km._workspace
+
+    def workspace(plan, device):
+        w = workspace_of(plan, device)
+        given.append((plan.handle, None if w is None else weakref.ref(w)))
+        return w
+
+    monkeypatch.setattr(km, "_workspace", workspace)
+
+    def alive(handle):
+        for of, w in given:
+            if of is handle and w is not None:
+                had.add(seen[-1])
+                assert w() is not None, f"{seen[-1]}: its workspace went back to the allocator before it"
+
+    inside.append(alive)
+    run_everything()
+    assert {"kudnn_moe_route_run", "kudnn_grouped_linear_backward_input", "kudnn_grouped_linear_backward_weight", "kudnn_linear_fp8_run"} <= had
