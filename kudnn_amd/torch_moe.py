@@ -7,7 +7,8 @@ of rows, the 8-bit products with a scale for each block of 128, and the weighted
     out = combine(y, r.weights, r.slots)                        # back to the tokens
 
 ``route``, ``grouped_linear`` and ``combine`` are differentiable. ``linear_fp8`` and ``grouped_linear_fp8`` are the serving
-forms with e4m3 weights; they are forward only. :class:`MoEMlp` puts them together. Everything runs through the C ABI
+forms with e4m3 weights; they are forward only, and a backward pass that comes to them raises. No operator has a forward-mode
+derivative: dual tensors are refused. :class:`MoEMlp` puts them together. Everything runs through the C ABI
 (``include/kudnn_hip.h``) on torch's current stream, on the device of its arguments; nothing falls back to another path.
 
 Nothing here waits for the device: the sizes of the groups stay on it, and outputs have room for every row that the
@@ -21,6 +22,7 @@ from collections import OrderedDict
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import BF16, F16, F32, F8E4M3, U8, GroupedLinear, LinearFp8, MoeCombine, MoeRoute, check, desc, lib
 from . import quantize_blocks as _quantize_blocks
@@ -87,6 +89,31 @@ def _first_order(backward):
         return again(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
 
     return run
+
+
+def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a derivative may be taken through one of them. Dual tensors do not say so in requires_grad: while there can be any, calls go
+    through the autograd functions, which have no forward-mode derivative and refuse a tensor with a tangent."""
+    if _forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+class _ForwardOnly(torch.autograd.Function):
+    """A forward-only call: its result, and an error where a derivative through it is asked for."""
+
+    @staticmethod
+    def forward(ctx, name, call, *tensors):
+        ctx.name = name
+        return call(*tensors)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"kudnn {ctx.name} is forward only: it has no gradient")
 
 
 def _workspace(plan, device: torch.device) -> Optional[torch.Tensor]:
@@ -206,7 +233,7 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True, mask: Option
         mask = mask.contiguous()
     logits = _matrix(logits)
     normalize = bool(normalize)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _tracked(logits):
         rest = []
         return Routing(_Route.apply(logits, mask, top_k, normalize, rest), *rest)
     return Routing(*_route(logits, mask, top_k, normalize))
@@ -283,7 +310,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     _gpu("grouped_linear", x, weight, offsets, rows, slots)
     _order("grouped_linear", offsets, weight.shape[0], rows)
     xm, w = _matrix(x), _weight(weight)
-    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+    if _tracked(x, weight):
         if rows is not None and x.requires_grad and not (
                 slots is not None and slots.dtype == torch.int32 and slots.dim() == 2 and slots.shape[0] == x.shape[0]
                 and slots.numel() == rows.numel() and slots.is_contiguous()):
@@ -334,11 +361,18 @@ def _fp8_plan(x, w, dtype, bias, grouped, count, gather) -> LinearFp8:
 
 
 def _fp8(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype):
+    if _tracked(x, w, w_scale, bias, x_scale):
+        return _ForwardOnly.apply(name, lambda x, w, w_scale, bias, x_scale: _fp8_run(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype),
+                                  x, w, w_scale, bias, x_scale)
+    return _fp8_run(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype)
+
+
+def _fp8_run(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype):
     _gpu(name, x, w, w_scale, bias, offsets, rows, x_scale)
     device = x.device
     if _current() != device.index:
         with torch.cuda.device(device):
-            return _fp8(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype)
+            return _fp8_run(name, x, w, w_scale, bias, offsets, rows, x_scale, out_dtype)
     n, k = w.shape[-2:]
     blocks = ((n + 127) // 128, (k + 127) // 128)
     if w.dtype != _F8 or w_scale.dtype != torch.float32 or w_scale.shape != (*w.shape[:-2], *blocks):
@@ -467,7 +501,7 @@ def combine(y: torch.Tensor, weights: Optional[torch.Tensor], slots: torch.Tenso
         raise ValueError("kudnn combine: weights must be float32 of slots' shape")
     ym = _matrix(y)
     w = None if weights is None else weights.contiguous()
-    if (y.requires_grad or (w is not None and w.requires_grad)) and torch.is_grad_enabled():
+    if _tracked(y, w):
         return _Combine.apply(ym, w, slots)
     return _combine(ym, w, slots, y.dtype)
 
@@ -516,10 +550,15 @@ class QuantizedMoEMlp(torch.nn.Module):
                 self.register_buffer(name + "_scale", scale)
 
     def forward(self, x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if _tracked(x):
+            return _ForwardOnly.apply("QuantizedMoEMlp", lambda x: self._run(x, mask), x)
         with torch.no_grad():
-            tokens = x.reshape(-1, x.shape[-1])
-            r = route(torch.nn.functional.linear(tokens, self.router), self.top_k, self.normalize,
-                      None if mask is None else mask.reshape(-1, 1))
-            gate, up = grouped_linear_fp8(tokens, self.up, self.up_scale, r.offsets, r.rows).chunk(2, 1)
-            y = grouped_linear_fp8(torch.nn.functional.silu(gate) * up, self.down, self.down_scale, r.offsets)
-            return combine(y, r.weights, r.slots).reshape(x.shape)
+            return self._run(x, mask)
+
+    def _run(self, x, mask):
+        tokens = x.reshape(-1, x.shape[-1])
+        r = route(torch.nn.functional.linear(tokens, self.router), self.top_k, self.normalize,
+                  None if mask is None else mask.reshape(-1, 1))
+        gate, up = grouped_linear_fp8(tokens, self.up, self.up_scale, r.offsets, r.rows).chunk(2, 1)
+        y = grouped_linear_fp8(torch.nn.functional.silu(gate) * up, self.down, self.down_scale, r.offsets)
+        return combine(y, r.weights, r.slots).reshape(x.shape)
