@@ -265,7 +265,7 @@ KUDNN_HIP_API int kudnn_linear_postops_run_noalloc(kudnn_linear_postops_t plan, 
  * the largest value and makes the row's weights NaN, as the softmax does. normalize: weights are divided by the sum over
  * the chosen ones. A token with fewer than top_k open experts has expert -1, weight 0 and slot -1 in the places left.
  * Sums are in f32; the result does not depend on the order in which workgroups run. 1 <= top_k <= min(E, 32),
- * T * top_k < 2^31. */
+ * T * top_k < 2^31, T <= 2^29 - 64. */
 KUDNN_HIP_API int kudnn_moe_route_create(const kudnn_tensor_desc *logits, const kudnn_tensor_desc *mask, int top_k,
                                          int normalize, kudnn_moe_route_t *plan);
 KUDNN_HIP_API int64_t kudnn_moe_route_workspace_bytes(kudnn_moe_route_t plan);

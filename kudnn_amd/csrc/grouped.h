@@ -3,19 +3,9 @@
 #define KUDNN_GROUPED_H
 
 #include <cmath>
+#include <initializer_list>
 
 #include "moe.h"
-
-// Whether the grids of every kernel hold a product of these sizes (a grid's threads must stay below 2^32: 2^24
-// workgroups of 256); `backward`: also those of its gradients.
-inline bool kudnn_grouped_fits(int64_t R, int64_t E, int64_t N, int64_t K, bool backward)
-{
-    const int64_t most = int64_t(1) << 24;
-    const auto tiles = [](int64_t n) { return (n + 63) / 64; };
-    const int64_t rows = (R + 15) / 16 + (E + 1 < R ? E + 1 : R);
-    const auto fits = [&](int64_t a, int64_t b) { return a == 0 || b < most / a; };
-    return fits(rows, tiles(N)) && (!backward || (fits(rows, tiles(K)) && tiles(N) < most && fits(tiles(N) * tiles(K), E)));
-}
 
 // A tiled kernel of the forward product.
 struct GroupedTile {
@@ -95,6 +85,33 @@ inline GroupedTile kudnn_grouped_rule(int64_t R, int64_t groups, int64_t N, int6
         }
     }
     return best;
+}
+
+// Threads of a workgroup of the tile's kernel.
+inline int kudnn_grouped_threads(const GroupedTile &t)
+{
+    return t.kind == GroupedTile::STREAM ? t.form * 64 : (t.kind == GroupedTile::RING && t.bm == 64 ? 256 : 512);
+}
+
+// A grid's threads must stay below 2^32.
+inline bool kudnn_grid_fits(int64_t workgroups, int64_t threads) { return workgroups < (int64_t(1) << 32) / threads; }
+
+// Whether the grid of every kernel that a product of these sizes may take holds it: the rule's tiles for operands of either alignment and the
+// generic kernel's 64 x 64; `backward`: also those of its gradients.
+inline bool kudnn_grouped_fits(int64_t R, int64_t E, int64_t N, int64_t K, int dt, int c_dt, bool grouped, bool backward)
+{
+    const auto up = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
+    const auto rows = [&](int64_t bm) { return kudnn_max_row_tiles(R, E, bm, grouped); };
+    const int64_t cut = 128;      // whole 256 x 256 tiles that may be cut in two
+    if (R > 0) {
+        for (const bool any : {false, true}) {
+            const GroupedTile t = kudnn_grouped_rule(R, grouped ? (E < R ? E : R) : 1, N, K, dt, c_dt, any);
+            if (!kudnn_grid_fits(rows(t.bm) * up(N, t.bn) + (t.kind == GroupedTile::PINGPONG ? cut : 0), kudnn_grouped_threads(t))) return false;
+        }
+        if (!kudnn_grid_fits(rows(64) * up(N, 64), 256)) return false;
+    }
+    return !backward || (kudnn_grid_fits(rows(64) * up(K, 64), 256) && kudnn_grid_fits(rows(256) * up(K, 256) + cut, 512) &&
+                         kudnn_grid_fits(E * up(N, 64) * up(K, 64), 256) && kudnn_grid_fits(E * up(N, 256) * up(K, 256), 512));
 }
 
 // Whether an e4m3 product of R rows leaves the quantisation of x to the workgroups: each takes the whole of its rows (up to 48 KB

@@ -228,15 +228,6 @@ private:
     int lo_ = 0, hi_ = 0, tiles_ = 0, first_ = 0;
 };
 
-// Most row tiles that offsets of any contents in order can make: each group of rows leaves at most one part tile.
-inline int64_t max_row_tiles(int64_t R, int64_t E, int64_t bm, bool grouped)
-{
-    if (!grouped) return (R + bm - 1) / bm;
-    const int64_t groups = E + 1 < R ? E + 1 : R;
-    // n groups of which every one has a part tile: (R - n) / bm whole ones besides, at most
-    return groups + (R - groups) / bm;
-}
-
 // Four outputs of a row from column j at element `at` of C, with the bias; `wide`: a 16- or 8-byte store is aligned.
 __device__ __forceinline__ void store4(const GroupedArgs &g, int64_t at, int64_t j, float (&v)[4], bool wide)
 {

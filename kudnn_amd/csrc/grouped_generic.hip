@@ -159,7 +159,7 @@ void launch(const GroupedArgs &g, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + kT - 1) / kT;
     const int64_t tilesI = FORM == GROUPED_BWD_W ? g.E * ((g.I + kT - 1) / kT)
-                                                 : max_row_tiles(g.R, g.E, kT, g.offsets != nullptr);
+                                                 : kudnn_max_row_tiles(g.R, g.E, kT, g.offsets != nullptr);
     grouped_generic_kernel<DT, FORM><<<static_cast<unsigned>(tilesI * tilesJ), 256, 0, stream>>>(g, static_cast<int>(tilesJ));
 }
 

@@ -626,7 +626,7 @@ template <int CT, int FORM>
 void launch(const GroupedArgs &g, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + 255) / 256;
-    const int64_t tiles = FORM == GROUPED_BWD_W ? g.E * ((g.I + 255) / 256) : max_row_tiles(g.R, g.E, 256, g.offsets != nullptr);
+    const int64_t tiles = FORM == GROUPED_BWD_W ? g.E * ((g.I + 255) / 256) : kudnn_max_row_tiles(g.R, g.E, 256, g.offsets != nullptr);
     // up to a round of tiles may be cut in two
     const int64_t grid = tiles * tilesJ + (CT != KUDNN_DT_F8E4M3 && FORM != GROUPED_BWD_W ? (tiles * tilesJ < kCUs / 2 ? tiles * tilesJ : kCUs / 2) : 0);
     grouped_pingpong_kernel<CT, FORM><<<static_cast<unsigned>(grid), 512, 0, stream>>>(g, static_cast<int>(tilesJ), 4);

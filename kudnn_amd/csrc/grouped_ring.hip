@@ -290,7 +290,7 @@ template <int CT, int BM, int WM, int WN, int S, bool NATIVE>
 void launch(const GroupedArgs &g, bool hint, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + 127) / 128;
-    const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    const unsigned tiles = static_cast<unsigned>(kudnn_max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
     if (hint) {
         grouped_ring_kernel<CT, BM, WM, WN, S, true, NATIVE, false><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
     } else {
@@ -302,7 +302,7 @@ template <int CT, int BM, int WM, int WN, bool NATIVE>
 void launch_any(const GroupedArgs &g, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + 127) / 128;
-    const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    const unsigned tiles = static_cast<unsigned>(kudnn_max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
     grouped_ring_kernel<CT, BM, WM, WN, 2, false, NATIVE, true><<<tiles, WM * WN * 64, 0, stream>>>(g, static_cast<int>(tilesJ));
 }
 

@@ -303,7 +303,7 @@ template <int CT, int BM, int BN, int W, bool ANY = true, int XDT = 0>
 void launch(const GroupedArgs &g, bool hint, bool any, hipStream_t stream)
 {
     const int64_t tilesJ = (g.J + BN - 1) / BN;
-    const unsigned tiles = static_cast<unsigned>(max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
+    const unsigned tiles = static_cast<unsigned>(kudnn_max_row_tiles(g.R, g.E, BM, g.offsets != nullptr) * tilesJ);
     // the rows of a tile and their scales
     const size_t lds = XDT != 0 ? static_cast<size_t>(g.R * (kudnn_fp8_pitch(g.C) + (g.C + 127) / 128 * 4)) : 0;
     if (ANY && any) {

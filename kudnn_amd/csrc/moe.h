@@ -11,6 +11,7 @@
 
 constexpr int KUDNN_ROUTE_MAX_EXPERTS = 1024, KUDNN_ROUTE_MAX_K = 32;
 constexpr int KUDNN_ROUTE_TOKENS = 64;  // tokens of a workgroup: one bit each in an expert's 64-bit mask
+constexpr int KUDNN_ROUTE_THREADS = 512;  // of a workgroup
 
 struct RouteArgs {
     const void *logits;
@@ -85,6 +86,15 @@ struct GroupedArgs {
     int x_dt;                        // not 0: A is not quantised yet but of this 16-bit type (a_scale unused); see below
     bool a_padded, b_padded;         // the operand's rows (packed by the library) hold zeros up to a whole 16-byte chunk
 };
+
+// Most row tiles that offsets of any contents in order can make: each group of rows leaves at most one part tile.
+inline int64_t kudnn_max_row_tiles(int64_t R, int64_t E, int64_t bm, bool grouped)
+{
+    if (!grouped) return (R + bm - 1) / bm;
+    const int64_t groups = E + 1 < R ? E + 1 : R;
+    // n groups of which every one has a part tile: (R - n) / bm whole ones besides, at most
+    return groups + (R - groups) / bm;
+}
 
 // Any sizes, pitches and alignments (grouped_generic.hip).
 int kudnn_launch_grouped_generic(const GroupedArgs &g, hipStream_t stream);

@@ -197,8 +197,9 @@ int kudnn_moe_route_create(const kudnn_tensor_desc *logits, const kudnn_tensor_d
         if (top_k > KUDNN_ROUTE_MAX_K) {
             return Unsupported("router: top_k of at most 32");
         }
-        // a workgroup takes 64 tokens with 256 threads: the grid's threads must stay below 2^32
-        if (T * top_k > kMaxRows || T > (int64_t(1) << 29)) {
+        // the grid's threads must stay below 2^32 (the gradient's goes over the tokens in turns)
+        if (T > kMaxRows || T * top_k > kMaxRows ||
+            !kudnn_grid_fits((T + KUDNN_ROUTE_TOKENS - 1) / KUDNN_ROUTE_TOKENS, KUDNN_ROUTE_THREADS)) {
             return Unsupported("router: too many tokens");
         }
         auto p = new kudnn_moe_route_plan();
@@ -344,7 +345,7 @@ int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const kudnn_tensor_d
             return Bad("grouped Linear: no experts, or a width of zero");
         }
         if (R > kMaxRows || S > kMaxRows || E > kMaxExperts || K > kMaxSide || N > kMaxSide ||
-            !kudnn_grouped_fits(R, E, N, K, true)) {
+            !kudnn_grouped_fits(R, E, N, K, x->dtype, y->dtype, true, true)) {
             return Unsupported("grouped Linear: sizes beyond the grid's");
         }
         auto p = new kudnn_grouped_linear_plan();
@@ -655,7 +656,7 @@ int kudnn_linear_fp8_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc 
             }
         }
         if (R > kMaxRows || S > kMaxRows || E > kMaxExperts || K > kMaxSide || N > kMaxSide ||
-            S > (int64_t(1) << 27) / ((K + 127) / 128) || !kudnn_grouped_fits(R, E, N, K, false)) {
+            S > (int64_t(1) << 27) / ((K + 127) / 128) || !kudnn_grouped_fits(R, E, N, K, w->dtype, y->dtype, grouped != 0, false)) {
             return Unsupported("8-bit Linear: sizes beyond the grid's");
         }
         auto p = new kudnn_linear_fp8_plan();
@@ -788,9 +789,9 @@ int kudnn_moe_combine_create(const kudnn_tensor_desc *y, const kudnn_tensor_desc
         if (top_k < 1) {
             return Bad("weighted sum: top_k must be at least 1");
         }
-        // a workgroup of 256 threads a token: the grid's threads must stay below 2^32; 65535 pieces of a row
-        if (top_k > 64 || out->dims[0] > (int64_t(1) << 23) || y->dims[0] > kMaxRows || y->dims[1] > kMaxSide / 2) {
-            return Unsupported("weighted sum: at most 64 experts a token, 2^23 tokens and 2^23 columns");
+        // a grid has at most 65535 pieces of a row of 256 columns
+        if (top_k > 64 || out->dims[0] > kMaxRows || y->dims[0] > kMaxRows || y->dims[1] > kMaxSide / 2) {
+            return Unsupported("weighted sum: at most 64 experts a token, 2^31 - 1 tokens and 2^23 columns");
         }
         auto p = new kudnn_moe_combine_plan();
         p->T = out->dims[0];

@@ -158,7 +158,7 @@ __device__ __forceinline__ void clear_unnamed(const CombineArgs &a, uint32_t id,
 }
 
 // The first `1 << shift` workgroups (none with shift < 0) clear the rows that no slot names, as long as the others take; then a workgroup
-// a token. Thread partials of the k dot products meet in LDS.
+// a token (at a time). Thread partials of the k dot products meet in LDS.
 template <int DT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs a, int shift)
 {
@@ -172,40 +172,44 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineArgs 
         clear_unnamed<DT, VEC>(a, blockIdx.x, shift, named);
         return;
     }
-    const int64_t t = blockIdx.x - clearing;
-    for (int j = 0; j < a.k; ++j) {
-        const int64_t s = slot_of(a, t, j);
-        const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
-        float dot = 0.0f;
-        if (s >= 0) {
-            for (int64_t col = threadIdx.x * VEC; col < a.N; col += kThreads * VEC) {
-                float g[VEC], v[VEC];
-                load_vec<DT, VEC, false>(a.dout, t * a.N + col, g);
-                if (a.dweights != nullptr) {
-                    load_vec<DT, VEC, true>(a.y, s * a.ldy + col, v);
+    for (int64_t t = blockIdx.x - clearing; t < a.T; t += gridDim.x - clearing) {
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t s = slot_of(a, t, j);
+            const float w = a.weights == nullptr ? 1.0f : a.weights[t * a.k + j];
+            float dot = 0.0f;
+            if (s >= 0) {
+                for (int64_t col = threadIdx.x * VEC; col < a.N; col += kThreads * VEC) {
+                    float g[VEC], v[VEC];
+                    load_vec<DT, VEC, false>(a.dout, t * a.N + col, g);
+                    if (a.dweights != nullptr) {
+                        load_vec<DT, VEC, true>(a.y, s * a.ldy + col, v);
 #pragma unroll
-                    for (int q = 0; q < VEC; ++q) dot = fmaf(g[q], v[q], dot);
-                }
-                if (a.dy != nullptr) {
+                        for (int q = 0; q < VEC; ++q) dot = fmaf(g[q], v[q], dot);
+                    }
+                    if (a.dy != nullptr) {
 #pragma unroll
-                    for (int q = 0; q < VEC; ++q) v[q] = w * g[q];
-                    store_vec<DT, VEC>(a.dy, s * a.N + col, v);
+                        for (int q = 0; q < VEC; ++q) v[q] = w * g[q];
+                        store_vec<DT, VEC>(a.dy, s * a.N + col, v);
+                    }
                 }
             }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+            if (lane == 0) part[j][wave] = dot;
         }
+        if (a.dweights == nullptr) continue;
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < a.k) {
+            float dot = 0.0f;
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
-        if (lane == 0) part[j][wave] = dot;
-    }
-    if (a.dweights == nullptr) return;
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < a.k) {
-        float dot = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) dot += part[threadIdx.x][w];
-        a.dweights[t * a.k + threadIdx.x] = dot;
+            for (int w = 0; w < kWaves; ++w) dot += part[threadIdx.x][w];
+            a.dweights[t * a.k + threadIdx.x] = dot;
+        }
+        __syncthreads();   // before the next token's parts
     }
 }
+
+constexpr int64_t kMostTokens = int64_t(1) << 23;   // of a grid, half of what its 2^32 threads allow; more in turns
 
 template <int DT, int ODT>
 int launch(const CombineArgs &a, bool wide, hipStream_t stream)
@@ -213,7 +217,7 @@ int launch(const CombineArgs &a, bool wide, hipStream_t stream)
     const int64_t each = wide ? vec_of<ODT, true>() : 1, waves = (a.N + 64 * each - 1) / (64 * each);
     const unsigned threads = waves < kThreads / 64 ? static_cast<unsigned>(waves) * 64 : kThreads;   // none that has no columns
     const int64_t piece = threads * each, pieces = (a.N + piece - 1) / piece;
-    const dim3 grid(static_cast<unsigned>(a.T), static_cast<unsigned>(pieces));
+    const dim3 grid(static_cast<unsigned>(a.T < kMostTokens ? a.T : kMostTokens), static_cast<unsigned>(pieces));
     if (wide) {
         combine_kernel<DT, ODT, true><<<grid, threads, 0, stream>>>(a);
     } else {
@@ -228,7 +232,7 @@ int launch_backward(const CombineArgs &a, bool wide, hipStream_t stream)
     // clearing workgroups: a power of two, up to 256, of 64 rows each or more where there are that few
     int shift = a.dy != nullptr && a.R > 0 && a.N > 0 ? 0 : -1;
     while (shift >= 0 && shift < 8 && (int64_t(64) << shift) < a.R) ++shift;
-    const unsigned grid = static_cast<unsigned>(a.T + (shift < 0 ? 0 : 1 << shift));
+    const unsigned grid = static_cast<unsigned>((a.T < kMostTokens ? a.T : kMostTokens) + (shift < 0 ? 0 : 1 << shift));
     if (grid == 0) {
         return 0;
     }

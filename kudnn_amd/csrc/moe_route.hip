@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kTokens = KUDNN_ROUTE_TOKENS;
 // 8 lanes a token for all 64 tokens at once: with 256 threads, two after the other, 16384 x 128 took 15.6 us instead of 10.6
-constexpr int kThreads = 512;
+constexpr int kThreads = KUDNN_ROUTE_THREADS;
 constexpr int kEach = KUDNN_ROUTE_MAX_EXPERTS / kThreads;   // experts of a thread in the scan over them
 constexpr int kClosed = INT32_MIN;
 
@@ -344,11 +344,9 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int 
 // Gradient of the logits. L lanes a token as in the forward pass; the whole softmax p is formed again where it counts.
 //   normalize: dx_e = w_e (d_e - sum d w) for the chosen, else 0.  Otherwise: dx_e = p_e (d_e - sum d p), d_e = 0 unless chosen.
 template <int L, int V>
-__global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteBackwardArgs a)
+__device__ __forceinline__ void route_backward_token(const RouteBackwardArgs &a, int64_t tok)
 {
-    const int64_t tok = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;
     const int sub = threadIdx.x % L;
-    if (tok >= a.T) return;   // a token's lanes leave together: the shuffles below stay within L lanes
     float d[V], p[V];
     float dot = 0.0f;
 #pragma unroll
@@ -414,6 +412,16 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteBackwardA
     }
 }
 
+template <int L, int V>
+__global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteBackwardArgs a)
+{
+    // a token's lanes leave together: the shuffles stay within L lanes
+    for (int64_t tok = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L; tok < a.T;
+         tok += static_cast<int64_t>(gridDim.x) * (kThreads / L)) {
+        route_backward_token<L, V>(a, tok);
+    }
+}
+
 // Whether a row's logits and mask bytes can be read 4 values at a time.
 bool wide_rows(const void *logits, int dt, int64_t ld, const uint8_t *mask, int64_t mask_st, int64_t mask_se)
 {
@@ -459,8 +467,10 @@ int kudnn_launch_moe_route_backward(const RouteBackwardArgs &args, hipStream_t s
     a.wide_out = a.E % 4 == 0 && reinterpret_cast<uintptr_t>(a.dlogits) % 16 == 0;
     with_shape(a.E, [&](auto l, auto v) {
         constexpr int perBlock = kThreads / decltype(l)::value;
+        constexpr int64_t most = int64_t(1) << 22;    // half of what a grid's 2^32 threads allow; more tokens in turns
+        const int64_t blocks = (a.T + perBlock - 1) / perBlock;
         route_backward_kernel<decltype(l)::value, decltype(v)::value>
-            <<<static_cast<unsigned>((a.T + perBlock - 1) / perBlock), kThreads, 0, stream>>>(a);
+            <<<static_cast<unsigned>(blocks < most ? blocks : most), kThreads, 0, stream>>>(a);
         return 0;
     });
     return hipGetLastError() == hipSuccess ? 0 : -1;

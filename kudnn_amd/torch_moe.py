@@ -313,8 +313,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     if _tracked(x, weight):
         if rows is not None and x.requires_grad and not (
                 slots is not None and slots.dtype == torch.int32 and slots.dim() == 2 and slots.shape[0] == x.shape[0]
-                and slots.numel() == rows.numel() and slots.is_contiguous()):
-            raise ValueError("kudnn grouped_linear: the gradient of gathered rows needs slots, int32 [T, k]")
+                and slots.numel() == rows.numel() and slots.is_contiguous() and slots.shape[1] <= 64):
+            raise ValueError("kudnn grouped_linear: the gradient of gathered rows needs slots, int32 [T, k], k up to 64")
         return _GroupedLinear.apply(xm, w, offsets, rows, slots)
     return _grouped(xm, w, offsets, rows)
 

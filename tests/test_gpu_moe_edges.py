@@ -99,3 +99,39 @@ def test_combine_after_choices_are_dropped():
     keep = slots >= 0
     want[slots[keep].long()] = (r.weights.double()[:, :, None] * dout.double()[:, None, :])[keep]
     near(dy, want, want.abs(), 1, "dy")
+
+
+@pytest.mark.parametrize("tokens", [(1 << 23) + 101])
+def test_weighted_sum_of_more_tokens_than_a_grid(tokens):
+    g = gen(3)
+    y = randn(g, 1000, 8).bfloat16()
+    slots = torch.full((tokens, 1), -1, dtype=torch.int32, device=DEV)
+    last = torch.arange(tokens - 900, tokens, device=DEV)
+    slots[last, 0] = torch.randperm(1000, generator=g, device=DEV)[:900].int()
+    out = km.combine(y, None, slots)
+    assert torch.equal(out[last], y[slots[last, 0].long()]) and float(out[:-900].abs().sum()) == 0.0
+    dout = randn(g, tokens, 8).bfloat16()
+    dy, dw = torch.full_like(y, math.nan), torch.full((tokens, 1), math.nan, device=DEV)
+    K.MoeCombine(K.desc([1000, 8], K.BF16), K.desc([tokens, 8], K.BF16), 1).backward(y, None, slots, dout, dy, dw, torch.cuda.current_stream())
+    want = torch.zeros_like(y)
+    want[slots[last, 0].long()] = dout[last]
+    assert torch.equal(dy, want) and float(dw[:-900].abs().sum()) == 0.0
+    products = dout[last].double() * y[slots[last, 0].long()].double()
+    near(dw[last, 0], products.sum(1), products.abs().sum(1), 8, "dweights")
+
+
+def test_router_gradient_of_more_tokens_than_a_grid():
+    tokens = (1 << 28) + 77
+    g = gen(4)
+    logits = torch.zeros(tokens, 2, dtype=torch.float16, device=DEV)
+    ends = torch.cat([torch.arange(500, device=DEV), torch.arange(tokens - 500, tokens, device=DEV)])
+    logits[ends] = randn(g, 1000, 2).half()
+    experts = torch.zeros(tokens, 1, dtype=torch.int32, device=DEV)
+    p = torch.softmax(logits[ends].double(), 1)
+    weights, d = torch.full((tokens, 1), 0.5, device=DEV), torch.ones(tokens, 1, device=DEV)
+    weights[ends, 0], d[ends, 0] = p[:, 0].float(), randn(g, 1000)
+    dlogits = torch.full_like(logits, math.nan)
+    K.MoeRoute(K.desc([tokens, 2], K.F16), 1, False).backward(logits, None, weights, experts, d, dlogits, torch.cuda.current_stream())
+    assert bool((dlogits[500:-500] == torch.tensor([0.25, -0.25], device=DEV).half()).all())
+    dx = d[ends].double() * p[:, :1] * torch.stack([1 - p[:, 0], -p[:, 1]], 1)
+    near(dlogits[ends], dx, 2.0 ** 7 * d[ends].double().abs(), 1, "dlogits")
