@@ -12,6 +12,8 @@
 constexpr int KUDNN_ROUTE_MAX_EXPERTS = 1024, KUDNN_ROUTE_MAX_K = 32;
 constexpr int KUDNN_ROUTE_TOKENS = 64;  // tokens of a workgroup: one bit each in an expert's 64-bit mask
 constexpr int KUDNN_ROUTE_THREADS = 512;  // of a workgroup
+// Calls of more workgroups sum the counts of each run of KUDNN_ROUTE_RUN and scan the sums in launches of their own (moe_route.hip).
+constexpr int64_t KUDNN_ROUTE_DIRECT = 768, KUDNN_ROUTE_RUN = 128;
 
 struct RouteArgs {
     const void *logits;
@@ -22,6 +24,7 @@ struct RouteArgs {
     int32_t *experts, *offsets, *rows, *slots;
     uint8_t *counts;              // [workgroups][counts_ld]: a workgroup's rows of each expert; unused with one workgroup
     int counts_ld;
+    int32_t *sums;                // more than KUDNN_ROUTE_DIRECT workgroups: [1 + runs][counts_ld], all rows of each expert, then those before a run
     bool wide;                    // set by the launcher: rows can be read 4 values at a time
 };
 int kudnn_launch_moe_route(const RouteArgs &a, hipStream_t stream);

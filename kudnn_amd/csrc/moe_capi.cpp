@@ -16,7 +16,7 @@ using kudnn_host::DeviceMemory;
 
 struct kudnn_moe_route_plan : PlanBase {
     kudnn_moe_route_plan() : PlanBase(PLAN_MOE_ROUTE) {}
-    int64_t T = 0, ld = 0, maskSt = 0, maskSe = 0, workspace = 0;
+    int64_t T = 0, ld = 0, maskSt = 0, maskSe = 0, sumsAt = 0, workspace = 0;
     int E = 0, k = 0, dt = 0, normalize = 0, countsLd = 0;
     bool masked = false;
 };
@@ -221,9 +221,11 @@ int kudnn_moe_route_create(const kudnn_tensor_desc *logits, const kudnn_tensor_d
         p->normalize = normalize != 0 ? 1 : 0;
         p->countsLd = static_cast<int>((E + 3) / 4 * 4);
         const int64_t blocks = (T + KUDNN_ROUTE_TOKENS - 1) / KUDNN_ROUTE_TOKENS;
-        p->workspace = blocks > 1 ? blocks * p->countsLd : 0;
+        const int64_t runs = blocks > KUDNN_ROUTE_DIRECT ? (blocks + KUDNN_ROUTE_RUN - 1) / KUDNN_ROUTE_RUN : 0;
+        p->sumsAt = blocks * p->countsLd;
+        p->workspace = blocks > 1 ? p->sumsAt + (runs > 0 ? (runs + 1) * p->countsLd * static_cast<int64_t>(sizeof(int32_t)) : 0) : 0;
         p->desc = "moe_route T=" + std::to_string(T) + " E=" + std::to_string(E) + " k=" + std::to_string(top_k) +
-                  (p->workspace > 0 ? " launches=2" : " launches=1");
+                  (runs > 0 ? " launches=4" : (p->workspace > 0 ? " launches=2" : " launches=1"));
         *plan = p;
         return KUDNN_STATUS_SUCCESS;
     });
@@ -270,6 +272,7 @@ int kudnn_moe_route_run(kudnn_moe_route_t plan, const void *logits, const void *
     a.slots = slots;
     a.counts = static_cast<uint8_t *>(workspace);
     a.counts_ld = plan->countsLd;
+    a.sums = reinterpret_cast<int32_t *>(a.counts + plan->sumsAt);
     return Launched(kudnn_launch_moe_route(a, static_cast<hipStream_t>(stream)), "router: launch failed");
 }
 

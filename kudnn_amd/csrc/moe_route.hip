@@ -11,7 +11,9 @@
 // expert has a 64-bit mask of the workgroup's tokens (set by atomic OR, which commutes), and the place is a population
 // count. A second launch adds the counts of the earlier workgroups (bytes, at most 64 each) and of all experts before;
 // a call of at most 64 tokens is one launch. The counts are read by every workgroup again (T / 64 x E bytes from L2), which
-// at 16384 tokens and 128 experts costs less than a third launch that would scan them.
+// at 16384 tokens and 128 experts costs less than launches that would sum and scan them (16.0 against 21.0 us a call). That grows as the square of T,
+// so above 768 workgroups a launch sums each run of 128 of them, another scans those sums, and the last one reads its own run's counts
+// only: 65536 tokens 40.5 us against 45.5, 262144 tokens 117 against 270, 2^20 tokens 433 against 3009 (32768 tokens: 26.2 against 23.1).
 #include <type_traits>
 
 #include "device_common.h"
@@ -283,7 +285,77 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a, int single
     place(a, sh, t0, n, sh.expert);
 }
 
-// Adds the counts of the workgroups: thread (column c, slice s) sums 4 experts' bytes over every S-th workgroup.
+// Adds the counts of workgroups b0 up to b1 of the whole launch into total[], and those of them before workgroup `own` into before[] (both in
+// LDS, cleared): thread (column c, slice s) sums 4 experts' bytes over every S-th workgroup.
+template <bool BEFORE>
+__device__ __forceinline__ void add_counts(const RouteArgs &a, int b0, int b1, int own, int *total, int *before)
+{
+    const int words = a.counts_ld / 4;             // at most 256
+    const int S = kThreads / words, c = threadIdx.x % words, s = threadIdx.x / words;
+    if (s >= S) return;
+    // pairs of 16-bit sums: experts 0 and 2, 1 and 3 of the four
+    static_assert(KUDNN_ROUTE_DIRECT * kTokens < 65536 && KUDNN_ROUTE_RUN <= KUDNN_ROUTE_DIRECT, "a sum of 16 bits holds the workgroups' rows");
+    const uint32_t *p = reinterpret_cast<const uint32_t *>(a.counts) + c;
+    uint32_t all[2] = {0u, 0u}, bef[2] = {0u, 0u};
+#pragma unroll 8
+    for (int b = b0 + s; b < b1; b += S) {
+        const uint32_t w = p[static_cast<int64_t>(b) * words];
+        const uint32_t lo = w & 0x00ff00ffu, hi = (w >> 8) & 0x00ff00ffu;
+        all[0] += lo;
+        all[1] += hi;
+        if constexpr (BEFORE) {
+            const bool early = b < own;
+            bef[0] += early ? lo : 0u;
+            bef[1] += early ? hi : 0u;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        atomicAdd(&total[c * 4 + i], static_cast<int>((all[i & 1] >> (16 * (i >> 1))) & 0xffffu));   // integers: in any order
+        if constexpr (BEFORE) atomicAdd(&before[c * 4 + i], static_cast<int>((bef[i & 1] >> (16 * (i >> 1))) & 0xffffu));
+    }
+}
+
+// Many workgroups: the rows of each run of them into sums[1 + run].
+__global__ __launch_bounds__(kThreads) void route_sum_kernel(RouteArgs a, int blocks)
+{
+    __shared__ int total[KUDNN_ROUTE_MAX_EXPERTS];
+    for (int e = threadIdx.x; e < a.counts_ld; e += kThreads) total[e] = 0;
+    __syncthreads();
+    const int b0 = static_cast<int>(blockIdx.x * KUDNN_ROUTE_RUN), b1 = b0 + static_cast<int>(KUDNN_ROUTE_RUN);
+    add_counts<false>(a, b0, b1 < blocks ? b1 : blocks, 0, total, nullptr);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.counts_ld; e += kThreads) a.sums[(blockIdx.x + int64_t(1)) * a.counts_ld + e] = total[e];
+}
+
+// A lane an expert: sums[1 + run] becomes the rows of the runs before, sums[0] those of all.
+__global__ __launch_bounds__(64) void route_scan_kernel(RouteArgs a, int64_t runs)
+{
+    const int e = static_cast<int>(blockIdx.x * 64 + threadIdx.x);
+    if (e >= a.counts_ld) return;
+    int32_t *at = a.sums + a.counts_ld + e;
+    int before = 0;
+    int64_t run = 0;
+    for (; run + 16 <= runs; run += 16, at += 16 * a.counts_ld) {
+        int v[16];                                   // on their way together
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = at[i * a.counts_ld];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            at[i * a.counts_ld] = before;
+            before += v[i];
+        }
+    }
+    for (; run < runs; ++run, at += a.counts_ld) {
+        const int v = *at;
+        *at = before;
+        before += v;
+    }
+    a.sums[e] = before;
+}
+
+// Places the rows. SUMS: from the scanned sums of the runs and the counts of this run's workgroups, else from the counts of all workgroups.
+template <bool SUMS>
 __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int blocks)
 {
     __shared__ Shared sh;
@@ -294,36 +366,21 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a, int 
         sh.mask[e] = 0ull;
         before[e] = 0;
         total[e] = 0;
+        if (SUMS && e < a.counts_ld) {
+            before[e] = a.sums[(blockIdx.x / KUDNN_ROUTE_RUN + 1) * a.counts_ld + e];
+            total[e] = a.sums[e];
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n * a.k; i += kThreads) {
         const int e = a.experts[t0 * a.k + i];
         if (e >= 0) atomicOr(&sh.mask[e], 1ull << (i / a.k));
     }
-    const int words = a.counts_ld / 4;             // at most 256
-    const int S = kThreads / words, c = threadIdx.x % words, s = threadIdx.x / words;
-    if (s < S) {
-        // pairs of 16-bit sums: experts 0 and 2, 1 and 3 of the four (at most 64 x 1023 each; more workgroups in several goes)
-        const uint32_t *p = reinterpret_cast<const uint32_t *>(a.counts) + c;
-        for (int b0 = 0; b0 < blocks; b0 += 1023) {
-            uint32_t all[2] = {0u, 0u}, bef[2] = {0u, 0u};
-            const int b1 = b0 + 1023 < blocks ? b0 + 1023 : blocks;
-#pragma unroll 8
-            for (int b = b0 + s; b < b1; b += S) {
-                const uint32_t w = p[static_cast<int64_t>(b) * words];
-                const uint32_t lo = w & 0x00ff00ffu, hi = (w >> 8) & 0x00ff00ffu;
-                const bool early = b < static_cast<int>(blockIdx.x);
-                all[0] += lo;
-                all[1] += hi;
-                bef[0] += early ? lo : 0u;
-                bef[1] += early ? hi : 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                atomicAdd(&total[c * 4 + i], static_cast<int>((all[i & 1] >> (16 * (i >> 1))) & 0xffffu));   // integers: in any order
-                atomicAdd(&before[c * 4 + i], static_cast<int>((bef[i & 1] >> (16 * (i >> 1))) & 0xffffu));
-            }
-        }
+    const int own = static_cast<int>(blockIdx.x);
+    if constexpr (SUMS) {
+        add_counts<false>(a, own / static_cast<int>(KUDNN_ROUTE_RUN) * static_cast<int>(KUDNN_ROUTE_RUN), own, 0, before, nullptr);
+    } else {
+        add_counts<true>(a, 0, blocks, own, total, before);
     }
     __syncthreads();
     int v[kEach];
@@ -454,8 +511,13 @@ int kudnn_launch_moe_route(const RouteArgs &args, hipStream_t stream)
         route_kernel<decltype(l)::value, decltype(v)::value><<<blocks, kThreads, 0, stream>>>(a, single);
         return 0;
     });
-    if (!single) {
-        route_place_kernel<<<blocks, kThreads, 0, stream>>>(a, blocks);
+    if (blocks > KUDNN_ROUTE_DIRECT) {
+        const int64_t runs = (blocks + KUDNN_ROUTE_RUN - 1) / KUDNN_ROUTE_RUN;
+        route_sum_kernel<<<static_cast<unsigned>(runs), kThreads, 0, stream>>>(a, blocks);
+        route_scan_kernel<<<(a.counts_ld + 63) / 64, 64, 0, stream>>>(a, runs);
+        route_place_kernel<true><<<blocks, kThreads, 0, stream>>>(a, blocks);
+    } else if (!single) {
+        route_place_kernel<false><<<blocks, kThreads, 0, stream>>>(a, blocks);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

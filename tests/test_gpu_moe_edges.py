@@ -135,3 +135,24 @@ def test_router_gradient_of_more_tokens_than_a_grid():
     assert bool((dlogits[500:-500] == torch.tensor([0.25, -0.25], device=DEV).half()).all())
     dx = d[ends].double() * p[:, :1] * torch.stack([1 - p[:, 0], -p[:, 1]], 1)
     near(dlogits[ends], dx, 2.0 ** 7 * d[ends].double().abs(), 1, "dlogits")
+
+
+@pytest.mark.parametrize("tokens,experts,k", [(65, 60, 4), (768 * 64, 9, 3), (768 * 64 + 1, 9, 3), (70001, 130, 2), (140007, 1024, 1), (1 << 20, 8, 2)])
+def test_order_of_many_tokens(tokens, experts, k):
+    """The order by expert against a stable sort, around and far above the count of workgroups from which their counts are scanned."""
+    g = gen(experts)
+    logits = randn(g, tokens, experts) + 2 * randn(g, 1, experts)
+    mask = torch.rand(tokens, 1, generator=g, device=DEV) > 0.1
+    r = km.route(logits, k, True, mask)
+    top = torch.sort(logits, dim=1, descending=True, stable=True)
+    assert torch.equal(r.experts, torch.where(mask, top.indices[:, :k], -1).int())
+    key = torch.where(r.experts < 0, experts, r.experts).reshape(-1)
+    order = torch.sort(key, stable=True).indices
+    assert torch.equal(r.offsets, torch.searchsorted(key[order], torch.arange(experts + 1, device=DEV, dtype=torch.int32)).int())
+    count = int(r.offsets[-1])
+    assert torch.equal(r.rows, torch.where(torch.arange(tokens * k, device=DEV) < count, order // k, -1).int())
+    slots = torch.full((tokens * k,), -1, dtype=torch.int32, device=DEV)
+    slots[order[:count]] = torch.arange(count, dtype=torch.int32, device=DEV)
+    assert torch.equal(r.slots.reshape(-1), slots)
+    want = torch.softmax(top.values[:, :k].double(), 1) * mask
+    torch.testing.assert_close(r.weights.double(), want, rtol=2.0 ** -16, atol=1e-30)

@@ -23,6 +23,14 @@ def test_router_tokens():
     assert not accepted(lambda: K.MoeRoute(d(1 << 60, 8), 8))
 
 
+def test_router_launches():
+    """The counts of many workgroups are summed in launches of their own, so that a call's work grows as its tokens."""
+    d = lambda t: K.desc([t, 9], K.F32)
+    few, many = K.MoeRoute(d(768 * 64), 3), K.MoeRoute(d(768 * 64 + 1), 3)
+    assert "launches=2" in few.describe() and few.workspace_bytes == 768 * 12
+    assert "launches=4" in many.describe() and many.workspace_bytes == 769 * 12 + (7 + 1) * 12 * 4
+
+
 def test_weighted_sum_tokens():
     d = lambda t: K.desc([t, 8], K.F32)
     assert accepted(lambda: K.MoeCombine(d(1 << 24), d((1 << 31) - 1), 64)) and not accepted(lambda: K.MoeCombine(d(1 << 24), d(1 << 31), 2))
