@@ -156,3 +156,20 @@ def test_order_of_many_tokens(tokens, experts, k):
     assert torch.equal(r.slots.reshape(-1), slots)
     want = torch.softmax(top.values[:, :k].double(), 1) * mask
     torch.testing.assert_close(r.weights.double(), want, rtol=2.0 ** -16, atol=1e-30)
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("tokens,width,experts,pad", [(1, 256, 8, 0), (7, 40, 5, 3), (130, 33, 9, 0), (3001, 1024, 60, 0), (600, 264, 128, 8)])
+def test_router_projection(tokens, width, experts, pad, dtype):
+    g = gen(tokens + width)
+    wide = randn(g, tokens, width + pad).to(HALF[dtype])
+    x = wide[:, pad:].detach().requires_grad_(True)
+    w = (randn(g, experts, width) * width ** -0.5).to(HALF[dtype]).requires_grad_(True)
+    y = km._project(x, w)
+    xd, wd, dy = x.detach().double(), w.detach().double(), randn(g, tokens, experts).to(HALF[dtype])
+    near(y.detach(), xd @ wd.t(), xd.abs() @ wd.abs().t(), width + 1, "logits")
+    assert torch.equal(km._project(x.detach(), w.detach()), y.detach())
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    d = dy.double()
+    near(dx, d @ wd, d.abs() @ wd.abs(), experts + 1, "dx")
+    near(dw, d.t() @ xd, d.abs().t() @ xd.abs(), tokens + 1, "dw")

@@ -55,3 +55,27 @@ def test_8_bit_layer_refuses_a_gradient(calls, monkeypatch):  # noqa: F811
     with torch.no_grad():
         assert not layer(x).requires_grad
     assert not layer(x.detach()).requires_grad
+
+
+@pytest.mark.parametrize("tokens", [3, 0])
+def test_layers_make_no_library_products(calls, monkeypatch, tokens):  # noqa: F811
+    """The router's logits and their gradients come from the framework's own products."""
+    def library(*a, **kw):
+        raise AssertionError("a library product")
+
+    for name in ("linear", "bilinear"):
+        monkeypatch.setattr(torch.nn.functional, name, library)
+    for name in ("matmul", "mm", "bmm", "addmm", "einsum"):
+        monkeypatch.setattr(torch, name, library)
+        if hasattr(torch.Tensor, name):
+            monkeypatch.setattr(torch.Tensor, name, library)
+    monkeypatch.setattr(torch.Tensor, "__matmul__", library)
+    monkeypatch.setattr(km, "quantize_blocks", lambda w: (w.to(F8), torch.ones(w.shape[0], 1, 1)))
+    _, seen = calls
+    layer = km.MoEMlp(8, 16, 4, 2)
+    x = torch.randn(tokens, 8).bfloat16().requires_grad_(True)
+    layer(x).float().sum().backward()
+    assert layer.router.grad.shape == (4, 8) and x.grad.shape == (tokens, 8)
+    assert seen.count("kudnn_grouped_linear_run") == 3 and seen.count("kudnn_gemm_run") == (tokens > 0)
+    with torch.no_grad():
+        layer(x), layer.quantized()(x)
