@@ -254,7 +254,8 @@ KUDNN_HIP_API int kudnn_linear_postops_run_noalloc(kudnn_linear_postops_t plan, 
  *
  * The order by expert. A batch of T tokens with k experts each makes up to R = T * k rows. Sorted by expert, and within an
  * expert by token, they are described by
- *   offsets s32[E + 1]  expert e has the rows offsets[e] .. offsets[e + 1] - 1 (offsets[0] = 0);
+ *   offsets s32[E + 1]  expert e has the rows offsets[e] .. offsets[e + 1] - 1. The router's begin at 0; a product takes any part of them
+ *                       (a rank's experts), and the rows before its first expert's are rows of no expert, as those past the last;
  *   rows    s32[R]      the token of each row, -1 past offsets[E];
  *   slots   s32[T * k]  the row of each of a token's experts, -1 where it has none.
  * Values outside their range are read as "none": no call reads or writes outside its buffers for any contents. */
@@ -283,7 +284,7 @@ KUDNN_HIP_API int kudnn_moe_route_destroy(kudnn_moe_route_t plan);
 
 /* Grouped Linear: y[r] = x[r] x w[e] for the rows r of expert e. x {S, K} AB, w {E, K, N} ACB (each expert's weight
  * physically [N][K], as nn.Linear holds it), y {R, N} AB; one type, bf16 or f16; f32 accumulation, one rounding. gather != 0:
- * row r takes x[rows[r]], else S == R and it takes x[r]. Rows past offsets[E] are
+ * row r takes x[rows[r]], else S == R and it takes x[r]. Rows of no expert are
  * zero; a row whose token is out of range is taken as zeros. R < 2^31. */
 KUDNN_HIP_API int kudnn_grouped_linear_create(const kudnn_tensor_desc *x, const kudnn_tensor_desc *w,
                                               const kudnn_tensor_desc *y, int gather, kudnn_grouped_linear_t *plan);

@@ -49,7 +49,7 @@ private:
     std::unique_ptr<Detail::MoeRouteImpl> pImpl;
 };
 
-// y[r] = x[rows[r]] x w[e] for the rows r of expert e (x[r] without gather); zero past the last.
+// y[r] = x[rows[r]] x w[e] for the rows r of expert e (x[r] without gather); zero for rows of no expert.
 class KUDNN_API_PUBLIC GroupedLinear final {
 public:
     // x {S, K} AB, w {E, K, N} ACB, y {R, N} AB, all BF16 or all F16.

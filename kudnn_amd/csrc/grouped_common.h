@@ -127,7 +127,7 @@ __device__ __forceinline__ f32x4_t mfma(const u32x4_t &a, const u32x4_t &b, cons
 }
 
 
-// A tile of rows of one expert. e == E: the rows that belong to no expert (past offsets[E]).
+// A tile of rows of one expert. e == E: the rows that belong to no expert (before offsets[0], and past offsets[E]).
 struct RowTile {
     int e, begin, end;   // the expert's rows
     int r0;              // first row of the tile
@@ -148,10 +148,13 @@ public:
             halves_ = half(R) ? 1 : 0;
             return;
         }
-        for (int base = 0; base < E; base += 64) experts_ = scan(base, experts_);
+        for (int base = 0; base < E; base += 64) {
+            experts_ = scan(base, experts_);
+            if (base == 0) lead_ = __builtin_amdgcn_readfirstlane(lo_);    // the first expert's begin
+        }
         experts_ = __builtin_amdgcn_readfirstlane(experts_);
         rest_ = __builtin_amdgcn_readlane(hi_, (E - 1) & 63);    // the last expert's end
-        total_ = experts_ + (R - rest_ + bm - 1) / bm;
+        total_ = experts_ + (lead_ + bm - 1) / bm + (R - rest_ + bm - 1) / bm;
     }
     __device__ __forceinline__ int total() const { return total_; }
     __device__ __forceinline__ int halves() const { return halves_; }
@@ -180,9 +183,16 @@ public:
     // Tile number `want` < total(). Its members are the same in every lane.
     __device__ __forceinline__ RowTile find(int want)
     {
-        RowTile t{E_, rest_, R_, rest_ + (want - experts_) * bm_};
         if (offsets_ == nullptr) {
             return RowTile{0, 0, R_, want * bm_};
+        }
+        // behind the experts' tiles those of the rows before them, then those past them
+        const int none = want - experts_, lead = (lead_ + bm_ - 1) / bm_;
+        RowTile t{E_, rest_, R_, rest_ + (none - lead) * bm_};
+        if (none < lead) {
+            t.begin = 0;
+            t.end = lead_;
+            t.r0 = none * bm_;
         }
         int before = 0;
         for (int base = 0; base < E_ && want < experts_; base += 64) {
@@ -224,7 +234,7 @@ private:
         return before + __shfl(incl, 63);
     }
     const int32_t *offsets_;
-    int E_, R_, bm_, total_ = 0, experts_ = 0, rest_ = 0, halves_ = 0;
+    int E_, R_, bm_, total_ = 0, experts_ = 0, lead_ = 0, rest_ = 0, halves_ = 0;
     int lo_ = 0, hi_ = 0, tiles_ = 0, first_ = 0;
 };
 

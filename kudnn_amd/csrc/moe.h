@@ -94,7 +94,7 @@ struct GroupedArgs {
 inline int64_t kudnn_max_row_tiles(int64_t R, int64_t E, int64_t bm, bool grouped)
 {
     if (!grouped) return (R + bm - 1) / bm;
-    const int64_t groups = E + 1 < R ? E + 1 : R;
+    const int64_t groups = E + 2 < R ? E + 2 : R;   // with the rows before the experts' and those past them
     // n groups of which every one has a part tile: (R - n) / bm whole ones besides, at most
     return groups + (R - groups) / bm;
 }

@@ -299,7 +299,8 @@ class _GroupedLinear(torch.autograd.Function):
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
                    slots: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y[r] = x[rows[r]] @ weight[e].T (x[r] without rows) for the rows offsets[e] <= r < offsets[e + 1]; zero past the last.
+    """y[r] = x[rows[r]] @ weight[e].T (x[r] without rows) for the rows offsets[e] <= r < offsets[e + 1]; zero before the first and past
+    the last (offsets[i:j + 1] with weight[i:j] are the products of some of the experts).
 
     x: [T, K] with rows, [R, K] without, bfloat16 or float16; weight: [E, N, K], an nn.Linear weight for each expert, of x's type;
     offsets, rows, slots as ``route`` gives them. Differentiable in x and weight; with rows, the gradient of x is a sum over

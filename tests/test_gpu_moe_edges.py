@@ -173,3 +173,64 @@ def test_router_projection(tokens, width, experts, pad, dtype):
     d = dy.double()
     near(dx, d @ wd, d.abs() @ wd.abs(), experts + 1, "dx")
     near(dw, d.t() @ xd, d.abs().t() @ xd.abs(), tokens + 1, "dw")
+
+
+def part_of_the_experts(counts, skip, width, out, dtype, f8=False, gather=True):
+    """Products and gradients of the experts from `skip` on, over NaN: equal to the whole's in their rows, zero in the others."""
+    g = gen(width + out + skip)
+    offsets, rows = make_order(counts, 3, 50, g)
+    count, first = sum(counts) + 3, sum(counts[:skip])
+    part, e = offsets[skip:], len(counts) - skip
+    kind = K.BF16 if dtype == torch.bfloat16 else K.F16
+    x = randn(g, 50 if gather else count, width).to(dtype)
+    stream = torch.cuda.current_stream()
+    r = rows if gather else None
+    y = torch.full((count, out), math.nan, dtype=dtype, device=DEV)
+    if f8:
+        w, ws = make_fp8(g, len(counts), out, width)
+        plan = K.LinearFp8(K.desc(x.shape, kind), K.desc([e, width, out], K.F8E4M3, "ACB"), K.desc(y.shape, kind), None, True, gather)
+        room = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=DEV)
+        plan.run(x, None, w[skip:], ws[skip:].contiguous(), y, None, part, r, room, stream)
+        want = km.grouped_linear_fp8(x, w, ws, offsets, r).double()
+        assert float(y[:first].abs().sum()) == 0.0 and float(y[sum(counts):].abs().sum()) == 0.0
+        near(y[first:], want[first:], want[first:].abs(), width + 3 * (width // 128 + 1) + 2.0 ** 13, "y")
+        return plan.describe()
+    w = (randn(g, len(counts), out, width) * width ** -0.5).to(dtype)
+    dy = randn(g, count, out).to(dtype)
+    plan = K.GroupedLinear(K.desc(x.shape, kind), K.desc([e, width, out], kind, "ACB"), K.desc(y.shape, kind), gather)
+    room = torch.full((plan.workspace_bytes,), 255, dtype=torch.uint8, device=DEV)
+    dx, dw = torch.full((count, width), math.nan, dtype=dtype, device=DEV), torch.full((e, out, width), math.nan, dtype=dtype, device=DEV)
+    plan.run(x, w[skip:], part, r, y, stream)
+    plan.backward_input(dy, w[skip:], part, dx, stream, room)
+    plan.backward_weight(dy, x, part, r, dw, stream, room)
+    want, my, dxs, mx, dws, mw = grouped_plain(x, w[skip:], part, r, count, dy)
+    near(y, want, my, width + 1, "y")
+    near(dx, dxs, mx, out + 1, "dx")
+    near(dw, dws, mw, max(counts) + 1, "dw")
+    assert float(y[:first].abs().sum()) == 0.0 and float(dx[:first].abs().sum()) == 0.0
+    return plan.describe()
+
+
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("counts,skip,width,out", [
+    ([5, 3, 0, 9], 1, 64, 128), ([0, 17, 64, 1, 130], 2, 128, 96), ([70, 33, 5], 1, 8, 8), ([300, 5, 70], 1, 33, 7), ([700, 260, 1, 515], 1, 320, 512),
+    ([257, 700, 30], 1, 1000, 520), ([1] * 80, 9, 192, 320), ([2, 1, 5] * 50, 100, 64, 72), ([4, 0, 0], 1, 64, 64), ([90, 0], 2, 64, 64)])
+def test_part_of_the_experts(counts, skip, width, out, gather):
+    if skip == len(counts):
+        counts = counts + [0]               # an expert without rows behind all rows
+    part_of_the_experts(counts, skip, width, out, torch.bfloat16, gather=gather)
+    part_of_the_experts(counts, skip, width, out, torch.float16, f8=True, gather=gather)
+
+
+@pytest.mark.parametrize("counts,skip,width,out,tile", [
+    ([9] + [1] * 8, 1, 2048, 520, "stream16x32"), ([3, 3] + [1, 2, 0, 1] * 16, 2, 1024, 1032, "stream16x64"), ([35] + [20, 31, 0, 26, 22, 24, 30, 28], 1, 1024, 4096, "stream64x64"),
+    ([200] + [30] * 60 + [0, 90, 5, 1], 1, 520, 2056, "ring64x128"), ([300] + [70] * 60 + [0, 290, 5, 1], 1, 520, 2056, "ring128x128"),
+    ([300, 500, 1, 700, 900], 1, 2056, 4104, "pingpong256x256")])
+def test_part_of_the_experts_by_each_kernel(counts, skip, width, out, tile):
+    assert "tile=" + tile in part_of_the_experts(counts, skip, width, out, torch.bfloat16)
+
+
+@pytest.mark.parametrize("counts,skip,width,out,tile", [([128, 40, 0, 100] + [41] * 61, 1, 2064, 1032, "ring64x128/2 e4m3"),
+                                                        ([500, 1500, 77, 3000, 0], 1, 1040, 2056, "pingpong256x256 e4m3")])
+def test_part_of_the_experts_by_the_e4m3_instruction(counts, skip, width, out, tile):
+    assert "tile=" + tile in part_of_the_experts(counts, skip, width, out, torch.bfloat16, f8=True)
