@@ -234,3 +234,142 @@ def test_part_of_the_experts_by_each_kernel(counts, skip, width, out, tile):
                                                         ([500, 1500, 77, 3000, 0], 1, 1040, 2056, "pingpong256x256 e4m3")])
 def test_part_of_the_experts_by_the_e4m3_instruction(counts, skip, width, out, tile):
     assert "tile=" + tile in part_of_the_experts(counts, skip, width, out, torch.bfloat16, f8=True)
+
+
+@pytest.mark.parametrize("t,e,k,width,out", [(300, 12, 3, 256, 128), (64, 6, 6, 72, 200), (500, 20, 4, 33, 17)])
+def test_gradient_of_gathered_rows_is_rounded_once(t, e, k, width, out):
+    g = gen(t)
+    mask = torch.rand(t, e, generator=g, device=DEV) > 0.2
+    r = km.route(randn(g, t, e), k, True, mask)
+    x = randn(g, t, width).bfloat16().requires_grad_(True)
+    w = (randn(g, e, out, width) * width ** -0.5).bfloat16()
+    dy = randn(g, t * k, out).bfloat16()
+    dx, = torch.autograd.grad(km.grouped_linear(x, w, r.offsets, r.rows, r.slots), x, dy)
+    _, _, dxs, mx, *_ = grouped_plain(x.detach(), w, r.offsets, r.rows, t * k, dy)
+    took = (r.slots >= 0)[:, :, None]
+    pick = lambda v: torch.where(took, v[r.slots.long().clamp_min(0)], 0.0)
+    want, terms = pick(dxs).sum(1), out + 1 + k
+    near(dx, want, pick(mx).sum(1), terms, "dx")
+    with pytest.raises(AssertionError):         # rows of 16 bits before the sum would not pass
+        near(pick(dxs).bfloat16().double().sum(1).bfloat16(), want, pick(mx).sum(1), terms, "rows rounded first")
+
+
+@pytest.mark.parametrize("counts,width,out,tile", [
+    ([40, 0, 100] + [41] * 61, 2063, 1032, "ring64x128/2 any e4m3"), ([90] * 14 + [3, 300], 2050, 2056, "ring128x128/2 any e4m3"),
+    ([2500], 2047, 4096, "ring128x128/2 any e4m3"), ([1030], 2063, 2056, "ring64x128/2 any e4m3"), ([1500, 77, 3000, 0], 1041, 2056, "ring128x128/2 any e4m3")])
+def test_e4m3_instruction_on_rows_off_16_bytes(counts, width, out, tile):
+    """Bounds as for whole rows: the instruction drops at most 8 x 2^-13 of the largest of 8 products, on top of the f32 sums' rounding."""
+    g = gen(width + out)
+    count = sum(counts) + 3
+    offsets, rows = make_order(counts, 3, 777, g)
+    grouped = len(counts) > 1
+    x = (randn(g, 777 if grouped else count, width) * torch.exp(randn(g, 1, width))).bfloat16()
+    w, ws = make_fp8(g, len(counts), out, width)
+    xq, xs = km.quantize_rows(x)
+    plan = K.LinearFp8(K.desc(x.shape, K.BF16), K.desc([len(counts), width, out], K.F8E4M3, "ACB"), K.desc([count, out], K.BF16), None, grouped, grouped)
+    assert plan.describe().endswith("tile=" + tile), plan.describe()
+    terms = width + 3 * (width // 128 + 1) + 2.0 ** 13
+    if grouped:
+        want, mag, *_ = grouped_plain(dequant(xq, xs), dequant(w, ws, 128), offsets, rows, count)
+        ys = [km.grouped_linear_fp8(x, w, ws, offsets, rows), km.grouped_linear_fp8(xq, w, ws, offsets, rows, x_scale=xs)]
+        assert float(ys[0][sum(counts):].abs().sum()) == 0.0
+    else:
+        xd, wd = dequant(xq, xs), dequant(w[0], ws[0], 128)
+        want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+        ys = [km.linear_fp8(x, w[0], ws[0]), km.linear_fp8(xq, w[0], ws[0], x_scale=xs)]
+    assert torch.equal(*ys)
+    near(ys[0], want, mag, terms, "y")
+    assert float((ys[0].double() - want).norm() / want.norm()) < 2.0 ** -9
+
+
+WIDE = 1 << 20      # a row pitch of which some 4000 rows of 16 bits span 8 GB
+
+
+@pytest.fixture(scope="module")
+def room():
+    """10 GB that operands with wide pitches lie in; what lies between their elements holds anything."""
+    buffer = torch.empty(5 << 30, dtype=torch.bfloat16, device=DEV)
+    yield buffer
+    buffer.untyped_storage().resize_(0)
+    torch.cuda.empty_cache()
+
+
+def spread(room, values, *pitches):
+    v = room.view(values.dtype) if values.element_size() == 2 else room.view(torch.uint8).view(values.dtype)
+    at = torch.as_strided(v, values.shape, (*pitches, 1), 8)
+    at.copy_(values)
+    return at
+
+
+@pytest.mark.parametrize("count", [200, 2100])
+def test_offsets_past_32_bits_in_x_and_y(room, count):
+    g = gen(count)
+    x = spread(room, randn(g, 4200, 64).bfloat16(), WIDE + 8)
+    counts = [count // 3, 0, count // 2]
+    offsets, rows = make_order(counts, 5, 4200, g)
+    rows[:3] = torch.tensor([4199, 0, 4198], dtype=torch.int32)
+    total = sum(counts) + 5
+    w = (randn(g, 3, 96, 64) / 8).bfloat16()
+    dy = randn(g, total, 96).bfloat16()
+    want, my, _, _, dw, mw = grouped_plain(x.contiguous(), w, offsets, rows, total, dy)
+    near(km.grouped_linear(x, w, offsets, rows), want, my, 65, "y")
+    wr = w.detach().requires_grad_(True)
+    near(torch.autograd.grad(km.grouped_linear(x, wr, offsets, rows), wr, dy)[0], dw, mw, total, "dw")
+    # rows of x in order, and of y: each tile's base is past 32 bits
+    xs = spread(room, randn(g, total, 64).bfloat16(), 2 * WIDE + 8)
+    near(km.grouped_linear(xs, w, offsets), *grouped_plain(xs.contiguous(), w, offsets, None, total)[:2], 65)
+    y = spread(room, torch.zeros(total, 96).bfloat16(), 2 * WIDE + 8)
+    dense = randn(g, total, 64).bfloat16()
+    K.GroupedLinear(K.desc(dense.shape, K.BF16), K.desc([3, 64, 96], K.BF16, "ACB"), K.desc(y.shape, K.BF16, "AB", y.stride())).run(
+        dense, w, offsets, None, y, torch.cuda.current_stream())
+    near(y, *grouped_plain(dense, w, offsets, None, total)[:2], 65)
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 0, 50], [300, 500, 200]])
+def test_offsets_past_32_bits_in_weights(room, counts):
+    g = gen(sum(counts))
+    offsets, _ = make_order(counts, 0, 1, g)
+    total = sum(counts)
+    x, dy = randn(g, total, 64).bfloat16(), randn(g, total, 300).bfloat16()
+    for pitches, e in (((300 * (1 << 23), 1 << 23), 2), (((5 << 30) // 3 // 8 * 8 - 64 * 300, 64), 3)):     # far rows, far experts
+        w = spread(room, (randn(g, e, 300, 64) / 8).bfloat16(), *pitches)
+        mine = torch.cat([offsets[:e], offsets[-1:]]) if e == 3 else torch.cat([offsets[:2], offsets[-1:]])
+        xr, wr = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = km.grouped_linear(xr, wr, mine)
+        want, my, dxs, mx, dw, mw = grouped_plain(x, w.contiguous(), mine, None, total, dy)
+        near(y.detach(), want, my, 65, "y")
+        dx, = torch.autograd.grad(y, xr, dy)
+        near(dx, dxs, mx, 301, "dx")
+    w, ws = make_fp8(g, 3, 300, 128)
+    far = spread(room, w, (10 << 30) // 3 // 16 * 16 - 128 * 300, 128)
+    x = randn(g, total, 128).bfloat16()
+    assert torch.equal(km.grouped_linear_fp8(x, far, ws, offsets), km.grouped_linear_fp8(x, w, ws, offsets))
+
+
+def test_offsets_past_32_bits_in_8_bit_rows_logits_and_sums(room):
+    g = gen(5)
+    x = randn(g, 4200, 128).bfloat16()
+    w, ws = make_fp8(g, 1, 264, 128)
+    xq, xs = km.quantize_rows(x)
+    for m in (4200, 40):                       # of one weight: the last rows alone as well
+        far = spread(room, xq, 2 * WIDE + 16)[4200 - m:]
+        want = km.linear_fp8(xq[4200 - m:].contiguous(), w[0], ws[0], x_scale=xs[4200 - m:], out_dtype=torch.float32)
+        mag = dequant(xq, xs)[4200 - m:].abs() @ dequant(w[0], ws[0], 128).abs().t()
+        near(km.linear_fp8(far, w[0], ws[0], x_scale=xs[4200 - m:], out_dtype=torch.float32), want.double(), 2 * mag, 140)
+    far = spread(room, x, WIDE + 8)
+    q, s = km.quantize_rows(far)
+    assert torch.equal(q.view(torch.uint8), xq.view(torch.uint8)) and torch.equal(s, xs)
+    rows = torch.randint(0, 4200, (500,), generator=g, device=DEV, dtype=torch.int32)
+    offsets = torch.tensor([0, 500], dtype=torch.int32, device=DEV)
+    far8 = spread(room, xq, 2 * WIDE + 16)
+    xd, wd = dequant(xq, xs)[rows.long()], dequant(w[0], ws[0], 128)
+    near(km.grouped_linear_fp8(far8, w, ws, offsets, rows, xs, torch.float32), xd @ wd.t(), xd.abs() @ wd.abs().t(), 140, "gathered")
+    logits = randn(g, 4200, 60).bfloat16()
+    a, b = km.route(spread(room, logits, WIDE + 8), 4, False), km.route(logits, 4, False)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    slots = torch.randperm(4200, generator=g, device=DEV).int().reshape(2100, 2)
+    weights, dout = randn(g, 2100, 2), randn(g, 2100, 128).bfloat16()
+    y = spread(room, x, WIDE + 8)
+    assert torch.equal(km.combine(y, weights, slots), km.combine(x, weights, slots))
+    wr = weights.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(km.combine(y, wr, slots), wr, dout)[0], torch.autograd.grad(km.combine(x, wr, slots), wr, dout)[0])
