@@ -373,3 +373,25 @@ def test_offsets_past_32_bits_in_8_bit_rows_logits_and_sums(room):
     assert torch.equal(km.combine(y, weights, slots), km.combine(x, weights, slots))
     wr = weights.clone().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(km.combine(y, wr, slots), wr, dout)[0], torch.autograd.grad(km.combine(x, wr, slots), wr, dout)[0])
+
+
+def test_layers_in_graphs():
+    """Whole layers, captured at a size that no call had before and replayed between eager calls on other values."""
+    g = gen(23)
+    layer = km.MoEMlp(264, 200, 10, 3, device=DEV)
+    served = layer.quantized()
+    static = randn(g, 90, 264).bfloat16()
+    mask = torch.ones(90, dtype=torch.bool, device=DEV)
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = layer(static, mask), served(static, mask)
+        for i in range(3):
+            x, m = randn(g, 90, 264).bfloat16(), torch.rand(90, generator=g, device=DEV) > 0.3
+            eager = layer(x, m), served(x, m)
+            torch.cuda.synchronize()
+            static.copy_(x)
+            mask.copy_(m)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(eager, captured))
