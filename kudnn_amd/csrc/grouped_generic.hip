@@ -1,7 +1,8 @@
 // Grouped products of any sizes, pitches and alignments: 64 x 64 tiles, the operands read one element at a time.
 //
-// This is the kernel behind every form for operands that are not whole 16-byte pieces. A workgroup of four waves holds
-// a 64 x 64 tile of C, each wave a 32 x 32 quarter in four 16 x 16 MFMA accumulators; 32 of the summed index at a time pass
+// This is the kernel behind every form for what the others leave: rows of less than 16 bytes, operands past 32-bit offsets, and gradients of
+// misaligned bases or more than 65535 experts (other rows off 16-byte chunks pass through registers in the forward products and are packed for
+// the gradients). A workgroup of four waves holds a 64 x 64 tile of C, each wave a 32 x 32 quarter in four 16 x 16 MFMA accumulators; 32 of the summed index at a time pass
 // through LDS, masked to the operand's bounds. e4m3 values are widened to bf16, which holds them exactly; their products are
 // summed within a block of 128 and then scaled into the running sum.
 // Bound by the element-wise copies: the index arithmetic of 16 elements a thread and step outweighs its MFMAs (16384 rows of 32

@@ -6,7 +6,7 @@
 // line of consecutive lanes; rows that are not whole 16-byte pieces take the same kernel with one element a thread.
 // Sums over j run in j's order and dot products in a fixed tree, so results do not depend on timing.
 // What passes through once is read and written non-temporally: 8192 tokens x 4 rows of 4096 bf16 take 60 us forward
-// (335 MB, 5.6 TB/s; 73 us with cached accesses) and 116 us backward (604 MB, 5.2 TB/s), where a plain copy of 2 GiB reaches 4.9
+// (335 MB, 5.6 TB/s; 73 us with cached accesses) and 112 us backward (604 MB, 5.4 TB/s), where a plain copy of 2 GiB reaches 4.9
 // TB/s.
 #include "device_common.h"
 #include "moe.h"
@@ -113,8 +113,8 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a)
 
 // Rows of dy that no slot names are zero: workgroup `id` of `1 << shift` has the rows r with r % (1 << shift) == id, marks in LDS those that
 // are named, and clears the others. Rows are dealt in turn, since a router leaves its unused rows together at the end. These workgroups
-// start first and read under the others' traffic: 8192 x 4 rows of 4096 bf16 with 0, a 16th and half of the tokens without experts take 116, 111
-// and 89 us (130, 231 and 956 where one workgroup counted the slots and cleared the rows past the count).
+// start first and read under the others' traffic: 8192 x 4 rows of 4096 bf16 with 0, a 16th and half of the tokens without experts take 112, 110
+// and 85 us (130, 231 and 956 where one workgroup counted the slots and cleared the rows past the count).
 constexpr int kMarks = 131072;       // rows of a workgroup that one reading of the slots can mark: 2^25 rows of y in one
 
 template <int DT, int VEC>
